@@ -10,6 +10,7 @@
 #include "dense.cuh"
 #include "assign_tc.cuh"
 #include "prefill.cuh"
+#include "packed_attn.cuh"
 
 #include <map>
 #include <mutex>
@@ -388,9 +389,9 @@ static PfEncodeFn pf_encoder() {
 // dim's position.  HOKV_ERR_UNSUPPORTED when the strides do not nest.
 static int pf_tensor_map(CUtensorMap* m, const void* base, int dtype, int dim, int64_t tokens, int64_t ss,
                          int64_t heads, int64_t sh, int64_t batch, int64_t sb, int box_rows, int* slot_t,
-                         int* slot_h, int* slot_b) {
+                         int* slot_h, int* slot_b, const char* what = "prefill_attention") {
   PfEncodeFn enc = pf_encoder();
-  if (!enc) return fail(HOKV_ERR_CUDA, "prefill_attention: cuTensorMapEncodeTiled unavailable");
+  if (!enc) return fail(HOKV_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", what);
   int64_t ext[3] = {tokens, heads, batch}, str[3] = {ss, sh, sb};
   int order[3] = {0, 1, 2};
   for (int i = 0; i < 3; ++i)   // ascending stride; extent-1 dims last
@@ -408,7 +409,7 @@ static int pf_tensor_map(CUtensorMap* m, const void* base, int dtype, int dim, i
     int64_t s = str[d];
     if (ext[d] == 1) s = need;
     if (s < need)
-      return fail(HOKV_ERR_UNSUPPORTED, "prefill_attention: strides (%lld, %lld, %lld) do not nest",
+      return fail(HOKV_ERR_UNSUPPORTED, "%s: strides (%lld, %lld, %lld) do not nest", what,
                   (long long)ss, (long long)sh, (long long)sb);
     gstr[i] = (cuuint64_t)s * 2;
     need = s * ext[d];
@@ -423,7 +424,7 @@ static int pf_tensor_map(CUtensorMap* m, const void* base, int dtype, int dim, i
                          4, const_cast<void*>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(HOKV_ERR_UNSUPPORTED, "prefill_attention: tensor map encode failed (%d)", (int)r);
+  if (r != CUDA_SUCCESS) return fail(HOKV_ERR_UNSUPPORTED, "%s: tensor map encode failed (%d)", what, (int)r);
   return HOKV_OK;
 }
 
@@ -898,5 +899,220 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
 #undef HOKV_PF
 }
 
+
+}  // extern "C"
+
+// ---- packed-batch attention ---------------------------------------------------
+namespace hokv {
+
+static inline size_t pa_up(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// CTAs of the packed attention: one per SM.
+static int pa_ctas() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return std::min(sms, 240);   // the piece lists of the combine kernels hold 256
+}
+
+// Workspace layout (offsets in bytes; total in `bytes`).
+struct PaWs {
+  size_t desc, ml, o, info, row_ml, row_o, bytes;
+};
+static PaWs pa_ws(const hokv_packed_args* a, int ctas) {
+  PaWs w;
+  const size_t dp = a->head_dim <= 64 ? 64 : 128;
+  size_t at = 0;
+  w.desc = at;
+  at += pa_up((size_t)ctas * 2 * sizeof(PaDesc));
+  w.ml = at;
+  at += pa_up((size_t)ctas * 2 * 256 * 8);
+  w.o = at;
+  at += pa_up((size_t)ctas * 2 * 256 * dp * 4);
+  w.info = w.row_ml = w.row_o = at;
+  if (a->prefix_len > 0) {
+    at += pa_up(2 * (size_t)a->n_tokens * a->kv_heads * 8);
+    w.row_ml = at;
+    at += pa_up(2 * (size_t)a->n_tokens * a->q_heads * 8);
+    w.row_o = at;
+    at += pa_up(2 * (size_t)a->n_tokens * a->q_heads * dp * 4);
+  }
+  w.bytes = at;
+  return w;
+}
+
+static int pa_check(const hokv_packed_args* a) {
+  HOKV_REQUIRE(a->n_seqs >= 0 && a->n_tokens >= 0 && a->n_tokens < (1ll << 30) && a->n_seqs < (1 << 30),
+               "packed_attention: n_seqs=%d n_tokens=%lld", a->n_seqs, (long long)a->n_tokens);
+  HOKV_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads % a->kv_heads == 0 && a->kv_heads <= 65535,
+               "packed_attention: q_heads=%d kv_heads=%d", a->q_heads, a->kv_heads);
+  if (a->q_heads / a->kv_heads > PA_ROWS)
+    return fail(HOKV_ERR_UNSUPPORTED, "packed_attention: %d query heads per KV head (at most %d)",
+                a->q_heads / a->kv_heads, PA_ROWS);
+  if (a->dtype != HOKV_F16 && a->dtype != HOKV_BF16)
+    return fail(HOKV_ERR_UNSUPPORTED, "packed_attention: dtype %d (f16 and bf16 only)", a->dtype);
+  if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8)
+    return fail(HOKV_ERR_UNSUPPORTED, "packed_attention: head_dim %d (multiples of 8 up to 128 only)", a->head_dim);
+  HOKV_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "packed_attention: scale %g must be positive and finite", a->scale);
+  HOKV_REQUIRE(a->kv_rows >= 0 && a->kv_rows < (1ll << 30) && a->prefix_len >= 0 && a->prefix_len < (1ll << 30),
+               "packed_attention: kv_rows=%lld prefix_len=%lld", (long long)a->kv_rows, (long long)a->prefix_len);
+  return HOKV_OK;
+}
+
+template <int D, typename T>
+static int launch_packed(const PaMaps& maps, const PaP& p, cudaStream_t st) {
+  if (int e = ensure_smem(k_packed_attn<D, T>, PaGeo<D>::SMEM)) return e;
+  k_packed_attn<D, T><<<p.n_ctas, PA_THREADS, PaGeo<D>::SMEM, st>>>(maps, p);
+  if (int e = check_launch("k_packed_attn")) return e;
+  // the combine starts behind the last CTAs of the attention (programmatic launch; it waits for the grid's results)
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  if (p.prefix > 0) {
+    cfg.gridDim = dim3((unsigned)p.T, (unsigned)p.Hkv);
+    cfg.blockDim = dim3(128);
+    e = cudaLaunchKernelEx(&cfg, k_packed_combine_rows<D, T>, p);
+  } else {
+    const int64_t most = std::min<int64_t>(p.T, 2 * p.TT) * p.G * (p.D / 4);   // elements of the largest item
+    cfg.gridDim = dim3((unsigned)p.n_ctas, (unsigned)std::min<int64_t>(8, cdiv(most, 256)));
+    cfg.blockDim = dim3(256);
+    e = cudaLaunchKernelEx(&cfg, k_packed_combine<D, T>, p);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(HOKV_ERR_CUDA, "k_packed_combine launch: %s", cudaGetErrorString(e));
+  }
+  return check_launch("k_packed_combine");
+}
+
+static int packed_attention(const hokv_packed_args* a, void* stream) {
+  HOKV_REQUIRE(a, "packed_attention: null arguments");
+  if (int e = pa_check(a)) return e;
+  if (a->n_tokens == 0) return HOKV_OK;
+  HOKV_REQUIRE(a->q && a->out, "packed_attention: null pointer");
+  HOKV_REQUIRE(a->cu_seqlens_q || a->n_tokens == a->n_seqs,
+               "packed_attention: %lld tokens for %d sequences of one token", (long long)a->n_tokens, a->n_seqs);
+  HOKV_REQUIRE(a->kv_in_slots ? a->kv_len != nullptr : a->cu_seqlens_k != nullptr,
+               "packed_attention: null key lengths");
+  const int64_t rows_k = a->kv_in_slots ? a->kv_rows * a->n_seqs : a->kv_rows;
+  HOKV_REQUIRE(rows_k == 0 || (a->k && a->v), "packed_attention: null pointer");
+  HOKV_REQUIRE(a->prefix_len == 0 || (a->prefix_k && a->prefix_v), "packed_attention: null prefix pointer");
+  const int64_t st[16] = {a->q_stride_t, a->q_stride_h, a->out_stride_t, a->out_stride_h, a->k_stride_t, a->k_stride_h,
+                          a->k_stride_b, a->v_stride_t, a->v_stride_h, a->v_stride_b, a->pk_stride_t, a->pk_stride_h,
+                          a->pv_stride_t, a->pv_stride_h, 0, 0};
+  for (int i = 0; i < 14; ++i)
+    HOKV_REQUIRE(st[i] % 8 == 0 && st[i] >= 0, "packed_attention: stride %lld not a multiple of 8 elements",
+                 (long long)st[i]);
+  HOKV_REQUIRE(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) &&
+                   aligned(a->prefix_k, 16) && aligned(a->prefix_v, 16),
+               "packed_attention: pointers must be 16-byte aligned");
+  const int ctas = pa_ctas();
+  if (ctas < 1) return fail(HOKV_ERR_CUDA, "packed_attention: no device");
+  const PaWs ws = pa_ws(a, ctas);
+  if (!a->workspace || a->workspace_bytes < ws.bytes || !aligned(a->workspace, 16))
+    return fail(HOKV_ERR_WORKSPACE, "packed_attention: workspace of %zu bytes (16-byte aligned) needed, got %zu", ws.bytes,
+                a->workspace ? a->workspace_bytes : (size_t)0);
+  PaP p = {};
+  PaMaps maps;
+  p.G = a->q_heads / a->kv_heads;
+  p.TT = PA_ROWS / p.G;
+  p.D = a->head_dim;
+  const int64_t T = a->n_tokens;
+  // queries as (dim, head in group, KV head, token): a box is TT tokens x G heads, token-major rows
+  {
+    const int64_t need_t = (int64_t)a->q_heads * (a->q_heads > 1 ? a->q_stride_h : a->head_dim);
+    HOKV_REQUIRE(a->q_heads == 1 || a->q_stride_h >= a->head_dim, "packed_attention: query heads overlap");
+    HOKV_REQUIRE(T == 1 || a->q_stride_t >= need_t, "packed_attention: the query's token stride %lld must cover its heads (%lld)",
+                 (long long)a->q_stride_t, (long long)need_t);
+    PfEncodeFn enc = pf_encoder();
+    if (!enc) return fail(HOKV_ERR_CUDA, "packed_attention: cuTensorMapEncodeTiled unavailable");
+    const int64_t sh = a->q_heads > 1 ? a->q_stride_h : a->head_dim, stt = T > 1 ? a->q_stride_t : need_t;
+    cuuint64_t gdim[4] = {(cuuint64_t)p.D, (cuuint64_t)p.G, (cuuint64_t)a->kv_heads, (cuuint64_t)T};
+    cuuint64_t gstr[3] = {(cuuint64_t)sh * 2, (cuuint64_t)(sh * p.G) * 2, (cuuint64_t)stt * 2};
+    cuuint32_t es[4] = {1, 1, 1, 1}, bx[4] = {64, (cuuint32_t)p.G, 1, (cuuint32_t)p.TT};
+    const CUresult r =
+        enc(&maps.q, a->dtype == HOKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(a->q), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return fail(HOKV_ERR_UNSUPPORTED, "packed_attention: query tensor map encode failed (%d)", (int)r);
+  }
+  const bool keys = rows_k > 0;   // without a single key row the maps are never used
+  if (keys) {
+    const int64_t nb = a->kv_in_slots ? a->n_seqs : 1;
+    if (int e = pf_tensor_map(&maps.k, a->k, a->dtype, p.D, a->kv_rows, a->k_stride_t, a->kv_heads, a->k_stride_h, nb,
+                              a->k_stride_b, PA_BN, &p.k_t, &p.k_h, &p.k_b, "packed_attention"))
+      return e;
+    if (int e = pf_tensor_map(&maps.v, a->v, a->dtype, p.D, a->kv_rows, a->v_stride_t, a->kv_heads, a->v_stride_h, nb,
+                              a->v_stride_b, PA_BN, &p.v_t, &p.v_h, &p.v_b, "packed_attention"))
+      return e;
+  } else {
+    maps.k = maps.v = maps.q;
+    p.k_t = p.v_t = 1; p.k_h = p.v_h = 2; p.k_b = p.v_b = 3;
+  }
+  if (a->prefix_len > 0) {
+    if (int e = pf_tensor_map(&maps.pk, a->prefix_k, a->dtype, p.D, a->prefix_len, a->pk_stride_t, a->kv_heads,
+                              a->pk_stride_h, 1, 0, PA_BN, &p.pk_t, &p.pk_h, &p.pk_b, "packed_attention"))
+      return e;
+    if (int e = pf_tensor_map(&maps.pv, a->prefix_v, a->dtype, p.D, a->prefix_len, a->pv_stride_t, a->kv_heads,
+                              a->pv_stride_h, 1, 0, PA_BN, &p.pv_t, &p.pv_h, &p.pv_b, "packed_attention"))
+      return e;
+  } else {
+    maps.pk = maps.pv = maps.q;
+  }
+  p.out = a->out;
+  p.ost = a->out_stride_t;
+  p.osh = a->out_stride_h;
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_k = a->kv_in_slots ? nullptr : a->cu_seqlens_k;
+  p.kv_len = a->kv_in_slots ? a->kv_len : nullptr;
+  p.n_seqs = a->n_seqs;
+  p.T = (int)T;
+  p.Hq = a->q_heads;
+  p.Hkv = a->kv_heads;
+  p.kv_rows = keys ? a->kv_rows : 0;
+  p.prefix = (int)a->prefix_len;
+  p.causal = a->causal ? 1 : 0;
+  p.zero_tail = a->zero_tail ? 1 : 0;
+  p.n_ctas = ctas;
+  p.sl2 = a->scale * PA_LOG2E;
+  unsigned char* w = reinterpret_cast<unsigned char*>(a->workspace);
+  p.desc = reinterpret_cast<PaDesc*>(w + ws.desc);
+  p.ml = reinterpret_cast<float2*>(w + ws.ml);
+  p.o = reinterpret_cast<float4*>(w + ws.o);
+  p.tok_info = reinterpret_cast<int2*>(w + ws.info);
+  p.row_ml = reinterpret_cast<float2*>(w + ws.row_ml);
+  p.row_o = reinterpret_cast<float4*>(w + ws.row_o);
+  if (p.D <= 64)
+    return a->dtype == HOKV_F16 ? launch_packed<64, __half>(maps, p, S(stream))
+                                : launch_packed<64, __nv_bfloat16>(maps, p, S(stream));
+  return a->dtype == HOKV_F16 ? launch_packed<128, __half>(maps, p, S(stream))
+                              : launch_packed<128, __nv_bfloat16>(maps, p, S(stream));
+}
+}  // namespace hokv
+
+extern "C" {
+
+int hokv_packed_attention_workspace_size(const hokv_packed_args* a, size_t* bytes) {
+  HOKV_REQUIRE(a && bytes, "packed_attention_workspace_size: null pointer");
+  if (int e = pa_check(a)) return e;
+  const int ctas = pa_ctas();
+  if (ctas < 1) return fail(HOKV_ERR_CUDA, "packed_attention_workspace_size: no device");
+  *bytes = pa_ws(a, ctas).bytes;
+  return HOKV_OK;
+}
+
+int hokv_packed_attention(const hokv_packed_args* a, void* stream) {
+  try {
+    return packed_attention(a, stream);
+  } catch (...) {   // an allocation of the host library failed; nothing may unwind into C
+    return fail(HOKV_ERR_CUDA, "packed_attention: host failure");
+  }
+}
 
 }  // extern "C"

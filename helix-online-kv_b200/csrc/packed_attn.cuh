@@ -1,0 +1,748 @@
+// packed_attn.cuh -- exact attention of a packed batch: whole prompts, chunks
+// of prompts and single tokens of many sequences in one launch, K/V packed or
+// in slots, optionally behind a prefix that all sequences share.
+//
+// For sequence b with nq query tokens and n keys, query i of head h:
+//   out = sum_j w_j V_j / sum_j w_j,  w_j = exp(scale q . K_j),
+// over the keys j it may see (causal: j <= n - nq + i; else all n), and, with
+// a shared prefix, over all prefix keys too.  A query that sees no key gives 0.
+//
+// Rows.  A tile has 128 rows = TMEM lanes: TT = 128 / G tokens times the G
+// query heads of one KV head (row = token * G + head in group), so K and V are
+// read once for the group and a single token still fills G rows.  An item is
+// (up to 2 TT query tokens, one KV head) against its key tiles of 128 tokens.
+//
+// Work split.  Lengths live on the device only; every CTA derives the same
+// schedule from them.  An item costs PA_ITEM units plus 2 per key tile (1 when
+// its tokens fit one 128-row tile); the units of all items form one line,
+// (sequence, token pair, KV head) in order, which the CTAs (one per SM) cut
+// into equal shares.  An item cut by a share's border leaves pieces (running
+// maximum, sum and unnormalised output, fp32) in the workspace, which
+// k_packed_combine joins in CTA order: no atomics, the same result each run.
+//
+// One CTA, 384 threads: warps 0-3 and 4-7 are the softmax of tile slots 0 and
+// 1 (a thread owns a row), warp 8 loads (TMA), warp 9 issues the MMAs, warp
+// 10 walks the schedule into a ring of item descriptors.  A two-tile item
+// gives each slot one query tile and every key tile; a one-tile item gives
+// both slots the same query rows and every other key tile, joined in
+// registers at the end, so the tensor cores and the exponentials overlap for
+// single tokens too.  Per slot and key tile:
+//   S = Q K^T    tcgen05.mma kind::f16 into 128 fp32 TMEM columns
+//   P = 2^(S scale log2 e - m)   one thread per row, rounded to the input
+//                type and written over S in tensor memory (64 columns)
+//   O += P V     tcgen05.mma with P as the tensor-memory A operand
+// The running maximum m is raised only when it grows by more than 8 (log2
+// units): P stays below 2^8, and normalising by the same m is exact.  P is
+// rounded to the input type because the tensor cores multiply in it (half a
+// step of that type relative to each weight); sums, maxima and O are fp32.
+//
+// Rows behind a sequence's end: their scores are masked by selection (any bit
+// pattern, NaN included, drops out), and the V rows of the last, partial
+// 16-token step are zeroed in shared memory before the product, steps past it
+// are not issued.
+#pragma once
+#include "packed_schedule.cuh"
+#include "prefill.cuh"
+
+namespace hokv {
+
+constexpr int PA_THREADS = 384;
+constexpr int PA_ROWS = 128;        // rows of a tile
+constexpr int PA_QUEUE = 4;         // item descriptors in flight
+constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;   // 256 * 208 + 128 * 88 = 384 * 168
+constexpr float PA_LOG2E = 1.4426950408889634f;
+
+template <int D>
+struct PaGeo {
+  static constexpr int NB = D / 64;                       // 64-dim column blocks
+  static constexpr int Q_BYTES = PA_ROWS * D * 2;         // one query tile
+  static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
+  static constexpr int STAGES = D == 64 ? 8 : 5;          // ring of K and V tiles
+  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + 2048;
+};
+
+// Piece descriptors of a CTA: [0] the piece that continues an earlier CTA's
+// item, [1] the piece that begins an item it does not finish.
+struct PaDesc {
+  int valid, end, tok0, n_tok, hk, pad[3];
+};
+
+struct alignas(64) PaMaps {
+  CUtensorMap q, k, v, pk, pv;
+};
+
+struct PaP : PaSched {
+  void* out;
+  int64_t ost, osh;              // output element strides (token, head)
+  int Hq, G, D, zero_tail;
+  float sl2;                     // scale * log2(e)
+  int k_t, k_h, k_b, v_t, v_h, v_b, pk_t, pk_h, pk_b, pv_t, pv_h, pv_b;   // coordinate slots of the maps
+  PaDesc* desc;                  // [n_ctas][2]
+  float2* ml;                    // [n_ctas][2][256] (running maximum, sum)
+  float4* o;                     // [n_ctas][2][D / 4][256]
+  int2* tok_info;                // prefix only: [2][T][Hkv] (first CTA or -1: row-wise, token in item)
+  float2* row_ml;                // prefix only: [2][T][Hq]
+  float4* row_o;                 // prefix only: [2][T][Hq][D / 4]
+};
+
+// ---- barriers ----------------------------------------------------------------
+
+// Bounded wait of every calling thread; the first that gives up marks the CTA
+// aborted, and every other wait of the CTA then ends too.
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
+  const uint32_t a = smem_u32(bar);
+  const uint32_t hint_ns = 20000u;
+  unsigned long long t0 = 0;
+  for (int i = 0;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(hint_ns)
+        : "memory");
+    if (done) return true;
+    if (*abort_flag) return false;
+    if (i == 0) {
+      t0 = global_ns();
+    } else if (global_ns() - t0 > TC_WAIT_NS) {
+      if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void pa_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// kind::f16 MMA with A in tensor memory (16-bit pairs per column).
+__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc,
+                                            int accumulate) {
+  const uint32_t no_mask = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(no_mask));
+}
+
+// 32 packed columns of this thread's lane into tensor memory, without waiting.
+__device__ __forceinline__ void tmem_st32_nw(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- the kernel ----------------------------------------------------------------
+
+template <int D, typename T>
+__global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_constant__ PaMaps maps, const PaP p) {
+  using PG = PaGeo<D>;
+  constexpr int ST = PG::STAGES;
+  constexpr int BF = std::is_same<T, __half>::value ? 0 : 1;
+  extern __shared__ __align__(1024) unsigned char pa_smem[];
+  unsigned char* sQ = pa_smem;
+  unsigned char* sKV = sQ + 2 * PG::Q_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + ST * PG::KV_BYTES);
+  uint64_t* q_full = bars;                 // TMA bytes
+  uint64_t* q_empty = bars + 1;            // MMA commit after the item's last S
+  uint64_t* s_full = bars + 2;             // [2] MMA commit
+  uint64_t* p_full = bars + 4;             // [2] 4 softmax warps
+  uint64_t* o_full = bars + 6;             // [2] MMA commit after the item's last P V
+  uint64_t* o_empty = bars + 8;            // [2] 4 softmax warps: O read
+  uint64_t* it_full = bars + 10;           // [PA_QUEUE] scheduler
+  uint64_t* it_empty = it_full + PA_QUEUE; // [PA_QUEUE] load + MMA + 8 softmax warps
+  uint64_t* kv_full = it_empty + PA_QUEUE; // [ST] TMA bytes
+  uint64_t* kv_empty = kv_full + ST;       // [ST] MMA commit
+  uint64_t* ml_full = kv_empty + ST;       // 4 warps of slot 1: (m, l) in shared memory
+  PaItem* queue = reinterpret_cast<PaItem*>(bars + 40);                     // [PA_QUEUE]
+  uint32_t* ctl = reinterpret_cast<uint32_t*>(queue + PA_QUEUE);            // [0] tmem base, [1] abort
+  float2* s_ml = reinterpret_cast<float2*>(bars + 72);                      // [128] slot 1's (m, l)
+  volatile uint32_t* abort_flag = &ctl[1];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(ctl)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(ml_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
+    }
+    for (int i = 0; i < PA_QUEUE; ++i) {
+      mbar_init(&it_full[i], 1);
+      mbar_init(&it_empty[i], 10);
+    }
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    ctl[1] = 0u;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl[0];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int TT = p.TT, G = p.G;
+
+  if (warp < 8) {
+    // ---- softmax of tile slot sl, one row per thread ----------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
+    const int sl = warp >> 2, row = tid & 127;
+    const int row_tok = row / G, row_g = row - row_tok * G;
+    const int first_tok = ((warp & 3) * 32) / G;   // lowest token of this warp's rows
+    const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_sel + (uint32_t)(sl * 128);
+    const uint32_t o_addr = tmem + lane_sel + (uint32_t)(256 + sl * 128);
+    unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int qi = it % PA_QUEUE;
+      if (!pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag)) break;
+      const PaItem w = queue[qi];
+      __syncwarp();
+      if (lane == 0) pa_arrive(&it_empty[qi]);
+      if (w.out_mode == PA_STOP) break;
+      const bool two = w.n_tok > TT;
+      const int n = w.j1 - w.j0;
+      const int mine = two ? n : (sl == 0 ? (n + 1) >> 1 : n >> 1);   // key tiles of this slot
+      const int tok = (two ? sl * TT : 0) + row_tok;                  // this row's token in the item
+      const bool row_ok = row_tok < TT && tok < w.n_tok;
+      const int lim = min(w.kv_len, w.pos0 + tok + 1);                // keys this row sees
+      const int wtok = (two ? sl * TT : 0) + first_tok;
+      const bool warp_ok = first_tok < TT && wtok < w.n_tok;          // any row of the warp in use
+      const int wlim = min(w.kv_len, w.pos0 + wtok + 1);              // least such limit of the warp
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < mine; ++i) {
+        const int t0 = (w.j0 + (two ? i : 2 * i + sl)) * PA_BN;
+        if (!pa_wait(&s_full[sl], s_ph, abort_flag)) { ok = false; break; }
+        s_ph ^= 1;
+        tc_fence_after();
+        if (warp_ok) {
+          float v[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, *reinterpret_cast<float(*)[32]>(&v[c * 32]));
+          tmem_wait_ld();
+          if (t0 + PA_BN > wlim) {
+            const int lm = lim - t0;
+#pragma unroll
+            for (int j = 0; j < 128; ++j) v[j] = j < lm ? v[j] : -INFINITY;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.sl2;
+          const bool grow = mt > m_run + 8.f || (m_run == -INFINITY && mt > -INFINITY);
+          const float m_new = grow ? mt : m_run;
+          if (i > 0 && __any_sync(0xffffffffu, grow)) {
+            // O was last written by this slot's previous P V, complete before this S
+            const float f = grow ? pf_ex2(m_run - m_new) : 1.f;
+            l_run *= f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32(o_addr + c * 32, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= f;
+              tmem_st32(o_addr + c * 32, o);
+            }
+          }
+          m_run = m_new;
+          const float nm = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float2 a = __ffma2_rn(make_float2(v[h * 64 + 2 * j], v[h * 64 + 2 * j + 1]), s2, n2);
+              const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
+              acc = __fadd2_rn(acc, e);
+              pk[j] = pack2<T>(e.x, e.y);
+            }
+            tmem_st32_nw(s_addr + h * 32, pk);
+          }
+          l_run += acc.x + acc.y;
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pa_arrive(&p_full[sl]);
+      }
+      if (!ok) break;
+      // ---- epilogue: O of this slot (one-tile items: slot 0 joins both) -----------
+      const bool join = !two && n > 1;
+      if (mine > 0) {
+        if (!pa_wait(&o_full[sl], o_ph, abort_flag)) break;
+        o_ph ^= 1;
+        tc_fence_after();
+      }
+      if (!two && sl == 1) {
+        if (join) {
+          s_ml[row] = make_float2(m_run, l_run);
+          __syncwarp();
+          if (lane == 0) pa_arrive(ml_full);
+        }
+        continue;   // slot 0 reads O_1 and frees it
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if (join) {
+        if (!pa_wait(&o_full[1], o1_ph, abort_flag) || !pa_wait(ml_full, ml_ph, abort_flag)) break;
+        ml_ph ^= 1;
+        tc_fence_after();
+        const float2 b = s_ml[row];
+        const float mm = fmaxf(m_run, b.x);
+        f0 = m_run == -INFINITY ? 0.f : pf_ex2(m_run - mm);
+        f1 = b.x == -INFINITY ? 0.f : pf_ex2(b.x - mm);
+        m_run = mm;
+        l_run = l_run * f0 + b.y * f1;
+      }
+      if (sl == 0 && (join || (two && n > 0))) o1_ph ^= 1;   // slot 1 completed a phase too
+      const bool nothing = n == 0 || l_run == 0.f;
+      const float inv = nothing ? 0.f : 1.f / l_run;
+      const int64_t t = w.tok0 + tok;
+      const int hq = w.hk * G + row_g;
+      const int prow = (two ? sl * 128 : 0) + row;      // row in a piece
+      if (w.out_mode != PA_DIRECT && row_ok) {
+        if (w.out_mode == PA_PIECE) p.ml[(int64_t)w.out_at * 256 + prow] = make_float2(m_run, l_run);
+        else p.row_ml[((int64_t)w.src * p.T + t) * p.Hq + hq] = make_float2(m_run, l_run);
+      }
+      if (warp_ok) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (n > 0) {
+            tmem_ld32(o_addr + c * 32, o);
+            if (join) {
+              float o1[32];
+              tmem_ld32(o_addr + 128 + c * 32, o1);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = o[j] * f0 + o1[j] * f1;
+            }
+          }
+          if (nothing) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+          }
+          if (row_ok) {
+            if (w.out_mode == PA_DIRECT) {
+              T* og = reinterpret_cast<T*>(p.out) + t * p.ost + hq * p.osh;
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                if (c * 32 + j < p.D) {
+                  uint4 u;
+                  u.x = pack2<T>(o[j + 0] * inv, o[j + 1] * inv);
+                  u.y = pack2<T>(o[j + 2] * inv, o[j + 3] * inv);
+                  u.z = pack2<T>(o[j + 4] * inv, o[j + 5] * inv);
+                  u.w = pack2<T>(o[j + 6] * inv, o[j + 7] * inv);
+                  *reinterpret_cast<uint4*>(og + c * 32 + j) = u;
+                }
+              }
+            } else {
+              const bool piece = w.out_mode == PA_PIECE;
+              float4* base = piece ? p.o + ((int64_t)w.out_at * (D / 4)) * 256 + prow
+                                   : p.row_o + (((int64_t)w.src * p.T + t) * p.Hq + hq) * (D / 4);
+              const int step = piece ? 256 : 1;
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                base[(c * 8 + j / 4) * step] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            }
+          }
+        }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          pa_arrive(&o_empty[sl]);
+          if (join) pa_arrive(&o_empty[1]);
+        }
+      }
+    }
+    if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
+      const int used = pa_used(p);
+      const int64_t total = (int64_t)(p.T - used) * p.Hq * p.D;
+      for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < total; i += (int64_t)gridDim.x * 256) {
+        const int d = (int)(i % p.D);
+        const int64_t h = i / p.D % p.Hq, t = used + i / p.D / p.Hq;
+        reinterpret_cast<T*>(p.out)[t * p.ost + h * p.osh + d] = T(0.f);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
+    if (warp == 8) {
+      // ---- loads (lane 0): the item's query tiles, then K and V in the order of use ----
+      if (lane == 0) {
+        unsigned ring = 0, q_uses = 0;
+        bool ok = true;
+        for (int it = 0; ok; ++it) {
+          const int qi = it % PA_QUEUE;
+          if (!pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag)) break;
+          const PaItem w = queue[qi];
+          pa_arrive(&it_empty[qi]);
+          if (w.out_mode == PA_STOP) break;
+          const int n = w.j1 - w.j0;
+          if (n == 0) continue;
+          const bool two = w.n_tok > TT;
+          if (q_uses > 0 && !pa_wait(q_empty, (q_uses - 1) & 1, abort_flag)) break;
+          ++q_uses;
+          pf_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * PG::NB * TT * G * 128));
+          for (int t = 0; t < (two ? 2 : 1); ++t)
+#pragma unroll
+            for (int a = 0; a < PG::NB; ++a)
+              pf_tma4(sQ + t * PG::Q_BYTES + a * PA_ROWS * 128, &maps.q, a * 64, 0, w.hk, w.tok0 + t * TT, q_full);
+          const CUtensorMap* mk = w.src ? &maps.pk : &maps.k;
+          const CUtensorMap* mv = w.src ? &maps.pv : &maps.v;
+          auto load = [&](bool is_v, int j) {
+            const unsigned st = ring % ST, use = ring / ST;
+            if (use > 0 && !pa_wait(&kv_empty[st], (use - 1) & 1, abort_flag)) return false;
+            ++ring;
+            int c[4];
+            const int row = w.row0 + (w.j0 + j) * PA_BN;
+            if (is_v) pf_coords(w.src ? p.pv_t : p.v_t, w.src ? p.pv_h : p.v_h, w.src ? p.pv_b : p.v_b, row, w.hk, w.slot, c);
+            else pf_coords(w.src ? p.pk_t : p.k_t, w.src ? p.pk_h : p.k_h, w.src ? p.pk_b : p.k_b, row, w.hk, w.slot, c);
+            pf_expect_tx(&kv_full[st], PG::KV_BYTES);
+#pragma unroll
+            for (int a = 0; a < PG::NB; ++a)
+              pf_tma4(sKV + st * PG::KV_BYTES + a * PA_BN * 128, is_v ? mv : mk, a * 64, c[1], c[2], c[3], &kv_full[st]);
+            return true;
+          };
+          const int ahead = two ? 1 : 2;
+          for (int j = 0; ok && j < min(ahead, n); ++j) ok = load(false, j);
+          for (int j = 0; ok && j < n; ++j) {
+            ok = load(true, j);
+            if (ok && j + ahead < n) ok = load(false, j + ahead);
+          }
+        }
+        if (*abort_flag) {   // gave up: the copies in flight land before the CTA ends
+          for (unsigned k = ring > ST ? ring - ST : 0; k < ring; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
+          if (q_uses > 0) (void)mbar_wait(q_full, (q_uses - 1) & 1);
+        }
+      }
+    } else if (warp == 9) {
+      // ---- MMA issue (the warp waits, lane 0 issues) --------------------------------
+      const int kd = (p.D + 15) / 16;
+      const uint32_t idesc_s = umma_idesc_f16(PA_BN, BF, 0), idesc_o = umma_idesc_f16(kd * 16, BF, 1);
+      const uint32_t aQ = smem_u32(sQ), aKV = smem_u32(sKV);
+      unsigned ring = 0, q_uses = 0, p_ph[2] = {0, 0}, o_uses[2] = {0, 0};
+      bool ok = true;
+      // the next tile of the ring, once its bytes have landed
+      auto next_tile = [&]() {
+        const unsigned st = ring % ST, use = ring / ST;
+        ++ring;
+        ok = ok && pa_wait(&kv_full[st], use & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        return st;
+      };
+      auto issue_s = [&](int sl, int q, unsigned st, bool release, bool last) {   // S = Q_q K^T
+        if (lane == 0) {
+          const uint32_t a = aQ + q * PG::Q_BYTES, bk = aKV + st * PG::KV_BYTES;
+#pragma unroll
+          for (int kc = 0; kc < D / 16; ++kc)
+            if (kc < kd)
+              umma_f16(tmem + (uint32_t)(sl * 128), umma_desc_sw(a + (kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32, 16, 1024),
+                       umma_desc_sw(bk + (kc >> 2) * PA_BN * 128 + (kc & 3) * 32, 16, 1024), idesc_s, kc > 0);
+          umma_commit(&s_full[sl]);
+          if (release) umma_commit(&kv_empty[st]);
+          if (last) umma_commit(q_empty);
+        }
+        __syncwarp();
+      };
+      for (int it = 0; ok; ++it) {
+        const int qi = it % PA_QUEUE;
+        ok = pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const PaItem w = queue[qi];
+        __syncwarp();
+        if (lane == 0) pa_arrive(&it_empty[qi]);
+        if (w.out_mode == PA_STOP) break;
+        const int n = w.j1 - w.j0;
+        if (n == 0) continue;
+        const bool two = w.n_tok > TT;
+        ok = pa_wait(q_full, q_uses & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        ++q_uses;
+        if (!ok) break;
+        unsigned st = next_tile();
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(0, 0, st, !two, !two && n == 1);
+        if (two) {
+          issue_s(1, 1, st, true, n == 1);
+        } else if (n > 1) {
+          st = next_tile();
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(1, 0, st, true, n == 2);
+        }
+        for (int j = 0; ok && j < n; ++j) {
+          const unsigned sv = next_tile();
+          if (!ok) break;
+          const uint32_t bv = aKV + sv * PG::KV_BYTES;
+          const int valid = min(PA_BN, w.kv_len - (w.j0 + j) * PA_BN);
+          const int ks = (valid + 15) >> 4;
+          if (valid & 15) {   // rows behind the sequence inside its last 16-token step
+            unsigned char* tile = sKV + sv * PG::KV_BYTES;
+            const int rows = ks * 16 - valid;
+            for (int e = lane; e < rows * PG::NB * 8; e += 32) {
+              const int r = valid + e / (PG::NB * 8), c = e % (PG::NB * 8);
+              *reinterpret_cast<uint4*>(tile + (c >> 3) * PA_BN * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+            __syncwarp();
+          }
+          unsigned sk = 0;
+          for (int h = 0; h < (two ? 2 : 1); ++h) {
+            const int sl = two ? h : (j & 1);
+            const bool first = two ? j == 0 : j < 2;
+            const bool last = two ? j == n - 1 : j >= n - 2;
+            ok = pa_wait(&p_full[sl], p_ph[sl], abort_flag);
+            if (ok && first && o_uses[sl] > 0) ok = pa_wait(&o_empty[sl], (o_uses[sl] - 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            p_ph[sl] ^= 1;
+            if (first) ++o_uses[sl];
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+              for (int kc = 0; kc < PA_BN / 16; ++kc)
+                if (kc < ks)
+                  umma_f16_ta(tmem + (uint32_t)(256 + sl * 128), tmem + (uint32_t)(sl * 128 + kc * 8),
+                              umma_desc_sw(bv + kc * 2048, PA_BN * 128, 1024), idesc_o, !first || kc > 0);
+              if (last) umma_commit(&o_full[sl]);
+              if (!two || h == 1) umma_commit(&kv_empty[sv]);
+            }
+            __syncwarp();
+            const int jn = j + (two ? 1 : 2);
+            if (jn < n) {
+              if (h == 0) {
+                sk = next_tile();
+                if (!ok) break;
+                tc_fence_after();
+              }
+              issue_s(sl, two ? h : 0, sk, !two || h == 1, jn == n - 1 && (!two || h == 1));
+            }
+          }
+        }
+      }
+    } else if (warp == 10) {
+      // ---- schedule: this CTA's share of the unit line ------------------------------
+      const int n_s = pa_n_seqs(p);
+      const int per = (n_s + 31) / 32;
+      const int s_lo = min(lane * per, n_s), s_hi = min(s_lo + per, n_s);
+      int64_t mine = 0;
+      bool bad = false;
+      for (int s = s_lo; s < s_hi; ++s) {
+        const PaSeq q = pa_seq(p, s);
+        bad = bad || q.bad;
+        mine += pa_seq_units(p, q);
+      }
+      if (bad) dev_flag(HOKV_ERR_DEVICE_INPUT);
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
+      const int64_t share = pa_share(p, total);
+      const int64_t begin = min((int64_t)blockIdx.x * share, total), end = min(begin + share, total);
+      if (lane < 2) p.desc[blockIdx.x * 2 + lane].valid = 0;
+      __syncwarp();
+      int n_items = 0;
+      auto push = [&](const PaItem& w) {
+        const int qi = n_items % PA_QUEUE, use = n_items / PA_QUEUE;
+        if (use > 0 && !__all_sync(0xffffffffu, pa_wait(&it_empty[qi], (unsigned)((use - 1) & 1), abort_flag))) return false;
+        if (lane == 0) {
+          queue[qi] = w;
+          pa_arrive(&it_full[qi]);
+        }
+        __syncwarp();
+        ++n_items;
+        return true;
+      };
+      bool ok = true;
+      if (begin < end) {
+        // the sequence that holds unit `begin`, and the units before it
+        const int owner = __ffs(__ballot_sync(0xffffffffu, incl > begin)) - 1;
+        int s = 0;
+        int64_t at = 0;
+        if (lane == owner) {
+          at = incl - mine;
+          s = pa_find(p, s_lo, s_hi, begin, at);
+        }
+        s = __shfl_sync(0xffffffffu, s, owner);
+        at = __shfl_sync(0xffffffffu, at, owner);
+        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends) {
+          if (w.out_mode == PA_PIECE && lane == 0) {
+            PaDesc d;
+            d.valid = 1;
+            d.end = ends;
+            d.tok0 = w.tok0;
+            d.n_tok = w.n_tok;
+            d.hk = w.hk;
+            p.desc[w.out_at] = d;
+          }
+          if (p.prefix > 0 && begins)   // where k_packed_combine_rows finds this item's rows
+            for (int i = lane; i < w.n_tok; i += 32)
+              p.tok_info[((int64_t)w.src * p.T + w.tok0 + i) * p.Hkv + w.hk] =
+                  make_int2(ends ? -1 : (int)blockIdx.x, i);
+          return push(w);
+        });
+      }
+      if (ok) {
+        PaItem w = {};
+        w.out_mode = PA_STOP;
+        push(w);
+      }
+    }
+  }
+  // every role is done: each item's last products were awaited by its
+  // epilogue, or the CTA gave up
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ---- joining pieces ------------------------------------------------------------
+
+// Items cut by a share's border, one item per blockIdx.x (the CTA that began
+// it), its rows and 4-dim groups over blockIdx.y and the threads; the pieces
+// are added in CTA order.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) k_packed_combine(const PaP p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ int s_part[256];
+  __shared__ int s_n;
+  const PaDesc d = p.desc[blockIdx.x * 2 + 1];
+  if (!d.valid) return;
+  if (threadIdx.x < 32) {
+    // the pieces of the CTAs after this one, up to the one that ends the item
+    int n = 1;
+    if (threadIdx.x == 0) s_part[0] = blockIdx.x * 2 + 1;
+    for (int c = blockIdx.x + 1; c < p.n_ctas; c += 32) {
+      const int i = c + threadIdx.x;
+      PaDesc e;
+      e.valid = e.end = 0;
+      if (i < p.n_ctas) e = p.desc[i * 2];
+      const unsigned val = __ballot_sync(0xffffffffu, e.valid != 0);
+      const unsigned fin = __ballot_sync(0xffffffffu, e.valid && e.end);
+      const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
+      if (use >> threadIdx.x & 1) s_part[n + __popc(use & ((1u << threadIdx.x) - 1u))] = i * 2;
+      n += __popc(use);
+      if (fin) break;
+    }
+    if (threadIdx.x == 0) s_n = n;
+  }
+  __syncthreads();
+  const int n = s_n, rows = d.n_tok * p.G, groups = p.D / 4;
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < rows * groups; e += gridDim.y * 256) {
+    const int r = e % rows, d4 = e / rows;
+    const int tok = r / p.G, g = r - tok * p.G;
+    const int tile = tok / p.TT;
+    const int prow = tile * 128 + (tok - tile * p.TT) * p.G + g;
+    float m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[(int64_t)s_part[i] * 256 + prow].x);
+    float l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float2 ml = p.ml[(int64_t)s_part[i] * 256 + prow];
+      const float4 o = p.o[((int64_t)s_part[i] * (D / 4) + d4) * 256 + prow];
+      const float f = ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - m);
+      l += ml.y * f;
+      a.x += o.x * f; a.y += o.y * f; a.z += o.z * f; a.w += o.w * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* og = reinterpret_cast<T*>(p.out) + (int64_t)(d.tok0 + tok) * p.ost + (int64_t)(d.hk * p.G + g) * p.osh + d4 * 4;
+    *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+  }
+}
+
+// With a shared prefix every row joins its prefix part and its own part, each
+// one row-wise result or the pieces of a cut item.  Grid (tokens, KV heads).
+template <int D, typename T>
+__global__ void __launch_bounds__(128) k_packed_combine_rows(const PaP p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ int s_part[2][256];   // workspace slots, or -1: the row-wise result
+  __shared__ int s_n[2], s_prow[2];
+  const int t = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int used = pa_used(p);
+  if (t >= used) return;
+  if (warp < 2) {
+    int2 info = p.tok_info[((int64_t)warp * p.T + t) * p.Hkv + hk];
+    info.x = min(max(info.x, -1), p.n_ctas - 1);      // a token that no valid sequence covers has no entry
+    info.y = min(max(info.y, 0), 2 * p.TT - 1);
+    int n = 1;
+    if (info.x < 0) {
+      if (lane == 0) s_part[warp][0] = -1;
+    } else {
+      if (lane == 0) s_part[warp][0] = info.x * 2 + 1;
+      for (int c = info.x + 1; c < p.n_ctas; c += 32) {
+        const int i = c + lane;
+        PaDesc e;
+        e.valid = e.end = 0;
+        if (i < p.n_ctas) e = p.desc[i * 2];
+        const unsigned val = __ballot_sync(0xffffffffu, e.valid != 0);
+        const unsigned fin = __ballot_sync(0xffffffffu, e.valid && e.end);
+        const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
+        if (use >> lane & 1) s_part[warp][n + __popc(use & ((1u << lane) - 1u))] = i * 2;
+        n += __popc(use);
+        if (fin) break;
+      }
+    }
+    if (lane == 0) {
+      const int tile = info.y / p.TT;
+      s_n[warp] = n;
+      s_prow[warp] = tile * 128 + (info.y - tile * p.TT) * p.G;
+    }
+  }
+  __syncthreads();
+  const int groups = p.D / 4;
+  for (int e = threadIdx.x; e < p.G * groups; e += 128) {
+    const int g = e / groups, d4 = e - g * groups, hq = hk * p.G + g;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int src = 0; src < 2; ++src) {
+      const int64_t rw = ((int64_t)src * p.T + t) * p.Hq + hq;
+      const int prow = s_prow[src] + g, n = s_n[src];
+      for (int i = 0; i < n; ++i) {
+        const int at = s_part[src][i];
+        const float2 ml = at < 0 ? p.row_ml[rw] : p.ml[(int64_t)at * 256 + prow];
+        const float4 o = at < 0 ? p.row_o[rw * (D / 4) + d4] : p.o[((int64_t)at * (D / 4) + d4) * 256 + prow];
+        const float mn = fmaxf(m, ml.x);
+        const float fa = m == -INFINITY ? 0.f : pf_ex2(m - mn), fb = ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - mn);
+        l = l * fa + ml.y * fb;
+        a.x = a.x * fa + o.x * fb; a.y = a.y * fa + o.y * fb;
+        a.z = a.z * fa + o.z * fb; a.w = a.w * fa + o.w * fb;
+        m = mn;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* og = reinterpret_cast<T*>(p.out) + (int64_t)t * p.ost + (int64_t)hq * p.osh + d4 * 4;
+    *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+  }
+}
+
+}  // namespace hokv

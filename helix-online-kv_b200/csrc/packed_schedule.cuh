@@ -1,0 +1,221 @@
+// packed_schedule.cuh -- how the packed attention cuts its work over the CTAs.
+//
+// An item is up to 2 TT query tokens of one sequence and one KV head (a token
+// pair of tiles, TT = 128 / G tokens each) against the key tiles it sees.  It
+// costs PA_ITEM units plus 2 per key tile, 1 when its tokens fit one tile.  The
+// units of all items, ordered by (sequence, pair, KV head), form one line; CTA
+// c takes units [c, c + 1) * share.  A border inside an item cuts it at a key
+// tile into pieces.  The units before a pair have a closed form (a lattice
+// sum), so a CTA finds its first item without walking the others.
+//
+// Plain C++ apart from the HD marks, so the host can check the same code.
+#pragma once
+#include "hokv_math.cuh"
+
+namespace hokv {
+
+constexpr int PA_BN = 128;          // keys of a tile
+constexpr int PA_ITEM = 2;          // units of an item besides its tiles (start and epilogue)
+constexpr int PA_MIN_SHARE = 4;     // smallest share of a CTA: an item's start and two key tiles of a one-tile item
+
+enum { PA_DIRECT = 0, PA_PIECE = 1, PA_ROWWISE = 2, PA_STOP = 3 };
+
+struct PaItem {
+  int tok0, n_tok;     // query tokens [tok0, tok0 + n_tok)
+  int src;             // 0: own keys, 1: shared prefix
+  int row0, slot;      // first key row and slot of the sequence in its tensor
+  int hk;
+  int j0, j1;          // key tiles of this piece
+  int kv_len, pos0;    // token i sees keys < min(kv_len, pos0 + i + 1)
+  int out_mode;        // PA_DIRECT: final rows; PA_PIECE: workspace slot out_at; PA_ROWWISE: a result per row
+  int out_at;
+};
+
+struct PaSched {
+  const int* cu_q;               // [n_seqs + 1] or null: one token each
+  const int* cu_k;               // packed keys: [n_seqs + 1]
+  const int* kv_len;             // keys in slots: [n_seqs]
+  int n_seqs, T, Hkv, TT;
+  int64_t kv_rows;               // rows of the packed keys, or of a slot
+  int prefix;                    // shared prefix length, 0 without one
+  int causal, n_ctas;
+};
+
+struct PaSeq {
+  int q0, nq, row0, slot, kv, src, causal, bad;
+};
+
+HD int64_t pa_min(int64_t a, int64_t b) { return a < b ? a : b; }
+HD int64_t pa_max(int64_t a, int64_t b) { return a > b ? a : b; }
+
+HD int pa_n_seqs(const PaSched& p) { return p.n_seqs + (p.prefix > 0 ? 1 : 0); }
+// Query tokens that belong to a sequence.
+HD int pa_used(const PaSched& p) { return p.cu_q ? (int)pa_min(pa_max(p.cu_q[p.n_seqs], 0), p.T) : p.n_seqs; }
+
+// Sequence s of the schedule (with a prefix, 0 is the prefix against all
+// tokens).  One whose lengths do not fit the tensors is `bad` and empty, so
+// that nothing outside the buffers is read or written.
+HD PaSeq pa_seq(const PaSched& p, int s) {
+  PaSeq r;
+  r.bad = 0;
+  if (p.prefix > 0) {
+    if (s == 0) {
+      r.q0 = r.row0 = r.slot = 0;
+      r.nq = pa_used(p);
+      r.kv = p.prefix;
+      r.src = 1;
+      r.causal = 0;
+      return r;
+    }
+    s -= 1;
+  }
+  const int a = p.cu_q ? p.cu_q[s] : s, e = p.cu_q ? p.cu_q[s + 1] : s + 1;
+  bool bad = a < 0 || e < a || e > p.T;
+  r.src = 0;
+  r.causal = p.causal;
+  if (p.cu_k) {
+    const int ka = p.cu_k[s], ke = p.cu_k[s + 1];
+    bad = bad || ka < 0 || ke < ka || ke > p.kv_rows;
+    r.row0 = ka;
+    r.slot = 0;
+    r.kv = bad ? 0 : ke - ka;
+  } else {
+    r.row0 = 0;
+    r.slot = s;
+    r.kv = p.kv_len[s];
+    bad = bad || r.kv < 0 || r.kv > p.kv_rows;
+  }
+  r.q0 = bad ? 0 : a;
+  r.nq = bad ? 0 : e - a;
+  r.bad = bad;
+  return r;
+}
+
+// sum_{i < n} floor((a i + b) / 128), a and b >= 0: lattice points below a
+// line, by the Euclidean recursion.
+HD int64_t pa_floor_sum(int64_t n, int64_t a, int64_t b) {
+  int64_t m = PA_BN, ans = 0;
+  while (n > 0) {
+    ans += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return ans;
+}
+
+// Key tiles that token pair `pr` (W = 2 TT tokens) of a sequence sees.
+HD int pa_tiles(const PaSeq& s, int W, int pr) {
+  const int64_t e = s.causal ? (int64_t)s.kv - s.nq + pa_min((int64_t)(pr + 1) * W, s.nq) : s.kv;
+  return e <= 0 ? 0 : (int)((e + PA_BN - 1) / PA_BN);
+}
+
+// Units, of one KV head, of the first n pairs (none of them the last).
+HD int64_t pa_units_before(const PaSeq& s, int W, int64_t n) {
+  int64_t tiles;
+  if (!s.causal) {
+    tiles = n * ((s.kv + PA_BN - 1) / PA_BN);
+  } else {
+    const int64_t off = (int64_t)s.kv - s.nq;
+    const int64_t skip = off < 0 ? pa_min(n, -off / W) : 0;   // pairs that see nothing
+    tiles = pa_floor_sum(n - skip, W, off + (skip + 1) * W + PA_BN - 1);
+  }
+  return n * PA_ITEM + 2 * tiles;
+}
+
+// Units of one KV head's item of pair `pr`.
+HD int pa_item_units(const PaSeq& s, int W, int pr) {
+  return PA_ITEM + (s.nq - pr * W > W / 2 ? 2 : 1) * pa_tiles(s, W, pr);
+}
+
+HD int64_t pa_seq_units(const PaSched& p, const PaSeq& s) {
+  const int W = 2 * p.TT;
+  if (s.nq <= 0) return 0;
+  const int np = (s.nq + W - 1) / W;
+  return (int64_t)p.Hkv * (pa_units_before(s, W, np - 1) + pa_item_units(s, W, np - 1));
+}
+
+HD int64_t pa_share(const PaSched& p, int64_t total) {
+  return pa_max((total + p.n_ctas - 1) / p.n_ctas, PA_MIN_SHARE);
+}
+
+// The sequence of [lo, hi) that holds unit `unit`; `at`: units before lo, on
+// return before that sequence.
+HD int pa_find(const PaSched& p, int lo, int hi, int64_t unit, int64_t& at) {
+  int s = lo;
+  for (; s < hi - 1; ++s) {
+    const int64_t u = pa_seq_units(p, pa_seq(p, s));
+    if (at + u > unit) break;
+    at += u;
+  }
+  return s;
+}
+
+// CTA `cta`'s items: units [begin, end), which start in sequence s (`at` units
+// before it).  emit(item, begins, ends): whether the piece holds the item's
+// first and its last key tile; false stops the walk.
+template <typename Emit>
+HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, int64_t at, Emit emit) {
+  const int W = 2 * p.TT, n_s = pa_n_seqs(p);
+  int64_t pos = begin;
+  for (; s < n_s && pos < end; ++s) {
+    const PaSeq q = pa_seq(p, s);
+    const int64_t units = pa_seq_units(p, q);
+    if (units == 0) continue;
+    const int np = (q.nq + W - 1) / W;
+    int pr = 0;
+    if (pos > at) {   // the last pair that starts at or before pos
+      int lo = 0, hi = np - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at + (int64_t)p.Hkv * pa_units_before(q, W, mid) <= pos) lo = mid;
+        else hi = mid - 1;
+      }
+      pr = lo;
+    }
+    int64_t pair_at = at + (int64_t)p.Hkv * pa_units_before(q, W, pr);
+    for (; pr < np && pos < end; ++pr) {
+      const int left = q.nq - pr * W;
+      const int n_tok = left < W ? left : W;
+      const int tiles = pa_tiles(q, W, pr);
+      const int wt = n_tok > p.TT ? 2 : 1;
+      const int iu = PA_ITEM + wt * tiles;
+      for (int hk = (int)((pos - pair_at) / iu); hk < p.Hkv && pos < end; ++hk) {
+        const int64_t item_at = pair_at + (int64_t)hk * iu;
+        const int x0 = (int)(pos - item_at), x1 = (int)pa_min(iu, end - item_at);
+        // a tile belongs to the piece in which its units start
+        const int t0 = x0 <= PA_ITEM ? 0 : (int)pa_min((x0 - PA_ITEM + wt - 1) / wt, tiles);
+        const int t1 = x1 == iu ? tiles : x1 <= PA_ITEM ? 0 : (int)pa_min((x1 - PA_ITEM + wt - 1) / wt, tiles);
+        pos = item_at + x1;
+        if (tiles > 0 ? t0 == t1 : x0 != 0) continue;
+        PaItem w;
+        w.tok0 = q.q0 + pr * W;
+        w.n_tok = n_tok;
+        w.src = q.src;
+        w.row0 = q.row0;
+        w.slot = q.slot;
+        w.hk = hk;
+        w.j0 = t0;
+        w.j1 = t1;
+        w.kv_len = q.kv;
+        w.pos0 = q.causal ? q.kv - q.nq + pr * W : 0x3fffffff;
+        const bool begins = t0 == 0, ends = t1 == tiles;
+        w.out_mode = !(begins && ends) ? PA_PIECE : p.prefix > 0 ? PA_ROWWISE : PA_DIRECT;
+        // a CTA's share begins with at most one unfinished item and ends with at most one
+        w.out_at = cta * 2 + (begins ? 1 : 0);
+        if (!emit(w, begins, ends)) return false;
+      }
+      pair_at += (int64_t)p.Hkv * iu;
+    }
+    at += units;
+  }
+  return true;
+}
+
+}  // namespace hokv

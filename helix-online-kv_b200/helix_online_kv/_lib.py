@@ -8,6 +8,7 @@ pure bookkeeping stay usable), but the first call that needs the device raises
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -67,6 +68,24 @@ class Cdc03Args(ctypes.Structure):
     ]
 
 
+class PackedArgs(ctypes.Structure):
+    """Mirror of ``hokv_packed_args`` (include/hokv.h)."""
+
+    _fields_ = [
+        ("dtype", _c_int), ("n_seqs", _c_int), ("q_heads", _c_int), ("kv_heads", _c_int), ("head_dim", _c_int),
+        ("causal", _c_int), ("kv_in_slots", _c_int), ("zero_tail", _c_int), ("scale", _c_f32), ("n_tokens", _c_i64),
+        ("q", _vp), ("q_stride_t", _c_i64), ("q_stride_h", _c_i64),
+        ("out", _vp), ("out_stride_t", _c_i64), ("out_stride_h", _c_i64),
+        ("cu_seqlens_q", _vp),
+        ("k", _vp), ("k_stride_b", _c_i64), ("k_stride_h", _c_i64), ("k_stride_t", _c_i64),
+        ("v", _vp), ("v_stride_b", _c_i64), ("v_stride_h", _c_i64), ("v_stride_t", _c_i64),
+        ("kv_rows", _c_i64), ("cu_seqlens_k", _vp), ("kv_len", _vp),
+        ("prefix_k", _vp), ("pk_stride_h", _c_i64), ("pk_stride_t", _c_i64),
+        ("prefix_v", _vp), ("pv_stride_h", _c_i64), ("pv_stride_t", _c_i64), ("prefix_len", _c_i64),
+        ("workspace", _vp), ("workspace_bytes", _c_sz),
+    ]
+
+
 _SIGS = {
     "hokv_abi_version": (_c_int, []),
     "hokv_status_string": (ctypes.c_char_p, [_c_int]),
@@ -104,6 +123,8 @@ _SIGS = {
                                       _c_sz, _vp]),
     "hokv_prefill_attention": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]
                                + [_c_i64] * 12 + [_c_f32, _c_int, _vp]),
+    "hokv_packed_attention_workspace_size": (_c_int, [ctypes.POINTER(PackedArgs), ctypes.POINTER(_c_sz)]),
+    "hokv_packed_attention": (_c_int, [ctypes.POINTER(PackedArgs), _vp]),
     "hokv_softmax": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _c_sz, _vp]),
     "hokv_prefilter_mask": (_c_int, [_vp, _c_int, _vp, _c_i64, _c_int, _vp, _vp]),
     "hokv_scale_f32_to_f64": (_c_int, [_vp, _c_i64, _c_f64, _vp, _vp]),
@@ -162,6 +183,13 @@ def check(status: int, what: str = ""):
 
 def stream():
     return _vp(torch.cuda.current_stream().cuda_stream)
+
+
+def on_device(dev):
+    """Context in which `dev` is the current device (nothing to do when it is already)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def ptr(t):

@@ -8,10 +8,16 @@ shared KV head, f16/bf16, head_dim 64 or 128, (batch, head, token) strides that
 nest (any permutation of a packed layout, or a slice of one: the CDC-03 store's
 views and the transposed projections a model passes need no copy), contiguous
 head dims, key and value with the same strides.
+
+``packed_attention`` is the same attention for a batch of sequences of
+different lengths in one launch (hokv_packed_attention): whole prompts, chunks
+of prompts behind their histories and single tokens side by side, with the keys
+and values packed like the queries or in slots (a CDC-03 store's tiers).
 """
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -78,4 +84,115 @@ def prefill_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
         query.stride(0), query.stride(1), query.stride(2), key.stride(0), key.stride(1), key.stride(2),
         value.stride(0), value.stride(1), value.stride(2), out.stride(0), out.stride(2), out.stride(1),
         scale, 1 if is_causal else 0, L.stream()), "prefill_attention")
+    return out
+
+
+def _lengths(t, n: Optional[int], name: str, device) -> None:
+    """A contiguous int32 CUDA vector (of n entries, when given) on `device`."""
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device or not t.is_cuda:
+        raise ValueError(f"Expected {name} as a contiguous int32 vector on {device}, got {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device}")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"Expected {name} of {n} entries, got {t.shape[0]}")
+
+
+def _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out):
+    """Checked arguments of hokv_packed_attention and the output tensor."""
+    if query.dtype not in _DTYPES or not query.is_cuda or query.dim() != 3:
+        raise ValueError(f"Expected f16/bf16 CUDA queries [T, H_q, D], got {tuple(query.shape)} {query.dtype} on "
+                         f"{query.device}")
+    T, Hq, D = query.shape
+    dev = query.device
+    slots = key.dim() == 4
+    for name, t in (("key", key), ("value", value)):
+        if t.dtype != query.dtype or t.device != dev or t.dim() not in (3, 4) or t.shape != key.shape or t.shape[-1] != D:
+            raise ValueError(f"Expected {name} [S, H_kv, {D}] or [B, H_kv, capacity, {D}] like the key, {query.dtype} on "
+                             f"{dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    Hkv = key.shape[1]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv or Hq // Hkv > 128:
+        raise ValueError(f"Expected query heads a multiple (up to 128) of the KV heads, got {Hq} and {Hkv}")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"Expected a head_dim in multiples of 8 up to 128, got {D}")
+    a = L.PackedArgs()
+    if slots:
+        if kv_len is None or cu_seqlens_k is not None:
+            raise ValueError("keys in slots [B, H_kv, capacity, D] need kv_len [B] (and no cu_seqlens_k)")
+        B = key.shape[0]
+        _lengths(kv_len, B, "kv_len", dev)
+        a.kv_len, a.kv_in_slots, a.kv_rows = kv_len.data_ptr(), 1, key.shape[2]
+    else:
+        if kv_len is not None:
+            raise ValueError("packed keys [S, H_kv, D] take cu_seqlens_k, not kv_len")
+        if cu_seqlens_k is None:
+            cu_seqlens_k = cu_seqlens_q
+        if cu_seqlens_k is None:
+            raise ValueError("packed keys [S, H_kv, D] need cu_seqlens_k or cu_seqlens_q")
+        _lengths(cu_seqlens_k, None, "cu_seqlens_k", dev)
+        B = cu_seqlens_k.shape[0] - 1
+        a.cu_seqlens_k, a.kv_rows = cu_seqlens_k.data_ptr(), key.shape[0]
+    if cu_seqlens_q is not None:
+        _lengths(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
+        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+    elif T != B:
+        raise ValueError(f"without cu_seqlens_q every sequence has one query: got {T} queries for {B} sequences")
+    if B < 0:
+        raise ValueError("cu_seqlens_k needs at least one entry")
+    scale = float(scaling) if scaling is not None else D ** -0.5
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"Expected a positive finite scaling, got {scaling}")
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1])):
+            raise ValueError(f"Expected {name} with contiguous head dims, strides in multiples of 8 elements and 16-byte "
+                             f"aligned data, got strides {t.stride()}")
+    if T > 1 and query.stride(0) < (Hq * query.stride(1) if Hq > 1 else D):
+        raise ValueError(f"Expected queries [T, H_q, D] whose token stride covers the heads, got strides {query.stride()}")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=query.dtype, device=dev)
+        a.zero_tail = 1
+    elif (out.shape != query.shape or out.dtype != query.dtype or out.device != dev
+          or (out.numel() and (out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8))):
+        raise ValueError(f"Expected out [{T}, {Hq}, {D}] {query.dtype} on {dev} with contiguous 16-byte aligned rows, got "
+                         f"{tuple(out.shape)} {out.dtype} on {out.device}")
+    a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim, a.causal = _DTYPES[query.dtype], B, Hq, Hkv, D, bool(is_causal)
+    a.scale, a.n_tokens = scale, T
+    a.q, a.q_stride_t, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
+    a.out, a.out_stride_t, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    a.k, a.v = key.data_ptr(), value.data_ptr()
+    if slots:
+        a.k_stride_b, a.k_stride_h, a.k_stride_t = key.stride()[:3]
+        a.v_stride_b, a.v_stride_h, a.v_stride_t = value.stride()[:3]
+    else:
+        a.k_stride_t, a.k_stride_h = key.stride()[:2]
+        a.v_stride_t, a.v_stride_h = value.stride()[:2]
+    return a, out
+
+
+def _packed_launch(a, what: str, device) -> None:
+    """Workspace of this call from the allocator, and the launch, on `device`'s current stream."""
+    lib = L.lib()
+    with L.on_device(device):
+        need = ctypes.c_size_t(0)
+        L.check(lib.hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), what)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+        L.check(lib.hokv_packed_attention(ctypes.byref(a), L.stream()), what)
+
+
+def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                     cu_seqlens_q: Optional[torch.Tensor] = None, cu_seqlens_k: Optional[torch.Tensor] = None,
+                     kv_len: Optional[torch.Tensor] = None, scaling: Optional[float] = None, is_causal: bool = True,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(query key^T * scaling [causal]) value for every sequence of a packed batch.
+
+    query [T, H_q, D]: sequence b owns tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (without cu_seqlens_q, token
+    b).  key/value either packed [S, H_kv, D] with cu_seqlens_k [B + 1] (default: cu_seqlens_q) or in slots [B,
+    H_kv, capacity, D] with kv_len [B], the keys each sequence holds, its new tokens included (a slot's rows behind
+    kv_len are not used).  Lengths are int32 CUDA vectors and stay on the device.  Causal: query i of a sequence
+    with n keys and m queries sits at position n - m + i; a query that sees no key gives zeros.  f16/bf16, head
+    dims in multiples of 8 up to 128, contiguous head dims, strides in multiples of 8 elements, H_q a multiple of
+    H_kv.  -> [T, H_q, D] in the query's dtype; rows behind the last sequence are zeros, or left as they were in a
+    given ``out`` (which must not overlap the inputs)."""
+    a, out = _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)
+    if out.numel():
+        _packed_launch(a, "packed_attention", out.device)
     return out

@@ -199,6 +199,59 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
                            int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_s, float scale,
                            int causal, void* stream);
 
+/* Exact attention of a packed batch: per sequence b (query tokens
+ * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q, n_b keys) and query head h,
+ *   out_i = softmax_j(scale q_i . k_j) v_j
+ * over the keys query i may see: with `causal` the keys j <= n_b - nq_b + i
+ * (query i sits at position n_b - nq_b + i; a query before position 0 sees
+ * none), else all n_b; with a shared prefix (prefix_len > 0) all prefix keys
+ * as well.  A query that sees no key gives zeros.  The reference leaves this
+ * to the model's own attention, one unpadded batch at a time
+ * (compressed_cache.py:72-105).
+ *
+ * q and out [n_tokens, q_heads, head_dim], element strides (token, head), the
+ * head dim contiguous; q's token stride covers its heads.  cu_seqlens_q
+ * [n_seqs + 1] or NULL (one token per sequence, n_tokens = n_seqs).  Keys and
+ * values either packed (kv_in_slots = 0: [kv_rows, kv_heads, head_dim],
+ * cu_seqlens_k [n_seqs + 1]) or in slots (kv_in_slots = 1: [n_seqs, kv_heads,
+ * kv_rows, head_dim], kv_len [n_seqs]; rows behind kv_len are never used,
+ * whatever they hold); strides that nest, as hokv_prefill_attention.  The
+ * prefix is [kv_heads, prefix_len, head_dim].  Lengths are device int32:
+ * nothing is read back, so a call can be captured into a graph and replayed
+ * with new lengths.  Lengths that do not fit the tensors set
+ * HOKV_ERR_DEVICE_INPUT in the device status and leave that sequence's rows
+ * of out unspecified.  Rows of out behind cu_seqlens_q[n_seqs] are left as
+ * they are (zero_tail = 0) or zeroed (1).
+ *
+ * f16/bf16, head_dim a multiple of 8 up to 128, up to 128 query heads per KV
+ * head, scale > 0, strides multiples of 8 elements, 16-byte aligned pointers.
+ * fp32 sums; the softmax weights are rounded to the input type before the
+ * second product.  Non-finite keys or values that a causal mask hides from a
+ * query may still reach it when they share its 128-key tile.  Results are the
+ * same on every run (no atomics).  Calls that overlap on the GPU need
+ * workspaces of their own. */
+typedef struct hokv_packed_args {
+  int dtype, n_seqs, q_heads, kv_heads, head_dim, causal, kv_in_slots, zero_tail;
+  float scale;
+  int64_t n_tokens;
+  const void* q; int64_t q_stride_t, q_stride_h;
+  void* out; int64_t out_stride_t, out_stride_h;
+  const int* cu_seqlens_q;
+  const void* k; int64_t k_stride_b, k_stride_h, k_stride_t;
+  const void* v; int64_t v_stride_b, v_stride_h, v_stride_t;
+  int64_t kv_rows;
+  const int* cu_seqlens_k; const int* kv_len;
+  const void* prefix_k; int64_t pk_stride_h, pk_stride_t;
+  const void* prefix_v; int64_t pv_stride_h, pv_stride_t;
+  int64_t prefix_len;
+  void* workspace; size_t workspace_bytes;
+} hokv_packed_args;
+
+/* Scratch bytes of a call (q_heads, kv_heads, head_dim, n_tokens, prefix_len
+ * of `a`; the current device). */
+int hokv_packed_attention_workspace_size(const hokv_packed_args* a, size_t* bytes);
+int hokv_packed_attention(const hokv_packed_args* a, void* stream);
+
 /* scipy.special.softmax over n values stored f32 (is_f64 = 0) or f64, computed
  * in f64 (compressed_attention.py:31-33). */
 int hokv_softmax(const void* in, int is_f64, int64_t n, void* out, void* workspace,

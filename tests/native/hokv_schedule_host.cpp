@@ -1,0 +1,38 @@
+// Host build of the packed attention's schedule (packed_schedule.cuh).
+#include "packed_schedule.cuh"
+
+using namespace hokv;
+
+extern "C" {
+
+int64_t host_floor_sum(int64_t n, int64_t a, int64_t b) { return pa_floor_sum(n, a, b); }
+
+// Every piece of every CTA, 16 ints each: cta, begins, ends, then PaItem's
+// fields.  Returns the number of pieces, or -1 when `cap` is too small.
+int64_t host_schedule(const int* cu_q, const int* cu_k, const int* kv_len, int n_seqs, int T, int Hkv, int TT,
+                      int64_t kv_rows, int prefix, int causal, int n_ctas, int* out, int64_t cap, int64_t* units) {
+  PaSched p = {cu_q, cu_k, kv_len, n_seqs, T, Hkv, TT, kv_rows, prefix, causal, n_ctas};
+  const int n_s = pa_n_seqs(p);
+  int64_t total = 0;
+  for (int s = 0; s < n_s; ++s) total += pa_seq_units(p, pa_seq(p, s));
+  *units = total;
+  const int64_t share = pa_share(p, total);
+  int64_t n = 0;
+  for (int c = 0; c < n_ctas; ++c) {
+    const int64_t begin = pa_min(c * share, total), end = pa_min(begin + share, total);
+    if (begin >= end) continue;
+    int64_t at = 0;
+    const int s = pa_find(p, 0, n_s, begin, at);
+    const bool ok = pa_walk(p, c, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends) {
+      if (n == cap) return false;
+      int* o = out + 16 * n++;
+      const int f[16] = {c, begins, ends, w.tok0, w.n_tok, w.src, w.row0, w.slot, w.hk, w.j0, w.j1, w.kv_len, w.pos0,
+                         w.out_mode, w.out_at, 0};
+      for (int i = 0; i < 16; ++i) o[i] = f[i];
+      return true;
+    });
+    if (!ok) return -1;
+  }
+  return n;
+}
+}
