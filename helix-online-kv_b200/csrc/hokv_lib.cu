@@ -11,6 +11,7 @@
 #include "assign_tc.cuh"
 #include "prefill.cuh"
 #include "packed_attn.cuh"
+#include "norm_rotate.cuh"
 
 #include <map>
 #include <mutex>
@@ -1116,3 +1117,76 @@ int hokv_packed_attention(const hokv_packed_args* a, void* stream) {
 }
 
 }  // extern "C"
+
+// ---- norm, rotation and append of new tokens -------------------------------------
+namespace hokv {
+
+template <typename T>
+static int launch_norm_rotate(NraP p, bool vec, cudaStream_t st) {
+  const int heads = p.Hq + 2 * p.Hkv;
+  if (!vec) {
+    const int64_t blocks = cdiv((int64_t)p.T * heads, NRA_THREADS / 32);
+    HOKV_REQUIRE(blocks < (1ll << 31), "norm_rotate_append: grid too large");
+    k_norm_rotate_scalar<T><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
+    return check_launch("k_norm_rotate_scalar");
+  }
+  const int lpr = p.D <= 64 ? 4 : p.D <= 128 ? 8 : 16;
+  // several heads share a token's angles once that leaves every SM full (2048 threads)
+  p.hpg = 1;
+  for (int n = 8; n > 1 && p.hpg == 1; n >>= 1)
+    if ((int64_t)p.T * cdiv(heads, n) * lpr >= (int64_t)pa_ctas() * 2048) p.hpg = n;
+  p.chunks = (int)cdiv(heads, p.hpg);
+  const int64_t blocks = cdiv((int64_t)p.T * p.chunks, NRA_THREADS / lpr);
+  HOKV_REQUIRE(blocks < (1ll << 31), "norm_rotate_append: grid too large");
+  if (lpr == 4) k_norm_rotate<T, 4><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
+  else if (lpr == 8) k_norm_rotate<T, 8><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
+  else k_norm_rotate<T, 16><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
+  return check_launch("k_norm_rotate");
+}
+
+}  // namespace hokv
+
+extern "C" int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* stream) {
+  HOKV_REQUIRE(a, "norm_rotate_append: null arguments");
+  HOKV_REQUIRE(a->dtype == HOKV_F16 || a->dtype == HOKV_BF16 || a->dtype == HOKV_F32, "norm_rotate_append: dtype %d",
+               a->dtype);
+  HOKV_REQUIRE(a->n_tokens >= 0 && a->n_tokens < (1ll << 30) && a->n_seqs >= 0 && a->n_seqs < (1 << 30) &&
+                   a->capacity >= 0 && a->capacity < (1ll << 30),
+               "norm_rotate_append: n_tokens=%lld n_seqs=%d capacity=%lld", (long long)a->n_tokens, a->n_seqs,
+               (long long)a->capacity);
+  HOKV_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads < (1 << 20) && a->kv_heads < (1 << 20),
+               "norm_rotate_append: q_heads=%d kv_heads=%d", a->q_heads, a->kv_heads);
+  if (a->head_dim < 2 || a->head_dim > 256 || a->head_dim % 2)
+    return fail(HOKV_ERR_UNSUPPORTED, "norm_rotate_append: head_dim %d (even, up to 256)", a->head_dim);
+  HOKV_REQUIRE(a->n_freq >= 0 && 2 * a->n_freq <= a->head_dim, "norm_rotate_append: %d frequencies for head_dim %d",
+               a->n_freq, a->head_dim);
+  HOKV_REQUIRE(a->eps >= 0.f && a->eps < INFINITY, "norm_rotate_append: eps %g", a->eps);
+  if (a->n_tokens == 0) return HOKV_OK;
+  HOKV_REQUIRE(a->q && a->k && a->v && a->out && a->kv_len && (a->n_freq == 0 || a->inv_freq),
+               "norm_rotate_append: null pointer");
+  HOKV_REQUIRE((a->k_slots && a->v_slots) || a->capacity == 0 || a->n_seqs == 0, "norm_rotate_append: null slots");
+  HOKV_REQUIRE(a->cu_seqlens || a->n_tokens == a->n_seqs, "norm_rotate_append: %lld tokens for %d sequences of one token",
+               (long long)a->n_tokens, a->n_seqs);
+  NraP p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.qw = a->q_weight; p.kw = a->k_weight;
+  p.out = a->out; p.ks = a->k_slots; p.vs = a->v_slots;
+  p.q_t = a->q_stride_t; p.q_h = a->q_stride_h; p.k_t = a->k_stride_t; p.k_h = a->k_stride_h;
+  p.v_t = a->v_stride_t; p.v_h = a->v_stride_h; p.out_t = a->out_stride_t; p.out_h = a->out_stride_h;
+  p.ks_b = a->ks_stride_b; p.ks_h = a->ks_stride_h; p.ks_t = a->ks_stride_t;
+  p.vs_b = a->vs_stride_b; p.vs_h = a->vs_stride_h; p.vs_t = a->vs_stride_t;
+  p.cu = a->cu_seqlens; p.kv_len = a->kv_len; p.pos = a->positions; p.inv_freq = a->inv_freq;
+  p.cap = a->capacity;
+  p.n_seqs = a->n_seqs; p.T = (int)a->n_tokens; p.Hq = a->q_heads; p.Hkv = a->kv_heads; p.D = a->head_dim;
+  p.n_freq = a->n_freq; p.interleaved = a->interleaved ? 1 : 0; p.zero_tail = a->zero_tail ? 1 : 0;
+  p.eps = a->eps;
+  // 16-byte rows and whole 8-element chunks of both halves: the vector form
+  const int e16 = a->dtype == HOKV_F32 ? 4 : 8;
+  bool vec = p.D % 16 == 0 && (p.interleaved || p.n_freq % 8 == 0);
+  const int64_t st[14] = {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h, p.out_t, p.out_h, p.ks_b, p.ks_h, p.ks_t, p.vs_b, p.vs_h, p.vs_t};
+  for (int i = 0; i < 14; ++i) vec = vec && st[i] % e16 == 0;
+  vec = vec && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16) && aligned(p.out, 16) && aligned(p.ks, 16) &&
+        aligned(p.vs, 16);
+  if (a->dtype == HOKV_F16) return launch_norm_rotate<__half>(p, vec, S(stream));
+  if (a->dtype == HOKV_BF16) return launch_norm_rotate<__nv_bfloat16>(p, vec, S(stream));
+  return launch_norm_rotate<float>(p, vec, S(stream));
+}

@@ -86,6 +86,23 @@ class PackedArgs(ctypes.Structure):
     ]
 
 
+class NormRotateArgs(ctypes.Structure):
+    """Mirror of ``hokv_norm_rotate_args`` (include/hokv.h)."""
+
+    _fields_ = [
+        ("dtype", _c_int), ("n_seqs", _c_int), ("q_heads", _c_int), ("kv_heads", _c_int), ("head_dim", _c_int),
+        ("n_freq", _c_int), ("interleaved", _c_int), ("zero_tail", _c_int), ("eps", _c_f32), ("n_tokens", _c_i64),
+        ("q", _vp), ("q_stride_t", _c_i64), ("q_stride_h", _c_i64),
+        ("k", _vp), ("k_stride_t", _c_i64), ("k_stride_h", _c_i64),
+        ("v", _vp), ("v_stride_t", _c_i64), ("v_stride_h", _c_i64),
+        ("out", _vp), ("out_stride_t", _c_i64), ("out_stride_h", _c_i64),
+        ("k_slots", _vp), ("ks_stride_b", _c_i64), ("ks_stride_h", _c_i64), ("ks_stride_t", _c_i64),
+        ("v_slots", _vp), ("vs_stride_b", _c_i64), ("vs_stride_h", _c_i64), ("vs_stride_t", _c_i64),
+        ("capacity", _c_i64), ("cu_seqlens", _vp), ("kv_len", _vp), ("positions", _vp), ("inv_freq", _vp),
+        ("q_weight", _vp), ("k_weight", _vp),
+    ]
+
+
 _SIGS = {
     "hokv_abi_version": (_c_int, []),
     "hokv_status_string": (ctypes.c_char_p, [_c_int]),
@@ -125,6 +142,7 @@ _SIGS = {
                                + [_c_i64] * 12 + [_c_f32, _c_int, _vp]),
     "hokv_packed_attention_workspace_size": (_c_int, [ctypes.POINTER(PackedArgs), ctypes.POINTER(_c_sz)]),
     "hokv_packed_attention": (_c_int, [ctypes.POINTER(PackedArgs), _vp]),
+    "hokv_norm_rotate_append": (_c_int, [ctypes.POINTER(NormRotateArgs), _vp]),
     "hokv_softmax": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _c_sz, _vp]),
     "hokv_prefilter_mask": (_c_int, [_vp, _c_int, _vp, _c_i64, _c_int, _vp, _vp]),
     "hokv_scale_f32_to_f64": (_c_int, [_vp, _c_i64, _c_f64, _vp, _vp]),

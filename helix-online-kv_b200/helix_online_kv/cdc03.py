@@ -26,7 +26,9 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from .prefill import packed_attention
 from .product_codebook import SLOTS
+from .rotary import norm_rotate_append
 
 
 def code_bytes_for(M: int) -> int:
@@ -162,6 +164,39 @@ class CDC03Store:
         for layer in range(self.L):
             self.age(layer, cold_from, cold_to, order)
         self.seq_len += 1
+
+    # ---- packed batches ---------------------------------------------------------
+    # One step of a ragged batch (whole prompts, chunks, single tokens side by
+    # side): append_packed and attend_packed for every layer, then advance.
+    def append_packed(self, layer: int, query, key, value, cu_seqlens, inv_freq, q_weight=None, k_weight=None,
+                      eps: float = 1e-6, interleaved: bool = False, positions=None):
+        """Norm and rotate the new tokens of one layer and write their keys and
+        values behind the rows each sequence holds (rotary.norm_rotate_append on
+        this layer's tiers and seq_len).  query [T, H_q, D], key/value [T, H_kv, D],
+        cu_seqlens [B + 1]; returns the rotated queries.  seq_len is advanced
+        once per step, by ``advance``."""
+        return norm_rotate_append(query, key, value, self.k[layer], self.v[layer], cu_seqlens, self.seq_len, inv_freq,
+                                  q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                  positions=positions)
+
+    def attend_packed(self, layer: int, query, cu_seqlens, kv_len, scale: float, out=None):
+        """Exact causal attention of the new tokens over one layer's tiers
+        (prefill.packed_attention); kv_len [B] counts them (``lengths_after``)."""
+        return packed_attention(query, self.k[layer], self.v[layer], cu_seqlens, kv_len=kv_len, scaling=scale, out=out)
+
+    def lengths_after(self, cu_seqlens):
+        """seq_len with the step's new tokens (device int32 [B]; no host sync)."""
+        return self.seq_len + cu_seqlens.diff()
+
+    def advance(self, cu_seqlens, hot_window: int = 256, layers=None, order: int | None = None):
+        """End of a packed step: the tokens that leave the hot window get their PQ
+        codes in ``layers`` (default: all; pass the calibrated ones) and seq_len
+        grows by each sequence's new tokens.  Device-side only."""
+        new = self.lengths_after(cu_seqlens)
+        cold_from, cold_to = torch.clamp(self.seq_len - hot_window, min=0), torch.clamp(new - hot_window, min=0)
+        for layer in range(self.L) if layers is None else layers:
+            self.age(layer, cold_from, cold_to, order)
+        self.seq_len.copy_(new)
 
     # ---- decode ---------------------------------------------------------------
     def args(self, layer: int, q, out, scale: float, top_k: int = 128, sink_tokens: int = 4,

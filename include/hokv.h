@@ -252,6 +252,39 @@ typedef struct hokv_packed_args {
 int hokv_packed_attention_workspace_size(const hokv_packed_args* a, size_t* bytes);
 int hokv_packed_attention(const hokv_packed_args* a, void* stream);
 
+/* The new tokens of a packed batch, before attention: per token i of sequence
+ * b (cu_seqlens [n_seqs + 1], or NULL: one token each), at position kv_len[b] +
+ * i (or positions[t]), RMS norm of every query and key head,
+ *   y = x w / sqrt(mean(x^2) + eps)     (q_weight / k_weight NULL: y = x),
+ * the rotation of dims (f, f + n_freq), or (2f, 2f + 1) when interleaved, f <
+ * n_freq, by the angle position * inv_freq[f] (formed in 64 bits), queries to
+ * `out`, keys and values (copied) to row kv_len[b] + i of slot b, [n_seqs,
+ * kv_heads, capacity, head_dim].  kv_len is not advanced.  The reference leaves
+ * this to the model and appends rotated keys token by token
+ * (layer_state.py:68-133).  f16, bf16 or f32 throughout (weights too;
+ * inv_freq f32), element strides, head dims contiguous, even head_dim up to
+ * 256; fp32 arithmetic, rounded once.  `out` may be q itself.  A row that does
+ * not fit its slot is not written and sets HOKV_ERR_DEVICE_INPUT.  Tokens
+ * behind the last sequence append nothing; their rows of `out` are left as
+ * they are (zero_tail = 0) or zeroed (1). */
+typedef struct hokv_norm_rotate_args {
+  int dtype, n_seqs, q_heads, kv_heads, head_dim, n_freq, interleaved, zero_tail;
+  float eps;
+  int64_t n_tokens;
+  const void* q; int64_t q_stride_t, q_stride_h;
+  const void* k; int64_t k_stride_t, k_stride_h;
+  const void* v; int64_t v_stride_t, v_stride_h;
+  void* out; int64_t out_stride_t, out_stride_h;
+  void* k_slots; int64_t ks_stride_b, ks_stride_h, ks_stride_t;
+  void* v_slots; int64_t vs_stride_b, vs_stride_h, vs_stride_t;
+  int64_t capacity;
+  const int* cu_seqlens; const int* kv_len; const int* positions;
+  const float* inv_freq;
+  const void* q_weight; const void* k_weight;
+} hokv_norm_rotate_args;
+
+int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* stream);
+
 /* scipy.special.softmax over n values stored f32 (is_f64 = 0) or f64, computed
  * in f64 (compressed_attention.py:31-33). */
 int hokv_softmax(const void* in, int is_f64, int64_t n, void* out, void* workspace,
