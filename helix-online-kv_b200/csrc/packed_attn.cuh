@@ -117,15 +117,39 @@ __device__ __forceinline__ void pa_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// kind::f16 MMA with A in tensor memory (16-bit pairs per column).
-__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc,
-                                            int accumulate) {
-  const uint32_t no_mask = 0u;
+// The MMA warp runs as a whole with warp-uniform values and one elected lane
+// issues: operands that the compiler cannot prove uniform cost a loop of votes
+// per instruction (130 cycles for each MMA, twice the 128 x 128 x 16 product
+// itself).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Halves of umma_desc_sw (128-byte swizzle): the low one holds address and
+// leading byte offset, the high one the stride byte offset and constants.
+__device__ __forceinline__ uint32_t pa_desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t PA_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+
+// kind::f16 MMA, A and B in shared memory.
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(no_mask));
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "n"(PA_DESC_HI)
+      : "memory");
+}
+// The same with A in tensor memory (16-bit pairs per column).
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "n"(PA_DESC_HI)
+      : "memory");
 }
 
 // 32 packed columns of this thread's lane into tensor memory, without waiting.
@@ -140,7 +164,27 @@ __device__ __forceinline__ void tmem_st32_nw(uint32_t taddr, const uint32_t (&v)
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+// Scale 8 fp32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One 32-byte store (a whole sector): a thread's row of O.
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* u) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+               "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
 
 // ---- the kernel ----------------------------------------------------------------
 
@@ -197,7 +241,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl[0];
+  constexpr uint32_t tmem = 0;   // all 512 columns are this CTA's: the base is column 0
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int TT = p.TT, G = p.G;
 
@@ -210,27 +254,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_sel + (uint32_t)(sl * 128);
     const uint32_t o_addr = tmem + lane_sel + (uint32_t)(256 + sl * 128);
+    // rows of out on 32-byte boundaries and in whole 16-element steps: 32-byte stores
+    const bool wide = p.D % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) % 32 | (uint64_t)(p.ost % 16) | (uint64_t)(p.osh % 16)) == 0;
     unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int qi = it % PA_QUEUE;
       if (!pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag)) break;
-      const PaItem w = queue[qi];
-      __syncwarp();
-      if (lane == 0) pa_arrive(&it_empty[qi]);
+      const volatile PaItem& w = queue[qi];   // read again where needed: registers are short in the loop
       if (w.out_mode == PA_STOP) break;
       const bool two = w.n_tok > TT;
       const int n = w.j1 - w.j0;
       const int mine = two ? n : (sl == 0 ? (n + 1) >> 1 : n >> 1);   // key tiles of this slot
-      const int tok = (two ? sl * TT : 0) + row_tok;                  // this row's token in the item
-      const bool row_ok = row_tok < TT && tok < w.n_tok;
-      const int lim = min(w.kv_len, w.pos0 + tok + 1);                // keys this row sees
-      const int wtok = (two ? sl * TT : 0) + first_tok;
-      const bool warp_ok = first_tok < TT && wtok < w.n_tok;          // any row of the warp in use
-      const int wlim = min(w.kv_len, w.pos0 + wtok + 1);              // least such limit of the warp
+      const bool warp_ok = first_tok < TT && (two ? sl * TT : 0) + first_tok < w.n_tok;   // any row of the warp in use
+      // keys this row sees, and the least such limit of the warp, counted from the slot's key tile
+      int lim = min(w.kv_len, w.pos0 + (two ? sl * TT : 0) + row_tok + 1) - (w.j0 + (two ? 0 : sl)) * PA_BN;
+      int wlim = __shfl_sync(0xffffffffu, lim, 0);
+      const int step = two ? PA_BN : 2 * PA_BN;
+      auto item_done = [&]() {
+        __syncwarp();
+        if (lane == 0) pa_arrive(&it_empty[qi]);
+      };
       float m_run = -INFINITY, l_run = 0.f;
-      for (int i = 0; i < mine; ++i) {
-        const int t0 = (w.j0 + (two ? i : 2 * i + sl)) * PA_BN;
+      for (int i = 0; i < mine; ++i, lim -= step, wlim -= step) {
         if (!pa_wait(&s_full[sl], s_ph, abort_flag)) { ok = false; break; }
         s_ph ^= 1;
         tc_fence_after();
@@ -239,10 +285,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, *reinterpret_cast<float(*)[32]>(&v[c * 32]));
           tmem_wait_ld();
-          if (t0 + PA_BN > wlim) {
-            const int lm = lim - t0;
+          if (wlim < PA_BN) {
 #pragma unroll
-            for (int j = 0; j < 128; ++j) v[j] = j < lm ? v[j] : -INFINITY;
+            for (int j = 0; j < 128; ++j) v[j] = j < lim ? v[j] : -INFINITY;
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -254,14 +299,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             // O was last written by this slot's previous P V, complete before this S
             const float f = grow ? pf_ex2(m_run - m_new) : 1.f;
             l_run *= f;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32(o_addr + c * 32, o);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] *= f;
-              tmem_st32(o_addr + c * 32, o);
-            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
+            tmem_wait_st();
           }
           m_run = m_new;
           const float nm = m_run == -INFINITY ? 0.f : -m_run;
@@ -300,6 +340,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           __syncwarp();
           if (lane == 0) pa_arrive(ml_full);
         }
+        item_done();
         continue;   // slot 0 reads O_1 and frees it
       }
       float f0 = 1.f, f1 = 0.f;
@@ -317,12 +358,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       if (sl == 0 && (join || (two && n > 0))) o1_ph ^= 1;   // slot 1 completed a phase too
       const bool nothing = n == 0 || l_run == 0.f;
       const float inv = nothing ? 0.f : 1.f / l_run;
+      const int tok = (two ? sl * TT : 0) + row_tok;                  // this row's token in the item
+      const bool row_ok = row_tok < TT && tok < w.n_tok;
+      const int out_mode = w.out_mode, src = w.src, out_at = w.out_at;
       const int64_t t = w.tok0 + tok;
       const int hq = w.hk * G + row_g;
       const int prow = (two ? sl * 128 : 0) + row;      // row in a piece
-      if (w.out_mode != PA_DIRECT && row_ok) {
-        if (w.out_mode == PA_PIECE) p.ml[(int64_t)w.out_at * 256 + prow] = make_float2(m_run, l_run);
-        else p.row_ml[((int64_t)w.src * p.T + t) * p.Hq + hq] = make_float2(m_run, l_run);
+      if (out_mode != PA_DIRECT && row_ok) {
+        if (out_mode == PA_PIECE) p.ml[(int64_t)out_at * 256 + prow] = make_float2(m_run, l_run);
+        else p.row_ml[((int64_t)src * p.T + t) * p.Hq + hq] = make_float2(m_run, l_run);
       }
       if (warp_ok) {
 #pragma unroll
@@ -342,23 +386,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
           }
           if (row_ok) {
-            if (w.out_mode == PA_DIRECT) {
+            if (out_mode == PA_DIRECT) {
               T* og = reinterpret_cast<T*>(p.out) + t * p.ost + hq * p.osh;
+              uint32_t u[16];
 #pragma unroll
-              for (int j = 0; j < 32; j += 8) {
-                if (c * 32 + j < p.D) {
-                  uint4 u;
-                  u.x = pack2<T>(o[j + 0] * inv, o[j + 1] * inv);
-                  u.y = pack2<T>(o[j + 2] * inv, o[j + 3] * inv);
-                  u.z = pack2<T>(o[j + 4] * inv, o[j + 5] * inv);
-                  u.w = pack2<T>(o[j + 6] * inv, o[j + 7] * inv);
-                  *reinterpret_cast<uint4*>(og + c * 32 + j) = u;
-                }
+              for (int j = 0; j < 16; ++j) u[j] = pack2<T>(o[2 * j] * inv, o[2 * j + 1] * inv);
+              if (wide) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 8)
+                  if (c * 32 + 2 * j < p.D) st_global_32(og + c * 32 + 2 * j, &u[j]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4)
+                  if (c * 32 + 2 * j < p.D)
+                    *reinterpret_cast<uint4*>(og + c * 32 + 2 * j) = make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
               }
             } else {
-              const bool piece = w.out_mode == PA_PIECE;
-              float4* base = piece ? p.o + ((int64_t)w.out_at * (D / 4)) * 256 + prow
-                                   : p.row_o + (((int64_t)w.src * p.T + t) * p.Hq + hq) * (D / 4);
+              const bool piece = out_mode == PA_PIECE;
+              float4* base = piece ? p.o + ((int64_t)out_at * (D / 4)) * 256 + prow
+                                   : p.row_o + (((int64_t)src * p.T + t) * p.Hq + hq) * (D / 4);
               const int step = piece ? 256 : 1;
 #pragma unroll
               for (int j = 0; j < 32; j += 4)
@@ -375,6 +421,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           if (join) pa_arrive(&o_empty[1]);
         }
       }
+      item_done();
     }
     if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
       const int used = pa_used(p);
@@ -437,69 +484,82 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         }
       }
     } else if (warp == 9) {
-      // ---- MMA issue (the warp waits, lane 0 issues) --------------------------------
+      // ---- MMA issue --------------------------------------------------------------
       const int kd = (p.D + 15) / 16;
       const uint32_t idesc_s = umma_idesc_f16(PA_BN, BF, 0), idesc_o = umma_idesc_f16(kd * 16, BF, 1);
-      const uint32_t aQ = smem_u32(sQ), aKV = smem_u32(sKV);
-      unsigned ring = 0, q_uses = 0, p_ph[2] = {0, 0}, o_uses[2] = {0, 0};
+      const uint32_t q_lo = pa_desc_lo(smem_u32(sQ), 16), k_lo = pa_desc_lo(smem_u32(sKV), 16),
+                     v_lo = pa_desc_lo(smem_u32(sKV), PA_BN * 128);
+      unsigned stage = 0, stage_ph = 0, q_ph = 0, p_ph0 = 0, p_ph1 = 0, oe_ph0 = 1, oe_ph1 = 1;
       bool ok = true;
+      auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
       // the next tile of the ring, once its bytes have landed
       auto next_tile = [&]() {
-        const unsigned st = ring % ST, use = ring / ST;
-        ++ring;
-        ok = ok && pa_wait(&kv_full[st], use & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        const unsigned st = stage;
+        ok = all(pa_wait(&kv_full[st], stage_ph, abort_flag));
+        if (++stage == ST) stage = 0, stage_ph ^= 1;
+        tc_fence_after();
         return st;
       };
-      auto issue_s = [&](int sl, int q, unsigned st, bool release, bool last) {   // S = Q_q K^T
-        if (lane == 0) {
-          const uint32_t a = aQ + q * PG::Q_BYTES, bk = aKV + st * PG::KV_BYTES;
+      // S of slot SL = Q_q K^T
+      auto issue_s = [&](auto slc, unsigned q, unsigned st, bool release, bool last) {
+        constexpr int SL = decltype(slc)::value;
+        const uint32_t a = q_lo + q * (PG::Q_BYTES >> 4), b = k_lo + st * (PG::KV_BYTES >> 4);
+        if (elect_one()) {
 #pragma unroll
-          for (int kc = 0; kc < D / 16; ++kc)
-            if (kc < kd)
-              umma_f16(tmem + (uint32_t)(sl * 128), umma_desc_sw(a + (kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32, 16, 1024),
-                       umma_desc_sw(bk + (kc >> 2) * PA_BN * 128 + (kc & 3) * 32, 16, 1024), idesc_s, kc > 0);
-          umma_commit(&s_full[sl]);
+          for (int kc = 0; kc < D / 16; ++kc) {   // 16 dims = 32 bytes inside a 64-dim column block
+            const uint32_t off = (uint32_t)(((kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32) >> 4);
+            if (kc < kd) pa_mma_ss(SL * 128, a + off, b + off, idesc_s, kc > 0);
+          }
+          umma_commit(&s_full[SL]);
           if (release) umma_commit(&kv_empty[st]);
           if (last) umma_commit(q_empty);
         }
         __syncwarp();
       };
+      // O of slot SL += P V over ks steps of 16 tokens
+      auto issue_pv = [&](auto slc, unsigned sv, int ks, bool first, bool release, bool last) {
+        constexpr int SL = decltype(slc)::value;
+        unsigned& ph = SL ? p_ph1 : p_ph0;
+        unsigned& oe = SL ? oe_ph1 : oe_ph0;
+        ok = all(pa_wait(&p_full[SL], ph, abort_flag));
+        ph ^= 1;
+        if (first) {   // the epilogue of the slot's last item has read O (passes at once the first time)
+          ok = all(ok && pa_wait(&o_empty[SL], oe, abort_flag));
+          oe ^= 1;
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t b = v_lo + sv * (PG::KV_BYTES >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int kc = 0; kc < PA_BN / 16; ++kc)
+            if (kc < ks) pa_mma_ts(256 + SL * 128, SL * 128 + kc * 8, b + kc * (2048 >> 4), idesc_o, !first || kc > 0);
+          if (last) umma_commit(&o_full[SL]);
+          if (release) umma_commit(&kv_empty[sv]);
+        }
+        __syncwarp();
+      };
+      constexpr std::integral_constant<int, 0> S0;
+      constexpr std::integral_constant<int, 1> S1;
       for (int it = 0; ok; ++it) {
         const int qi = it % PA_QUEUE;
-        ok = pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
         if (!ok) break;
-        const PaItem w = queue[qi];
+        const int mode = uniform(queue[qi].out_mode), n = uniform(queue[qi].j1 - queue[qi].j0),
+                  two = uniform(queue[qi].n_tok > TT), left = uniform(queue[qi].kv_len - queue[qi].j0 * PA_BN);
         __syncwarp();
         if (lane == 0) pa_arrive(&it_empty[qi]);
-        if (w.out_mode == PA_STOP) break;
-        const int n = w.j1 - w.j0;
+        if (mode == PA_STOP) break;
         if (n == 0) continue;
-        const bool two = w.n_tok > TT;
-        ok = pa_wait(q_full, q_uses & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        ++q_uses;
+        ok = all(pa_wait(q_full, q_ph, abort_flag));
+        q_ph ^= 1;
         if (!ok) break;
-        unsigned st = next_tile();
-        if (!ok) break;
-        tc_fence_after();
-        issue_s(0, 0, st, !two, !two && n == 1);
-        if (two) {
-          issue_s(1, 1, st, true, n == 1);
-        } else if (n > 1) {
-          st = next_tile();
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(1, 0, st, true, n == 2);
-        }
-        for (int j = 0; ok && j < n; ++j) {
+        // V(j) ready: its stage and 16-token steps; rows behind the sequence inside the last step are zeroed
+        auto ready_v = [&](int j, int& ks) {
           const unsigned sv = next_tile();
-          if (!ok) break;
-          const uint32_t bv = aKV + sv * PG::KV_BYTES;
-          const int valid = min(PA_BN, w.kv_len - (w.j0 + j) * PA_BN);
-          const int ks = (valid + 15) >> 4;
-          if (valid & 15) {   // rows behind the sequence inside its last 16-token step
+          const int valid = min(PA_BN, left - j * PA_BN);
+          ks = (valid + 15) >> 4;
+          if (ok && (valid & 15)) {
             unsigned char* tile = sKV + sv * PG::KV_BYTES;
             const int rows = ks * 16 - valid;
             for (int e = lane; e < rows * PG::NB * 8; e += 32) {
@@ -509,37 +569,42 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             fence_async_smem();
             __syncwarp();
           }
-          unsigned sk = 0;
-          for (int h = 0; h < (two ? 2 : 1); ++h) {
-            const int sl = two ? h : (j & 1);
-            const bool first = two ? j == 0 : j < 2;
-            const bool last = two ? j == n - 1 : j >= n - 2;
-            ok = pa_wait(&p_full[sl], p_ph[sl], abort_flag);
-            if (ok && first && o_uses[sl] > 0) ok = pa_wait(&o_empty[sl], (o_uses[sl] - 1) & 1, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
+          return sv;
+        };
+        unsigned st = next_tile();
+        if (!ok) break;
+        int ks = 0;
+        if (two) {
+          issue_s(S0, 0, st, false, false);
+          issue_s(S1, 1, st, true, n == 1);
+          for (int j = 0; ok && j < n; ++j) {
+            const unsigned sv = ready_v(j, ks);
             if (!ok) break;
-            p_ph[sl] ^= 1;
-            if (first) ++o_uses[sl];
-            tc_fence_after();
-            if (lane == 0) {
-#pragma unroll
-              for (int kc = 0; kc < PA_BN / 16; ++kc)
-                if (kc < ks)
-                  umma_f16_ta(tmem + (uint32_t)(256 + sl * 128), tmem + (uint32_t)(sl * 128 + kc * 8),
-                              umma_desc_sw(bv + kc * 2048, PA_BN * 128, 1024), idesc_o, !first || kc > 0);
-              if (last) umma_commit(&o_full[sl]);
-              if (!two || h == 1) umma_commit(&kv_empty[sv]);
+            issue_pv(S0, sv, ks, j == 0, false, j == n - 1);
+            if (ok && j + 1 < n) {
+              st = next_tile();
+              if (ok) issue_s(S0, 0, st, false, false);
             }
-            __syncwarp();
-            const int jn = j + (two ? 1 : 2);
-            if (jn < n) {
-              if (h == 0) {
-                sk = next_tile();
-                if (!ok) break;
-                tc_fence_after();
-              }
-              issue_s(sl, two ? h : 0, sk, !two || h == 1, jn == n - 1 && (!two || h == 1));
+            if (ok) issue_pv(S1, sv, ks, j == 0, true, j == n - 1);
+            if (ok && j + 1 < n) issue_s(S1, 1, st, true, j + 1 == n - 1);
+          }
+        } else {
+          issue_s(S0, 0, st, true, n == 1);
+          if (n > 1) {
+            st = next_tile();
+            if (ok) issue_s(S1, 0, st, true, n == 2);
+          }
+          auto half = [&](auto slc, int j) {
+            const unsigned sv = ready_v(j, ks);
+            if (ok) issue_pv(slc, sv, ks, j < 2, true, j >= n - 2);
+            if (ok && j + 2 < n) {
+              st = next_tile();
+              if (ok) issue_s(slc, 0, st, true, j + 2 == n - 1);
             }
+          };
+          for (int j = 0; ok && j < n; j += 2) {
+            half(S0, j);
+            if (ok && j + 1 < n) half(S1, j + 1);
           }
         }
       }
