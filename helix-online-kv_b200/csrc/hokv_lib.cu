@@ -968,6 +968,7 @@ static int launch_packed(const PaMaps& maps, const PaP& p, cudaStream_t st) {
   // the combine starts behind the last CTAs of the attention (programmatic launch; it waits for the grid's results)
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
+  cfg.blockDim = dim3(256);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -975,13 +976,12 @@ static int launch_packed(const PaMaps& maps, const PaP& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   cudaError_t e;
   if (p.prefix > 0) {
-    cfg.gridDim = dim3((unsigned)p.T, (unsigned)p.Hkv);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned)p.T, (unsigned)p.Hkv, (unsigned)cdiv(p.G, PA_JOIN));
     e = cudaLaunchKernelEx(&cfg, k_packed_combine_rows<D, T>, p);
   } else {
-    const int64_t most = std::min<int64_t>(p.T, 2 * p.TT) * p.G * (p.D / 4);   // elements of the largest item
-    cfg.gridDim = dim3((unsigned)p.n_ctas, (unsigned)std::min<int64_t>(8, cdiv(most, 256)));
-    cfg.blockDim = dim3(256);
+    const int64_t most = std::min<int64_t>(p.T, 2 * p.TT) * p.G;   // rows of the largest item
+    // few blocks: most items are whole, and a block without one still costs its start
+    cfg.gridDim = dim3((unsigned)p.n_ctas, (unsigned)std::min<int64_t>(8, cdiv(most, PA_JOIN)));
     e = cudaLaunchKernelEx(&cfg, k_packed_combine<D, T>, p);
   }
   if (e != cudaSuccess) {

@@ -691,123 +691,184 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 }
 
 // ---- joining pieces ------------------------------------------------------------
+// A block joins up to PA_JOIN rows of one KV head.  Bound by latency, not
+// bytes: a long key axis cut over every SM leaves dozens of pieces of a few
+// rows each, so the statistics of all pieces are read at once, the weights
+// 2^(m - max m) go through shared memory and the sums run over independent
+// loads.  Pieces are added in CTA order (and, for half the threads' worth of
+// elements, in two interleaved halves): the same result each run.
 
-// Items cut by a share's border, one item per blockIdx.x (the CTA that began
-// it), its rows and 4-dim groups over blockIdx.y and the threads; the pieces
-// are added in CTA order.
-template <int D, typename T>
-__global__ void __launch_bounds__(256) k_packed_combine(const PaP p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ int s_part[256];
-  __shared__ int s_n;
-  const PaDesc d = p.desc[blockIdx.x * 2 + 1];
-  if (!d.valid) return;
-  if (threadIdx.x < 32) {
-    // the pieces of the CTAs after this one, up to the one that ends the item
-    int n = 1;
-    if (threadIdx.x == 0) s_part[0] = blockIdx.x * 2 + 1;
-    for (int c = blockIdx.x + 1; c < p.n_ctas; c += 32) {
-      const int i = c + threadIdx.x;
-      PaDesc e;
-      e.valid = e.end = 0;
-      if (i < p.n_ctas) e = p.desc[i * 2];
-      const unsigned val = __ballot_sync(0xffffffffu, e.valid != 0);
-      const unsigned fin = __ballot_sync(0xffffffffu, e.valid && e.end);
-      const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
-      if (use >> threadIdx.x & 1) s_part[n + __popc(use & ((1u << threadIdx.x) - 1u))] = i * 2;
-      n += __popc(use);
-      if (fin) break;
+constexpr int PA_JOIN = 8;
+constexpr int PA_MAX_PIECES = 256;       // of one source: 240 CTAs at most
+
+template <int PIECES>
+struct PaJoin {
+  int n;                        // pieces
+  int piece[PIECES];            // workspace slot, or -1 - src: the row-wise result of that source
+  int2 prow[PA_JOIN];           // row in a piece, by source of the piece (x: own keys, y: prefix)
+  float m[PIECES * PA_JOIN];               // statistics; m becomes the weight
+  alignas(16) float l[PIECES * PA_JOIN];   // (reused for float4 sums)
+  float inv[PA_JOIN];
+};
+constexpr int PA_SECOND = 1 << 20;       // flag of a slot that holds the prefix's rows
+
+// Appends the pieces of an item begun by CTA `first` (its slot 1, then slot 0
+// of the valid CTAs after it, up to the one that ends it) to j; one warp.
+template <typename Join>
+__device__ __forceinline__ int pa_chain(const PaP& p, Join& j, int n, int first, int flag) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) j.piece[n] = (first * 2 + 1) | flag;
+  ++n;
+  for (int c = first + 1; c < p.n_ctas; c += 32) {
+    const int i = c + lane;
+    int valid = 0, end = 0;
+    if (i < p.n_ctas) {
+      valid = p.desc[i * 2].valid;
+      end = p.desc[i * 2].end;
     }
-    if (threadIdx.x == 0) s_n = n;
+    const unsigned val = __ballot_sync(0xffffffffu, valid != 0);
+    const unsigned fin = __ballot_sync(0xffffffffu, valid && end);
+    const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
+    if (use >> lane & 1) j.piece[n + __popc(use & ((1u << lane) - 1u))] = (i * 2) | flag;
+    n += __popc(use);
+    if (fin) break;
+  }
+  return n;
+}
+
+// Rows [0, rows) of the block: row r is out row `t(r)`, head `h(r)`.
+template <int D, typename T, typename Join, typename RowOf>
+__device__ __forceinline__ void pa_join_rows(const PaP& p, Join& j, int rows, RowOf row_of) {
+  const int n = j.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < n * PA_JOIN; e += 256) {
+    const int r = e % PA_JOIN, at = j.piece[e / PA_JOIN];
+    float2 v = make_float2(-INFINITY, 0.f);
+    if (r < rows) {
+      if (at < 0) {
+        const int2 th = row_of(r);
+        v = p.row_ml[((int64_t)(-1 - at) * p.T + th.x) * p.Hq + th.y];
+      } else {
+        v = p.ml[(int64_t)(at & (PA_SECOND - 1)) * 256 + (at & PA_SECOND ? j.prow[r].y : j.prow[r].x)];
+      }
+    }
+    j.m[e] = v.x;
+    j.l[e] = v.y;
   }
   __syncthreads();
-  const int n = s_n, rows = d.n_tok * p.G, groups = p.D / 4;
-  for (int e = blockIdx.y * 256 + threadIdx.x; e < rows * groups; e += gridDim.y * 256) {
-    const int r = e % rows, d4 = e / rows;
-    const int tok = r / p.G, g = r - tok * p.G;
-    const int tile = tok / p.TT;
-    const int prow = tile * 128 + (tok - tile * p.TT) * p.G + g;
-    float m = -INFINITY;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[(int64_t)s_part[i] * 256 + prow].x);
-    float l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float2 ml = p.ml[(int64_t)s_part[i] * 256 + prow];
-      const float4 o = p.o[((int64_t)s_part[i] * (D / 4) + d4) * 256 + prow];
-      const float f = ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - m);
-      l += ml.y * f;
-      a.x += o.x * f; a.y += o.y * f; a.z += o.z * f; a.w += o.w * f;
+  {   // warp r: the weights of row r
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, j.m[i * PA_JOIN + warp]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = lane; i < n; i += 32) {
+      const float x = j.m[i * PA_JOIN + warp];
+      const float f = x == -INFINITY ? 0.f : pf_ex2(x - m);
+      j.m[i * PA_JOIN + warp] = f;
+      l += j.l[i * PA_JOIN + warp] * f;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* og = reinterpret_cast<T*>(p.out) + (int64_t)(d.tok0 + tok) * p.ost + (int64_t)(d.hk * p.G + g) * p.osh + d4 * 4;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) j.inv[warp] = l == 0.f ? 0.f : 1.f / l;
+  }
+  __syncthreads();
+  constexpr int E = PA_JOIN * (D / 4), HALVES = 256 / E;
+  const int e = threadIdx.x % E, half = threadIdx.x / E, r = e % PA_JOIN, d4 = e / PA_JOIN;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r < rows && d4 * 4 < p.D) {
+    const int2 th = row_of(r);
+    const int2 pr = j.prow[r];
+#pragma unroll 8
+    for (int i = half; i < n; i += HALVES) {
+      const int at = j.piece[i];
+      const float4* src = at < 0 ? p.row_o + (((int64_t)(-1 - at) * p.T + th.x) * p.Hq + th.y) * (D / 4) + d4
+                                 : p.o + ((int64_t)(at & (PA_SECOND - 1)) * (D / 4) + d4) * 256 +
+                                       (at & PA_SECOND ? pr.y : pr.x);
+      const float4 o = *src;
+      const float f = j.m[i * PA_JOIN + r];
+      if (f != 0.f) {   // a part that saw nothing holds no values
+        a.x += o.x * f; a.y += o.y * f; a.z += o.z * f; a.w += o.w * f;
+      }
+    }
+  }
+  if (HALVES == 2) {
+    __syncthreads();
+    float4* other = reinterpret_cast<float4*>(j.l);
+    if (half == 1) other[e] = a;
+    __syncthreads();
+    const float4 b = other[e];
+    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+  }
+  if (half == 0 && r < rows && d4 * 4 < p.D) {
+    const int2 th = row_of(r);
+    const float inv = j.inv[r];
+    T* og = reinterpret_cast<T*>(p.out) + (int64_t)th.x * p.ost + (int64_t)th.y * p.osh + d4 * 4;
     *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
   }
 }
 
-// With a shared prefix every row joins its prefix part and its own part, each
-// one row-wise result or the pieces of a cut item.  Grid (tokens, KV heads).
+__device__ __forceinline__ int pa_piece_row(const PaP& p, int tok, int g) {
+  const int tile = tok / p.TT;
+  return tile * PA_ROWS + (tok - tile * p.TT) * p.G + g;
+}
+
+// Items cut by a share's border: blockIdx.x is the CTA that began the item, its
+// rows are taken PA_JOIN at a time over blockIdx.y.
 template <int D, typename T>
-__global__ void __launch_bounds__(128) k_packed_combine_rows(const PaP p) {
+__global__ void __launch_bounds__(256) k_packed_combine(const PaP p) {
+  __shared__ __align__(16) PaJoin<PA_MAX_PIECES> j;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ int s_part[2][256];   // workspace slots, or -1: the row-wise result
-  __shared__ int s_n[2], s_prow[2];
-  const int t = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int used = pa_used(p);
-  if (t >= used) return;
-  if (warp < 2) {
-    int2 info = p.tok_info[((int64_t)warp * p.T + t) * p.Hkv + hk];
-    info.x = min(max(info.x, -1), p.n_ctas - 1);      // a token that no valid sequence covers has no entry
-    info.y = min(max(info.y, 0), 2 * p.TT - 1);
-    int n = 1;
-    if (info.x < 0) {
-      if (lane == 0) s_part[warp][0] = -1;
-    } else {
-      if (lane == 0) s_part[warp][0] = info.x * 2 + 1;
-      for (int c = info.x + 1; c < p.n_ctas; c += 32) {
-        const int i = c + lane;
-        PaDesc e;
-        e.valid = e.end = 0;
-        if (i < p.n_ctas) e = p.desc[i * 2];
-        const unsigned val = __ballot_sync(0xffffffffu, e.valid != 0);
-        const unsigned fin = __ballot_sync(0xffffffffu, e.valid && e.end);
-        const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
-        if (use >> lane & 1) s_part[warp][n + __popc(use & ((1u << lane) - 1u))] = i * 2;
-        n += __popc(use);
-        if (fin) break;
+  const PaDesc d = p.desc[blockIdx.x * 2 + 1];
+  if (!d.valid) return;
+  if (threadIdx.x < 32) {
+    const int n = pa_chain(p, j, 0, blockIdx.x, 0);
+    if (threadIdx.x == 0) j.n = n;
+  }
+  for (int r0 = blockIdx.y * PA_JOIN; r0 < d.n_tok * p.G; r0 += gridDim.y * PA_JOIN) {
+    const int rows = min(d.n_tok * p.G - r0, PA_JOIN);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      const int r = r0 + threadIdx.x, tok = r / p.G;
+      j.prow[threadIdx.x].x = pa_piece_row(p, tok, r - tok * p.G);
+    }
+    __syncthreads();
+    pa_join_rows<D, T>(p, j, rows, [&](int r) {
+      const int tok = (r0 + r) / p.G;
+      return make_int2(d.tok0 + tok, d.hk * p.G + r0 + r - tok * p.G);
+    });
+  }
+}
+
+// With a shared prefix every row joins its prefix part and its own part, each
+// one row-wise result or the pieces of a cut item.  Grid (tokens, KV heads,
+// heads of a group in steps of PA_JOIN).
+template <int D, typename T>
+__global__ void __launch_bounds__(256) k_packed_combine_rows(const PaP p) {
+  __shared__ __align__(16) PaJoin<2 * PA_MAX_PIECES> j;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int t = blockIdx.x, hk = blockIdx.y, g0 = blockIdx.z * PA_JOIN, rows = min(p.G - g0, PA_JOIN);
+  if (t >= pa_used(p)) return;
+  if (threadIdx.x < 32) {
+    int n = 0;
+    for (int src = 0; src < 2; ++src) {
+      int2 info = p.tok_info[((int64_t)src * p.T + t) * p.Hkv + hk];
+      info.x = min(max(info.x, -1), p.n_ctas - 1);      // a token that no valid sequence covers has no entry
+      info.y = min(max(info.y, 0), 2 * p.TT - 1);
+      if (info.x < 0) {
+        if (threadIdx.x == 0) j.piece[n] = -1 - src;
+        ++n;
+      } else {
+        n = pa_chain(p, j, n, info.x, src ? PA_SECOND : 0);
+      }
+      if (threadIdx.x < rows) {
+        const int r = pa_piece_row(p, info.y, g0 + threadIdx.x);
+        if (src) j.prow[threadIdx.x].y = r;
+        else j.prow[threadIdx.x].x = r;
       }
     }
-    if (lane == 0) {
-      const int tile = info.y / p.TT;
-      s_n[warp] = n;
-      s_prow[warp] = tile * 128 + (info.y - tile * p.TT) * p.G;
-    }
+    if (threadIdx.x == 0) j.n = n;
   }
   __syncthreads();
-  const int groups = p.D / 4;
-  for (int e = threadIdx.x; e < p.G * groups; e += 128) {
-    const int g = e / groups, d4 = e - g * groups, hq = hk * p.G + g;
-    float m = -INFINITY, l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int src = 0; src < 2; ++src) {
-      const int64_t rw = ((int64_t)src * p.T + t) * p.Hq + hq;
-      const int prow = s_prow[src] + g, n = s_n[src];
-      for (int i = 0; i < n; ++i) {
-        const int at = s_part[src][i];
-        const float2 ml = at < 0 ? p.row_ml[rw] : p.ml[(int64_t)at * 256 + prow];
-        const float4 o = at < 0 ? p.row_o[rw * (D / 4) + d4] : p.o[((int64_t)at * (D / 4) + d4) * 256 + prow];
-        const float mn = fmaxf(m, ml.x);
-        const float fa = m == -INFINITY ? 0.f : pf_ex2(m - mn), fb = ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - mn);
-        l = l * fa + ml.y * fb;
-        a.x = a.x * fa + o.x * fb; a.y = a.y * fa + o.y * fb;
-        a.z = a.z * fa + o.z * fb; a.w = a.w * fa + o.w * fb;
-        m = mn;
-      }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* og = reinterpret_cast<T*>(p.out) + (int64_t)t * p.ost + (int64_t)hq * p.osh + d4 * 4;
-    *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-  }
+  pa_join_rows<D, T>(p, j, rows, [&](int r) { return make_int2(t, hk * p.G + g0 + r); });
 }
 
 }  // namespace hokv

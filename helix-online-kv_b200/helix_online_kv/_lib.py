@@ -8,7 +8,6 @@ pure bookkeeping stay usable), but the first call that needs the device raises
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -203,11 +202,44 @@ def stream():
     return _vp(torch.cuda.current_stream().cuda_stream)
 
 
-def on_device(dev):
-    """Context in which `dev` is the current device (nothing to do when it is already)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def raw_stream(index: int) -> int:
+    """Address of the current stream of device `index` (what ``stream`` wraps, without a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class on_device:
+    """Makes device `index` current for a block; nothing to do when it already is."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def signature(t):
+    """What an argument check goes by: everything of a tensor but its data."""
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
+
+
+class Checked(dict):
+    """Checked argument structures by the signatures of a call: a layer of a
+    model makes the same call with other data every step.  Holds no data and no
+    addresses; cleared when it grows past what a program's geometries need."""
+
+    def keep(self, key, value):
+        if len(self) >= 1024:
+            self.clear()
+        self[key] = value
+        return value
 
 
 def ptr(t):

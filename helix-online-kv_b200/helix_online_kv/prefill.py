@@ -96,8 +96,9 @@ def _lengths(t, n: Optional[int], name: str, device) -> None:
         raise ValueError(f"Expected {name} of {n} entries, got {t.shape[0]}")
 
 
-def _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out):
-    """Checked arguments of hokv_packed_attention and the output tensor."""
+def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out, prefix_key,
+                  prefix_value):
+    """hokv_packed_args of these arguments without their addresses, and its workspace bytes."""
     if query.dtype not in _DTYPES or not query.is_cuda or query.dim() != 3:
         raise ValueError(f"Expected f16/bf16 CUDA queries [T, H_q, D], got {tuple(query.shape)} {query.dtype} on "
                          f"{query.device}")
@@ -119,63 +120,99 @@ def _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling,
             raise ValueError("keys in slots [B, H_kv, capacity, D] need kv_len [B] (and no cu_seqlens_k)")
         B = key.shape[0]
         _lengths(kv_len, B, "kv_len", dev)
-        a.kv_len, a.kv_in_slots, a.kv_rows = kv_len.data_ptr(), 1, key.shape[2]
+        a.kv_in_slots, a.kv_rows = 1, key.shape[2]
     else:
         if kv_len is not None:
             raise ValueError("packed keys [S, H_kv, D] take cu_seqlens_k, not kv_len")
         if cu_seqlens_k is None:
-            cu_seqlens_k = cu_seqlens_q
-        if cu_seqlens_k is None:
             raise ValueError("packed keys [S, H_kv, D] need cu_seqlens_k or cu_seqlens_q")
         _lengths(cu_seqlens_k, None, "cu_seqlens_k", dev)
         B = cu_seqlens_k.shape[0] - 1
-        a.cu_seqlens_k, a.kv_rows = cu_seqlens_k.data_ptr(), key.shape[0]
-    if cu_seqlens_q is not None:
-        _lengths(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
-        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
-    elif T != B:
-        raise ValueError(f"without cu_seqlens_q every sequence has one query: got {T} queries for {B} sequences")
+        a.kv_rows = key.shape[0]
     if B < 0:
         raise ValueError("cu_seqlens_k needs at least one entry")
+    if cu_seqlens_q is not None:
+        _lengths(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
+    elif T != B:
+        raise ValueError(f"without cu_seqlens_q every sequence has one query: got {T} queries for {B} sequences")
     scale = float(scaling) if scaling is not None else D ** -0.5
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"Expected a positive finite scaling, got {scaling}")
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1])):
-            raise ValueError(f"Expected {name} with contiguous head dims, strides in multiples of 8 elements and 16-byte "
-                             f"aligned data, got strides {t.stride()}")
+    prefix = (("prefix_key", prefix_key), ("prefix_value", prefix_value)) if prefix_key is not None else ()
+    for name, t in prefix:
+        if t.dim() != 3 or t.shape[0] != Hkv or t.shape[2] != D or t.shape != prefix_key.shape or t.dtype != query.dtype \
+                or t.device != dev:
+            raise ValueError(f"Expected {name} [{Hkv}, P, {D}] {query.dtype} on {dev}, got {tuple(t.shape)} {t.dtype} on "
+                             f"{t.device}")
+    for name, t in (("query", query), ("key", key), ("value", value), *prefix):
+        if t.numel() and (t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1])):
+            raise ValueError(f"Expected {name} with contiguous head dims and strides in multiples of 8 elements, got "
+                             f"strides {t.stride()}")
     if T > 1 and query.stride(0) < (Hq * query.stride(1) if Hq > 1 else D):
         raise ValueError(f"Expected queries [T, H_q, D] whose token stride covers the heads, got strides {query.stride()}")
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=query.dtype, device=dev)
-        a.zero_tail = 1
-    elif (out.shape != query.shape or out.dtype != query.dtype or out.device != dev
-          or (out.numel() and (out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8))):
-        raise ValueError(f"Expected out [{T}, {Hq}, {D}] {query.dtype} on {dev} with contiguous 16-byte aligned rows, got "
-                         f"{tuple(out.shape)} {out.dtype} on {out.device}")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != dev
+                            or (out.numel() and (out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8))):
+        raise ValueError(f"Expected out [{T}, {Hq}, {D}] {query.dtype} on {dev} with contiguous rows and strides in "
+                         f"multiples of 8 elements, got {tuple(out.shape)} {out.dtype} on {out.device}")
     a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim, a.causal = _DTYPES[query.dtype], B, Hq, Hkv, D, bool(is_causal)
-    a.scale, a.n_tokens = scale, T
-    a.q, a.q_stride_t, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
-    a.out, a.out_stride_t, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    a.k, a.v = key.data_ptr(), value.data_ptr()
+    a.scale, a.n_tokens, a.zero_tail = scale, T, out is None
+    a.q_stride_t, a.q_stride_h = query.stride(0), query.stride(1)
+    a.out_stride_t, a.out_stride_h = (Hq * D, D) if out is None else out.stride()[:2]
     if slots:
         a.k_stride_b, a.k_stride_h, a.k_stride_t = key.stride()[:3]
         a.v_stride_b, a.v_stride_h, a.v_stride_t = value.stride()[:3]
     else:
         a.k_stride_t, a.k_stride_h = key.stride()[:2]
         a.v_stride_t, a.v_stride_h = value.stride()[:2]
-    return a, out
+    if prefix:
+        a.pk_stride_h, a.pk_stride_t = prefix_key.stride()[:2]
+        a.pv_stride_h, a.pv_stride_t = prefix_value.stride()[:2]
+        a.prefix_len = prefix_key.shape[1]
+    need = ctypes.c_size_t(0)
+    with L.on_device(dev.index):
+        L.check(L.lib().hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), "packed_attention")
+    return a, need.value
 
 
-def _packed_launch(a, what: str, device) -> None:
-    """Workspace of this call from the allocator, and the launch, on `device`'s current stream."""
-    lib = L.lib()
+_checked = L.Checked()
+
+
+def _packed(what, query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out, prefix_key=None,
+            prefix_value=None):
+    """Check, take the output and this call's workspace from the allocator, launch on the current stream."""
+    if cu_seqlens_k is None and kv_len is None:
+        cu_seqlens_k = cu_seqlens_q
+    sig = L.signature
+    geometry = (sig(query), sig(key), sig(value), sig(cu_seqlens_q), sig(cu_seqlens_k), sig(kv_len), scaling, is_causal,
+                sig(out), sig(prefix_key), sig(prefix_value))
+    known = _checked.get(geometry)
+    if known is None:
+        known = _checked.keep(geometry, _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling,
+                                                      is_causal, out, prefix_key, prefix_value))
+    device = geometry[0][3]
     with L.on_device(device):
-        need = ctypes.c_size_t(0)
-        L.check(lib.hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), what)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-        L.check(lib.hokv_packed_attention(ctypes.byref(a), L.stream()), what)
+        if out is None:
+            out = query.new_empty(query.shape)
+        if not query.numel():
+            return out
+        a = L.PackedArgs.from_buffer_copy(known[0])
+        ws = torch.empty(known[1], dtype=torch.uint8, device=query.device)
+        a.q, a.k, a.v, a.out, a.workspace, a.workspace_bytes = (query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                                                                out.data_ptr(), ws.data_ptr(), known[1])
+        if prefix_key is not None:
+            a.prefix_k, a.prefix_v = prefix_key.data_ptr(), prefix_value.data_ptr()
+        if cu_seqlens_q is not None:
+            a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+        if kv_len is not None:
+            a.kv_len = kv_len.data_ptr()
+        else:
+            a.cu_seqlens_k = cu_seqlens_k.data_ptr()
+        status = L.lib().hokv_packed_attention(ctypes.byref(a), L.raw_stream(device))
+        if status:
+            if status == L.ERR_INVALID:   # what the signatures do not show: addresses
+                raise ValueError(f"{what}: {L.lib().hokv_last_error().decode(errors='replace')}")
+            L.check(status, what)
+    return out
 
 
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -192,7 +229,4 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     dims in multiples of 8 up to 128, contiguous head dims, strides in multiples of 8 elements, H_q a multiple of
     H_kv.  -> [T, H_q, D] in the query's dtype; rows behind the last sequence are zeros, or left as they were in a
     given ``out`` (which must not overlap the inputs)."""
-    a, out = _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)
-    if out.numel():
-        _packed_launch(a, "packed_attention", out.device)
-    return out
+    return _packed("packed_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)

@@ -23,22 +23,9 @@ from .prefill import _lengths
 _DTYPES = {torch.float16: L.F16, torch.bfloat16: L.BF16, torch.float32: L.F32}
 
 
-def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_slots: torch.Tensor,
-                       value_slots: torch.Tensor, cu_seqlens: Optional[torch.Tensor], kv_len: torch.Tensor,
-                       inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
-                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
-                       positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Rotated queries [T, H_q, D]; keys and values appended to their slots.
-
-    query [T, H_q, D], key/value [T, H_kv, D] (contiguous head dims, any other strides: parts of one projection are
-    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]) (cu_seqlens None: token b).  Token i of b sits at
-    position kv_len[b] + i, or positions[t] when given (sequences behind a shared prefix), and its key and value go to
-    row kv_len[b] + i of key_slots/value_slots [B, H_kv, capacity, D].  kv_len (the rows held before the call) is
-    not changed.  With q_weight / k_weight [D] the head is first multiplied by weight / sqrt(mean(x^2) + eps).
-    inv_freq [F] float32, 2F <= D, turns dims (f, f + F), or (2f, 2f + 1) when ``interleaved``, by position *
-    inv_freq[f]; the dims behind 2F keep their values.  f16, bf16 or f32, the same for all but lengths and inv_freq;
-    even head dims up to 256.  ``out`` may be the query itself; rows behind the last sequence are zeros, or left
-    as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
+def _check(query, key, value, key_slots, value_slots, cu_seqlens, kv_len, inv_freq, q_weight, k_weight, eps,
+           interleaved, positions, out):
+    """hokv_norm_rotate_args of these arguments without their addresses."""
     if query.dtype not in _DTYPES or not query.is_cuda or query.dim() != 3:
         raise ValueError(f"Expected f16/bf16/f32 CUDA queries [T, H_q, D], got {tuple(query.shape)} {query.dtype} on "
                          f"{query.device}")
@@ -52,10 +39,6 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     slots = tuple(key_slots.shape)
     if key_slots.dim() != 4 or slots[1] != Hkv or slots[3] != D:
         raise ValueError(f"Expected key_slots [B, {Hkv}, capacity, {D}], got {slots}")
-    if out is None:
-        out, tail = torch.empty((T, Hq, D), dtype=dt, device=dev), 1
-    else:
-        tail = 0
     for name, t, shape in (("query", query, (T, Hq, D)), ("key", key, (T, Hkv, D)), ("value", value, (T, Hkv, D)),
                            ("key_slots", key_slots, slots), ("value_slots", value_slots, slots), ("out", out, (T, Hq, D)),
                            ("q_weight", q_weight, (D,)), ("k_weight", k_weight, (D,))):
@@ -78,23 +61,62 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
                          f"{tuple(inv_freq.shape)} {inv_freq.dtype} on {inv_freq.device}")
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"Expected a finite eps >= 0, got {eps}")
-    if T == 0:
-        return out
     a = L.NormRotateArgs()
     a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim = _DTYPES[dt], B, Hq, Hkv, D
-    a.n_freq, a.interleaved, a.zero_tail, a.eps, a.n_tokens = inv_freq.shape[0], bool(interleaved), tail, eps, T
-    a.q, a.q_stride_t, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
-    a.k, a.k_stride_t, a.k_stride_h = key.data_ptr(), key.stride(0), key.stride(1)
-    a.v, a.v_stride_t, a.v_stride_h = value.data_ptr(), value.stride(0), value.stride(1)
-    a.out, a.out_stride_t, a.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    a.k_slots, a.v_slots, a.capacity = key_slots.data_ptr(), value_slots.data_ptr(), slots[2]
+    a.n_freq, a.interleaved, a.zero_tail, a.eps, a.n_tokens = inv_freq.shape[0], bool(interleaved), out is None, eps, T
+    a.q_stride_t, a.q_stride_h = query.stride()[:2]
+    a.k_stride_t, a.k_stride_h = key.stride()[:2]
+    a.v_stride_t, a.v_stride_h = value.stride()[:2]
+    a.out_stride_t, a.out_stride_h = (Hq * D, D) if out is None else out.stride()[:2]
     a.ks_stride_b, a.ks_stride_h, a.ks_stride_t = key_slots.stride()[:3]
     a.vs_stride_b, a.vs_stride_h, a.vs_stride_t = value_slots.stride()[:3]
-    a.kv_len, a.inv_freq = kv_len.data_ptr(), inv_freq.data_ptr()
-    a.cu_seqlens = cu_seqlens.data_ptr() if cu_seqlens is not None else None
-    a.positions = positions.data_ptr() if positions is not None else None
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    with L.on_device(dev):
-        L.check(L.lib().hokv_norm_rotate_append(ctypes.byref(a), L.stream()), "norm_rotate_append")
+    a.capacity = slots[2]
+    return a
+
+
+_checked = L.Checked()
+
+
+def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_slots: torch.Tensor,
+                       value_slots: torch.Tensor, cu_seqlens: Optional[torch.Tensor], kv_len: torch.Tensor,
+                       inv_freq: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                       positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotated queries [T, H_q, D]; keys and values appended to their slots.
+
+    query [T, H_q, D], key/value [T, H_kv, D] (contiguous head dims, any other strides: parts of one projection are
+    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]) (cu_seqlens None: token b).  Token i of b sits at
+    position kv_len[b] + i, or positions[t] when given (sequences behind a shared prefix), and its key and value go to
+    row kv_len[b] + i of key_slots/value_slots [B, H_kv, capacity, D].  kv_len (the rows held before the call) is
+    not changed.  With q_weight / k_weight [D] the head is first multiplied by weight / sqrt(mean(x^2) + eps).
+    inv_freq [F] float32, 2F <= D, turns dims (f, f + F), or (2f, 2f + 1) when ``interleaved``, by position *
+    inv_freq[f]; the dims behind 2F keep their values.  f16, bf16 or f32, the same for all but lengths and inv_freq;
+    even head dims up to 256.  ``out`` may be the query itself; rows behind the last sequence are zeros, or left
+    as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
+    sig = L.signature
+    geometry = (sig(query), sig(key), sig(value), sig(key_slots), sig(value_slots), sig(cu_seqlens), sig(kv_len),
+                sig(inv_freq), sig(q_weight), sig(k_weight), eps, interleaved, sig(positions), sig(out))
+    known = _checked.get(geometry)
+    if known is None:
+        known = _checked.keep(geometry, _check(query, key, value, key_slots, value_slots, cu_seqlens, kv_len, inv_freq,
+                                               q_weight, k_weight, eps, interleaved, positions, out))
+    device = geometry[0][3]
+    with L.on_device(device):
+        if out is None:
+            out = query.new_empty(query.shape)
+        if not known.n_tokens:
+            return out
+        a = L.NormRotateArgs.from_buffer_copy(known)
+        a.q, a.k, a.v, a.out, a.k_slots, a.v_slots, a.kv_len, a.inv_freq = (
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(), key_slots.data_ptr(),
+            value_slots.data_ptr(), kv_len.data_ptr(), inv_freq.data_ptr())
+        if cu_seqlens is not None:
+            a.cu_seqlens = cu_seqlens.data_ptr()
+        if positions is not None:
+            a.positions = positions.data_ptr()
+        if q_weight is not None:
+            a.q_weight = q_weight.data_ptr()
+        if k_weight is not None:
+            a.k_weight = k_weight.data_ptr()
+        L.check(L.lib().hokv_norm_rotate_append(ctypes.byref(a), L.raw_stream(device)), "norm_rotate_append")
     return out

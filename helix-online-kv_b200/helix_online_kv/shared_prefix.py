@@ -17,7 +17,7 @@ from typing import Optional
 
 import torch
 
-from .prefill import _packed_args, _packed_launch
+from .prefill import _packed
 
 
 def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value: torch.Tensor,
@@ -32,19 +32,5 @@ def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefi
     [B, H_kv, capacity, D] with kv_len [B], or packed [S, H_kv, D] with cu_seqlens_k, causal among its own keys (query i
     of m sits at own position n - m + i).  -> [T, H_q, D].  Scratch grows with T (about 8 H_q D bytes per token), so
     this form is for decoding and drafted tokens, not for long prompts behind a prefix."""
-    a, out = _packed_args(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)
-    _, Hq, D = query.shape
-    want = (key.shape[1], prefix_key.shape[1] if prefix_key.dim() == 3 else -1, D)
-    for name, t in (("prefix_key", prefix_key), ("prefix_value", prefix_value)):
-        if t.dim() != 3 or tuple(t.shape) != want or t.dtype != query.dtype or t.device != query.device:
-            raise ValueError(f"Expected {name} [{key.shape[1]}, P, {D}] {query.dtype} on {query.device}, got "
-                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
-        if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(1) % 8):
-            raise ValueError(f"Expected {name} with contiguous head dims, strides in multiples of 8 elements and 16-byte "
-                             f"aligned data, got strides {t.stride()}")
-    a.prefix_k, a.pk_stride_h, a.pk_stride_t = prefix_key.data_ptr(), prefix_key.stride(0), prefix_key.stride(1)
-    a.prefix_v, a.pv_stride_h, a.pv_stride_t = prefix_value.data_ptr(), prefix_value.stride(0), prefix_value.stride(1)
-    a.prefix_len = prefix_key.shape[1]
-    if out.numel():
-        _packed_launch(a, "shared_prefix_attention", out.device)
-    return out
+    return _packed("shared_prefix_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal,
+                   out, prefix_key, prefix_value)

@@ -130,6 +130,9 @@ def test_python_refusals():
         args.update(kw)
         with pytest.raises(ValueError, match=text):
             packed_attention(**args)
+    off = z(4 * 8 * 64 + 8)[1:-7].view(4, 8, 64)   # rows that start between 16-byte boundaries
+    with pytest.raises(ValueError, match="aligned"):
+        packed_attention(off, k, k, cu)
     with pytest.raises(ValueError, match="one query"):
         packed_attention(q, slots, slots, kv_len=n1)
     for pk in (z(2, 9, 32), z(3, 9, 64), z(2, 9, 64, dtype=torch.bfloat16), z(9, 64), z(2, 9, 65)[:, :, :64]):
