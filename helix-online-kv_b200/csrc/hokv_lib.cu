@@ -1024,24 +1024,32 @@ static int packed_attention(const hokv_packed_args* a, void* stream) {
   p.TT = PA_ROWS / p.G;
   p.D = a->head_dim;
   const int64_t T = a->n_tokens;
-  // queries as (dim, head in group, KV head, token): a box is TT tokens x G heads, token-major rows
-  {
-    const int64_t need_t = (int64_t)a->q_heads * (a->q_heads > 1 ? a->q_stride_h : a->head_dim);
-    HOKV_REQUIRE(a->q_heads == 1 || a->q_stride_h >= a->head_dim, "packed_attention: query heads overlap");
-    HOKV_REQUIRE(T == 1 || a->q_stride_t >= need_t, "packed_attention: the query's token stride %lld must cover its heads (%lld)",
-                 (long long)a->q_stride_t, (long long)need_t);
-    PfEncodeFn enc = pf_encoder();
-    if (!enc) return fail(HOKV_ERR_CUDA, "packed_attention: cuTensorMapEncodeTiled unavailable");
-    const int64_t sh = a->q_heads > 1 ? a->q_stride_h : a->head_dim, stt = T > 1 ? a->q_stride_t : need_t;
+  // queries and outputs as (dim, head in group, KV head, token): a box is some tokens x G heads, token-major rows
+  PfEncodeFn enc = pf_encoder();
+  if (!enc) return fail(HOKV_ERR_CUDA, "packed_attention: cuTensorMapEncodeTiled unavailable");
+  auto rows_map = [&](CUtensorMap* m, const void* base, int64_t sh, int64_t stt, int tokens) {
     cuuint64_t gdim[4] = {(cuuint64_t)p.D, (cuuint64_t)p.G, (cuuint64_t)a->kv_heads, (cuuint64_t)T};
     cuuint64_t gstr[3] = {(cuuint64_t)sh * 2, (cuuint64_t)(sh * p.G) * 2, (cuuint64_t)stt * 2};
-    cuuint32_t es[4] = {1, 1, 1, 1}, bx[4] = {64, (cuuint32_t)p.G, 1, (cuuint32_t)p.TT};
-    const CUresult r =
-        enc(&maps.q, a->dtype == HOKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-            const_cast<void*>(a->q), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint32_t es[4] = {1, 1, 1, 1}, bx[4] = {64, (cuuint32_t)p.G, 1, (cuuint32_t)tokens};
+    return enc(m, a->dtype == HOKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+               const_cast<void*>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  {
+    const int64_t sh = a->q_heads > 1 ? a->q_stride_h : a->head_dim, need_t = a->q_heads * sh;
+    HOKV_REQUIRE(sh >= a->head_dim, "packed_attention: query heads overlap");
+    HOKV_REQUIRE(T == 1 || a->q_stride_t >= need_t, "packed_attention: the query's token stride %lld must cover its heads (%lld)",
+                 (long long)a->q_stride_t, (long long)need_t);
+    const CUresult r = rows_map(&maps.q, a->q, sh, T > 1 ? a->q_stride_t : need_t, p.TT);
     if (r != CUDA_SUCCESS)
       return fail(HOKV_ERR_UNSUPPORTED, "packed_attention: query tensor map encode failed (%d)", (int)r);
+  }
+  {   // outputs: 32 rows of whole tokens, where the strides nest
+    const int64_t sh = a->q_heads > 1 ? a->out_stride_h : a->head_dim, need_t = a->q_heads * sh;
+    p.tma_out = 32 % p.G == 0 && sh >= a->head_dim && (T == 1 || a->out_stride_t >= need_t) ? 32 / p.G : 0;
+    maps.out = maps.q;
+    if (p.tma_out && rows_map(&maps.out, a->out, sh, T > 1 ? a->out_stride_t : need_t, p.tma_out) != CUDA_SUCCESS)
+      p.tma_out = 0;
   }
   const bool keys = rows_k > 0;   // without a single key row the maps are never used
   if (keys) {

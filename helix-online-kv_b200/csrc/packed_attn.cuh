@@ -13,12 +13,11 @@
 // (up to 2 TT query tokens, one KV head) against its key tiles of 128 tokens.
 //
 // Work split.  Lengths live on the device only; every CTA derives the same
-// schedule from them.  An item costs PA_ITEM units plus 2 per key tile (1 when
-// its tokens fit one 128-row tile); the units of all items form one line,
-// (sequence, token pair, KV head) in order, which the CTAs (one per SM) cut
-// into equal shares.  An item cut by a share's border leaves pieces (running
-// maximum, sum and unnormalised output, fp32) in the workspace, which
-// k_packed_combine joins in CTA order: no atomics, the same result each run.
+// schedule from them (packed_schedule.cuh): the work of all items forms one
+// line that the CTAs, one per SM, cut into equal shares.  An item cut by a
+// share's border leaves pieces (running maximum, sum and unnormalised output,
+// fp32) in the workspace, which k_packed_combine joins in CTA order: no
+// atomics, the same result each run.
 //
 // One CTA, 384 threads: warps 0-3 and 4-7 are the softmax of tile slots 0 and
 // 1 (a thread owns a row), warp 8 loads (TMA), warp 9 issues the MMAs, warp
@@ -49,7 +48,7 @@ namespace hokv {
 constexpr int PA_THREADS = 384;
 constexpr int PA_ROWS = 128;        // rows of a tile
 constexpr int PA_QUEUE = 4;         // item descriptors in flight
-constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;   // 256 * 208 + 128 * 88 = 384 * 168
+constexpr int PA_REGS_SOFTMAX = 224, PA_REGS_OTHER = 56;   // 256 * 224 + 128 * 56 = 384 * 168
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
 template <int D>
@@ -57,8 +56,9 @@ struct PaGeo {
   static constexpr int NB = D / 64;                       // 64-dim column blocks
   static constexpr int Q_BYTES = PA_ROWS * D * 2;         // one query tile
   static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
-  static constexpr int STAGES = D == 64 ? 8 : 5;          // ring of K and V tiles
-  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + 2048;
+  static constexpr int STAGES = D == 64 ? 8 : 4;          // ring of K and V tiles
+  static constexpr int OUT_BYTES = 8 * 4096;              // 32 rows x 64 dims of O per softmax warp, on their way out
+  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + OUT_BYTES + 2048;
 };
 
 // Piece descriptors of a CTA: [0] the piece that continues an earlier CTA's
@@ -68,13 +68,13 @@ struct PaDesc {
 };
 
 struct alignas(64) PaMaps {
-  CUtensorMap q, k, v, pk, pv;
+  CUtensorMap q, k, v, out, pk, pv;
 };
 
 struct PaP : PaSched {
   void* out;
   int64_t ost, osh;              // output element strides (token, head)
-  int Hq, G, D, zero_tail;
+  int Hq, G, D, zero_tail, tma_out;   // tma_out: tokens of a warp's 32 rows, 0 when they are not whole tokens
   float sl2;                     // scale * log2(e)
   int k_t, k_h, k_b, v_t, v_h, v_b, pk_t, pk_h, pk_b, pv_t, pv_h, pv_b;   // coordinate slots of the maps
   PaDesc* desc;                  // [n_ctas][2]
@@ -91,16 +91,15 @@ struct PaP : PaSched {
 // aborted, and every other wait of the CTA then ends too.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
   const uint32_t a = smem_u32(bar);
-  const uint32_t hint_ns = 20000u;
   unsigned long long t0 = 0;
   for (int i = 0;; ++i) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done)
-        : "r"(a), "r"(parity), "r"(hint_ns)
+        : "r"(a), "r"(parity)
         : "memory");
     if (done) return true;
     if (*abort_flag) return false;
@@ -179,6 +178,12 @@ __device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));   // NaN wins
+  return d;
+}
+
 // One 32-byte store (a whole sector): a thread's row of O.
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t* u) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
@@ -196,7 +201,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   extern __shared__ __align__(1024) unsigned char pa_smem[];
   unsigned char* sQ = pa_smem;
   unsigned char* sKV = sQ + 2 * PG::Q_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + ST * PG::KV_BYTES);
+  unsigned char* sOut = sKV + ST * PG::KV_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + PG::OUT_BYTES);
   uint64_t* q_full = bars;                 // TMA bytes
   uint64_t* q_empty = bars + 1;            // MMA commit after the item's last S
   uint64_t* s_full = bars + 2;             // [2] MMA commit
@@ -291,22 +297,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
-          const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.sl2;
-          const bool grow = mt > m_run + 8.f || (m_run == -INFINITY && mt > -INFINITY);
-          const float m_new = grow ? mt : m_run;
+          for (int j = 0; j < 128; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[j], v[j + 1]);
+          const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
+          const bool grow = !(mt <= m_run + 8.f);   // also for NaN, and for the first key a row sees
           if (i > 0 && __any_sync(0xffffffffu, grow)) {
             // O was last written by this slot's previous P V, complete before this S
-            const float f = grow ? pf_ex2(m_run - m_new) : 1.f;
+            const float f = grow ? pf_ex2(m_run - mt) : 1.f;
             l_run *= f;
 #pragma unroll 1
             for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
             tmem_wait_st();
           }
-          m_run = m_new;
+          if (grow) m_run = mt + (mt - mt);         // an infinite maximum gives NaN, as inf - inf does
           const float nm = m_run == -INFINITY ? 0.f : -m_run;
           const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
-          float2 acc = make_float2(0.f, 0.f);
+          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t pk[32];
@@ -314,12 +319,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             for (int j = 0; j < 32; ++j) {
               const float2 a = __ffma2_rn(make_float2(v[h * 64 + 2 * j], v[h * 64 + 2 * j + 1]), s2, n2);
               const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
-              acc = __fadd2_rn(acc, e);
+              acc[j & 1] = __fadd2_rn(acc[j & 1], e);
               pk[j] = pack2<T>(e.x, e.y);
             }
             tmem_st32_nw(s_addr + h * 32, pk);
           }
-          l_run += acc.x + acc.y;
+          acc[0] = __fadd2_rn(acc[0], acc[1]);
+          l_run += acc[0].x + acc[0].y;
           tmem_wait_st();
         }
         tc_fence_before();
@@ -369,7 +375,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         else p.row_ml[((int64_t)src * p.T + t) * p.Hq + hq] = make_float2(m_run, l_run);
       }
       if (warp_ok) {
-#pragma unroll
+        // whole rows of whole tokens leave through shared memory (128-byte swizzled) and TMA; a warp with rows of
+        // no token (a sequence's end, groups that do not divide 32) stores its own rows, 32 bytes at a time
+        const bool bulk = out_mode == PA_DIRECT && p.tma_out > 0 && __all_sync(0xffffffffu, row_ok);
+        unsigned char* stage = sOut + warp * 4096 + lane * 128;
+#pragma unroll 1   // short code: an item's end is often its first use
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
           if (n > 0) {
@@ -385,31 +395,51 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0.f;
           }
-          if (row_ok) {
-            if (out_mode == PA_DIRECT) {
-              T* og = reinterpret_cast<T*>(p.out) + t * p.ost + hq * p.osh;
-              uint32_t u[16];
+          if (out_mode == PA_DIRECT) {
+            uint32_t u[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) u[j] = pack2<T>(o[2 * j] * inv, o[2 * j + 1] * inv);
+            for (int j = 0; j < 16; ++j) u[j] = pack2<T>(o[2 * j] * inv, o[2 * j + 1] * inv);
+            if (bulk) {
+              if ((c & 1) == 0) {   // the last copy has read the stage
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(stage + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) =
+                    make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+              if (c & 1) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  asm volatile(
+                      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(&maps.out),
+                      "r"((c >> 1) * 64), "r"(0), "r"(w.hk), "r"((int)t), "r"(smem_u32(stage))
+                      : "memory");
+                  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+              }
+            } else if (row_ok) {
+              T* og = reinterpret_cast<T*>(p.out) + t * p.ost + hq * p.osh + c * 32;
               if (wide) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 8)
-                  if (c * 32 + 2 * j < p.D) st_global_32(og + c * 32 + 2 * j, &u[j]);
+                  if (c * 32 + 2 * j < p.D) st_global_32(og + 2 * j, &u[j]);
               } else {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4)
                   if (c * 32 + 2 * j < p.D)
-                    *reinterpret_cast<uint4*>(og + c * 32 + 2 * j) = make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
+                    *reinterpret_cast<uint4*>(og + 2 * j) = make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
               }
-            } else {
-              const bool piece = out_mode == PA_PIECE;
-              float4* base = piece ? p.o + ((int64_t)out_at * (D / 4)) * 256 + prow
-                                   : p.row_o + (((int64_t)src * p.T + t) * p.Hq + hq) * (D / 4);
-              const int step = piece ? 256 : 1;
-#pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                base[(c * 8 + j / 4) * step] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
+          } else if (row_ok) {
+            const bool piece = out_mode == PA_PIECE;
+            float4* base = piece ? p.o + ((int64_t)out_at * (D / 4)) * 256 + prow
+                                 : p.row_o + (((int64_t)src * p.T + t) * p.Hq + hq) * (D / 4);
+            const int step = piece ? 256 : 1;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              base[(c * 8 + j / 4) * step] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         }
       }
@@ -423,6 +453,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       }
       item_done();
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the last rows are written
     if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
       const int used = pa_used(p);
       const int64_t total = (int64_t)(p.T - used) * p.Hq * p.D;
@@ -435,53 +466,69 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
     if (warp == 8) {
-      // ---- loads (lane 0): the item's query tiles, then K and V in the order of use ----
-      if (lane == 0) {
-        unsigned ring = 0, q_uses = 0;
-        bool ok = true;
-        for (int it = 0; ok; ++it) {
-          const int qi = it % PA_QUEUE;
-          if (!pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag)) break;
-          const PaItem w = queue[qi];
-          pa_arrive(&it_empty[qi]);
-          if (w.out_mode == PA_STOP) break;
-          const int n = w.j1 - w.j0;
-          if (n == 0) continue;
-          const bool two = w.n_tok > TT;
-          if (q_uses > 0 && !pa_wait(q_empty, (q_uses - 1) & 1, abort_flag)) break;
-          ++q_uses;
+      // ---- loads: the item's query tiles, then K and V in the order of use ------------
+      const int used = p.prefix > 0 ? 6 : 4;
+      if (lane < used) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps) + lane * sizeof(CUtensorMap)) : "memory");
+      unsigned stage = 0, stage_ph = 1, loads = 0, q_ph = 1, q_uses = 0;
+      bool ok = true;
+      auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
+      for (int it = 0; ok; ++it) {
+        const int qi = it % PA_QUEUE;
+        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
+        if (!ok) break;
+        const int mode = uniform(queue[qi].out_mode), n = uniform(queue[qi].j1 - queue[qi].j0),
+                  two = uniform(queue[qi].n_tok > TT), src = uniform(queue[qi].src), hk = uniform(queue[qi].hk),
+                  tok0 = uniform(queue[qi].tok0), slot = uniform(queue[qi].slot),
+                  row0 = uniform(queue[qi].row0 + queue[qi].j0 * PA_BN);
+        __syncwarp();
+        if (lane == 0) pa_arrive(&it_empty[qi]);
+        if (mode == PA_STOP) break;
+        if (n == 0) continue;
+        ok = all(pa_wait(q_empty, q_ph, abort_flag));   // passes at once the first time
+        if (!ok) break;
+        q_ph ^= 1;
+        ++q_uses;
+        if (elect_one()) {
           pf_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * PG::NB * TT * G * 128));
           for (int t = 0; t < (two ? 2 : 1); ++t)
 #pragma unroll
             for (int a = 0; a < PG::NB; ++a)
-              pf_tma4(sQ + t * PG::Q_BYTES + a * PA_ROWS * 128, &maps.q, a * 64, 0, w.hk, w.tok0 + t * TT, q_full);
-          const CUtensorMap* mk = w.src ? &maps.pk : &maps.k;
-          const CUtensorMap* mv = w.src ? &maps.pv : &maps.v;
-          auto load = [&](bool is_v, int j) {
-            const unsigned st = ring % ST, use = ring / ST;
-            if (use > 0 && !pa_wait(&kv_empty[st], (use - 1) & 1, abort_flag)) return false;
-            ++ring;
-            int c[4];
-            const int row = w.row0 + (w.j0 + j) * PA_BN;
-            if (is_v) pf_coords(w.src ? p.pv_t : p.v_t, w.src ? p.pv_h : p.v_h, w.src ? p.pv_b : p.v_b, row, w.hk, w.slot, c);
-            else pf_coords(w.src ? p.pk_t : p.k_t, w.src ? p.pk_h : p.k_h, w.src ? p.pk_b : p.k_b, row, w.hk, w.slot, c);
-            pf_expect_tx(&kv_full[st], PG::KV_BYTES);
+              pf_tma4(sQ + t * PG::Q_BYTES + a * PA_ROWS * 128, &maps.q, a * 64, 0, hk, tok0 + t * TT, q_full);
+        }
+        __syncwarp();
+        auto load = [&](const CUtensorMap* m, int at_t, int at_h, int j) {
+          ok = all(pa_wait(&kv_empty[stage], stage_ph, abort_flag));
+          if (!ok) return;
+          const int row = row0 + j * PA_BN;
+          const int c1 = at_t == 1 ? row : at_h == 1 ? hk : slot, c2 = at_t == 2 ? row : at_h == 2 ? hk : slot,
+                    c3 = at_t == 3 ? row : at_h == 3 ? hk : slot;
+          if (elect_one()) {
+            pf_expect_tx(&kv_full[stage], PG::KV_BYTES);
 #pragma unroll
             for (int a = 0; a < PG::NB; ++a)
-              pf_tma4(sKV + st * PG::KV_BYTES + a * PA_BN * 128, is_v ? mv : mk, a * 64, c[1], c[2], c[3], &kv_full[st]);
-            return true;
-          };
-          const int ahead = two ? 1 : 2;
-          for (int j = 0; ok && j < min(ahead, n); ++j) ok = load(false, j);
-          for (int j = 0; ok && j < n; ++j) {
-            ok = load(true, j);
-            if (ok && j + ahead < n) ok = load(false, j + ahead);
+              pf_tma4(sKV + stage * PG::KV_BYTES + a * PA_BN * 128, m, a * 64, c1, c2, c3, &kv_full[stage]);
           }
+          __syncwarp();
+          ++loads;
+          if (++stage == ST) stage = 0, stage_ph ^= 1;
+        };
+        auto load_k = [&](int j) {
+          if (src) load(&maps.pk, p.pk_t, p.pk_h, j);
+          else load(&maps.k, p.k_t, p.k_h, j);
+        };
+        auto load_v = [&](int j) {
+          if (src) load(&maps.pv, p.pv_t, p.pv_h, j);
+          else load(&maps.v, p.v_t, p.v_h, j);
+        };
+        const int ahead = two ? 1 : 2;
+        for (int j = -ahead; ok && j < n; ++j) {
+          if (j >= 0) load_v(j);
+          if (ok && j + ahead < n) load_k(j + ahead);
         }
-        if (*abort_flag) {   // gave up: the copies in flight land before the CTA ends
-          for (unsigned k = ring > ST ? ring - ST : 0; k < ring; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
-          if (q_uses > 0) (void)mbar_wait(q_full, (q_uses - 1) & 1);
-        }
+      }
+      if (*abort_flag) {   // gave up: the copies in flight land before the CTA ends
+        for (unsigned k = loads > ST ? loads - ST : 0; k < loads; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
+        if (q_uses > 0) (void)mbar_wait(q_full, (q_uses - 1) & 1);
       }
     } else if (warp == 9) {
       // ---- MMA issue --------------------------------------------------------------

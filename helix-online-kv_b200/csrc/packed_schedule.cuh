@@ -1,12 +1,13 @@
 // packed_schedule.cuh -- how the packed attention cuts its work over the CTAs.
 //
-// An item is up to 2 TT query tokens of one sequence and one KV head (a token
-// pair of tiles, TT = 128 / G tokens each) against the key tiles it sees.  It
-// costs PA_ITEM units plus 2 per key tile, 1 when its tokens fit one tile.  The
+// An item is up to 2 TT query tokens of one sequence and one KV head (a pair of
+// 128-row tiles, TT = 128 / G tokens each) against the keys it sees.  It costs
+// PA_ITEM units plus 2 per visible key, 1 when its tokens fit one tile.  The
 // units of all items, ordered by (sequence, pair, KV head), form one line; CTA
-// c takes units [c, c + 1) * share.  A border inside an item cuts it at a key
-// tile into pieces.  The units before a pair have a closed form (a lattice
-// sum), so a CTA finds its first item without walking the others.
+// c takes units [c, c + 1) * share.  A border inside an item cuts it between
+// two key tiles into pieces.  The units before a pair are an arithmetic
+// series, so a CTA finds its first item without walking the others, and with
+// few instructions: a short call waits for this code from cold caches.
 //
 // Plain C++ apart from the HD marks, so the host can check the same code.
 #pragma once
@@ -15,8 +16,8 @@
 namespace hokv {
 
 constexpr int PA_BN = 128;          // keys of a tile
-constexpr int PA_ITEM = 2;          // units of an item besides its tiles (start and epilogue)
-constexpr int PA_MIN_SHARE = 4;     // smallest share of a CTA: an item's start and two key tiles of a one-tile item
+constexpr int PA_ITEM = 256;        // units of an item besides its keys (start and epilogue): one two-tile key tile
+constexpr int PA_MIN_SHARE = 512;   // smallest share of a CTA: an item's start and two key tiles of a one-tile item
 
 enum { PA_DIRECT = 0, PA_PIECE = 1, PA_ROWWISE = 2, PA_STOP = 3 };
 
@@ -91,58 +92,41 @@ HD PaSeq pa_seq(const PaSched& p, int s) {
   return r;
 }
 
-// sum_{i < n} floor((a i + b) / 128), a and b >= 0: lattice points below a
-// line, by the Euclidean recursion.
-HD int64_t pa_floor_sum(int64_t n, int64_t a, int64_t b) {
-  int64_t m = PA_BN, ans = 0;
-  while (n > 0) {
-    ans += n * (n - 1) / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const int64_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const int64_t t = m;
-    m = a;
-    a = t;
-  }
-  return ans;
-}
-
-// Key tiles that token pair `pr` (W = 2 TT tokens) of a sequence sees.
-HD int pa_tiles(const PaSeq& s, int W, int pr) {
-  const int64_t e = s.causal ? (int64_t)s.kv - s.nq + pa_min((int64_t)(pr + 1) * W, s.nq) : s.kv;
-  return e <= 0 ? 0 : (int)((e + PA_BN - 1) / PA_BN);
+// Keys that token pair `pr` (W = 2 TT tokens) of a sequence sees.
+HD int pa_keys(const PaSeq& s, int W, int pr) {
+  if (!s.causal) return s.kv;
+  const int last = s.nq - pr * W < W ? s.nq : (pr + 1) * W;
+  return (int)pa_max(s.kv - s.nq + last, 0);
 }
 
 // Units, of one KV head, of the first n pairs (none of them the last).
-HD int64_t pa_units_before(const PaSeq& s, int W, int64_t n) {
-  int64_t tiles;
-  if (!s.causal) {
-    tiles = n * ((s.kv + PA_BN - 1) / PA_BN);
-  } else {
+HD int64_t pa_units_before(const PaSeq& s, int W, int n) {
+  int64_t keys = (int64_t)n * s.kv;
+  if (s.causal) {
     const int64_t off = (int64_t)s.kv - s.nq;
-    const int64_t skip = off < 0 ? pa_min(n, -off / W) : 0;   // pairs that see nothing
-    tiles = pa_floor_sum(n - skip, W, off + (skip + 1) * W + PA_BN - 1);
+    const int skip = off < 0 ? (int)pa_min(n, (int)-off / W) : 0;   // pairs that see nothing
+    const int64_t m = n - skip;
+    keys = m * off + W * (m * (m + 1) / 2 + m * skip);
   }
-  return n * PA_ITEM + 2 * tiles;
+  return (int64_t)n * PA_ITEM + 2 * keys;
 }
 
 // Units of one KV head's item of pair `pr`.
-HD int pa_item_units(const PaSeq& s, int W, int pr) {
-  return PA_ITEM + (s.nq - pr * W > W / 2 ? 2 : 1) * pa_tiles(s, W, pr);
+HD int64_t pa_item_units(const PaSeq& s, int W, int pr) {
+  return PA_ITEM + ((int64_t)pa_keys(s, W, pr) << (s.nq - pr * W > W / 2 ? 1 : 0));
 }
 
 HD int64_t pa_seq_units(const PaSched& p, const PaSeq& s) {
   const int W = 2 * p.TT;
   if (s.nq <= 0) return 0;
-  const int np = (s.nq + W - 1) / W;
-  return (int64_t)p.Hkv * (pa_units_before(s, W, np - 1) + pa_item_units(s, W, np - 1));
+  const int last = (s.nq + W - 1) / W - 1;
+  return (int64_t)p.Hkv * (pa_units_before(s, W, last) + pa_item_units(s, W, last));
 }
 
+// A share of at least total / n_ctas (the same value in every CTA; the product
+// is off by less than 1).
 HD int64_t pa_share(const PaSched& p, int64_t total) {
-  return pa_max((total + p.n_ctas - 1) / p.n_ctas, PA_MIN_SHARE);
+  return pa_max((int64_t)((double)total * (1.0 / p.n_ctas)) + 1, PA_MIN_SHARE);
 }
 
 // The sequence of [lo, hi) that holds unit `unit`; `at`: units before lo, on
@@ -171,29 +155,32 @@ HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, in
     const int np = (q.nq + W - 1) / W;
     int pr = 0;
     if (pos > at) {   // the last pair that starts at or before pos
-      int lo = 0, hi = np - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (at + (int64_t)p.Hkv * pa_units_before(q, W, mid) <= pos) lo = mid;
+      int hi = np - 1;
+      while (pr < hi) {
+        const int mid = (pr + hi + 1) >> 1;
+        if (at + (int64_t)p.Hkv * pa_units_before(q, W, mid) <= pos) pr = mid;
         else hi = mid - 1;
       }
-      pr = lo;
     }
-    int64_t pair_at = at + (int64_t)p.Hkv * pa_units_before(q, W, pr);
+    int64_t item_at = at + (int64_t)p.Hkv * pa_units_before(q, W, pr);
     for (; pr < np && pos < end; ++pr) {
       const int left = q.nq - pr * W;
       const int n_tok = left < W ? left : W;
-      const int tiles = pa_tiles(q, W, pr);
-      const int wt = n_tok > p.TT ? 2 : 1;
-      const int iu = PA_ITEM + wt * tiles;
-      for (int hk = (int)((pos - pair_at) / iu); hk < p.Hkv && pos < end; ++hk) {
-        const int64_t item_at = pair_at + (int64_t)hk * iu;
-        const int x0 = (int)(pos - item_at), x1 = (int)pa_min(iu, end - item_at);
+      const int keys = pa_keys(q, W, pr);
+      const int tiles = (keys + PA_BN - 1) / PA_BN;
+      const int sh = n_tok > p.TT ? 8 : 7;          // units of a key tile: 2^sh
+      const int64_t iu = pa_item_units(q, W, pr);
+      for (int hk = 0; hk < p.Hkv; ++hk, item_at += iu) {
+        if (item_at + iu <= pos) continue;
+        if (pos >= end) break;
         // a tile belongs to the piece in which its units start
-        const int t0 = x0 <= PA_ITEM ? 0 : (int)pa_min((x0 - PA_ITEM + wt - 1) / wt, tiles);
-        const int t1 = x1 == iu ? tiles : x1 <= PA_ITEM ? 0 : (int)pa_min((x1 - PA_ITEM + wt - 1) / wt, tiles);
-        pos = item_at + x1;
-        if (tiles > 0 ? t0 == t1 : x0 != 0) continue;
+        const int64_t x0 = pos - item_at - PA_ITEM, x1 = end - item_at - PA_ITEM;
+        const int64_t mask = ((int64_t)1 << sh) - 1;
+        const int t0 = x0 <= 0 ? 0 : (int)pa_min((x0 + mask) >> sh, tiles);
+        const int t1 = x1 <= 0 ? 0 : (int)pa_min((x1 + mask) >> sh, tiles);
+        const bool start = pos == item_at;
+        pos = pa_min(item_at + iu, end);
+        if (tiles > 0 ? t0 == t1 : !start) continue;
         PaItem w;
         w.tok0 = q.q0 + pr * W;
         w.n_tok = n_tok;
@@ -211,7 +198,6 @@ HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, in
         w.out_at = cta * 2 + (begins ? 1 : 0);
         if (!emit(w, begins, ends)) return false;
       }
-      pair_at += (int64_t)p.Hkv * iu;
     }
     at += units;
   }

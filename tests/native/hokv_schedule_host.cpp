@@ -5,8 +5,6 @@ using namespace hokv;
 
 extern "C" {
 
-int64_t host_floor_sum(int64_t n, int64_t a, int64_t b) { return pa_floor_sum(n, a, b); }
-
 // Every piece of every CTA, 16 ints each: cta, begins, ends, then PaItem's
 // fields.  Returns the number of pieces, or -1 when `cap` is too small.
 int64_t host_schedule(const int* cu_q, const int* cu_k, const int* kv_len, int n_seqs, int T, int Hkv, int TT,

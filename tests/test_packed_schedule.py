@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "helix-online-kv_b200", "csrc")
 OUT = os.path.join(HERE, "native", "_build", "libhokv_schedule_host.so")
 DIRECT, PIECE, ROWWISE = 0, 1, 2
-ITEM, MIN_SHARE = 2, 4
+ITEM, MIN_SHARE = 256, 512
 
 
 @pytest.fixture(scope="module")
@@ -25,8 +25,6 @@ def lib():
     src = os.path.join(HERE, "native", "hokv_schedule_host.cpp")
     subprocess.check_call(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, "-o", OUT, src])
     L = ctypes.CDLL(OUT)
-    L.host_floor_sum.restype = ctypes.c_int64
-    L.host_floor_sum.argtypes = [ctypes.c_int64] * 3
     L.host_schedule.restype = ctypes.c_int64
     vp, i, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
     L.host_schedule.argtypes = [vp, vp, vp, i, i, i, i, i64, i, i, i, vp, i64, vp]
@@ -50,7 +48,7 @@ def _schedule(lib, q, kv, hkv, tt, prefix, causal, ctas, layout, T=None, rows=No
 
 
 def _expected(q, kv, hkv, tt, prefix, causal):
-    """{(src, first token, KV head): (tokens, tiles)} of every item."""
+    """{(src, first token, KV head): (tokens, keys)} of every item."""
     W, items, starts = 2 * tt, {}, np.concatenate([[0], np.cumsum(q)]).astype(int)
     seqs = [(1, 0, int(starts[-1]), prefix, False)] if prefix else []
     seqs += [(0, int(s), n, k, causal) for s, n, k in zip(starts, q, kv)]
@@ -59,15 +57,15 @@ def _expected(q, kv, hkv, tt, prefix, causal):
             m = min(W, n - p * W)
             end = max(0, k - n + p * W + m) if c else k
             for h in range(hkv):
-                items[src, s + p * W, h] = (m, -(-end // 128))
+                items[src, s + p * W, h] = (m, end)
     return items
 
 
 def _check(lib, q, kv, hkv, tt, prefix, causal, ctas, layout="slots"):
     rows, units = _schedule(lib, q, kv, hkv, tt, prefix, causal, ctas, layout)
     want = _expected(q, kv, hkv, tt, prefix, causal)
-    assert units == sum(ITEM + (2 if m > tt else 1) * t for m, t in want.values())
-    share = max(-(-units // ctas), MIN_SHARE)
+    assert units == sum(ITEM + (2 if m > tt else 1) * e for m, e in want.values())
+    share = max(units // ctas + 1, MIN_SHARE)
     pieces, slots, load = {}, set(), {}
     for r in rows.tolist():
         cta, begins, ends, tok0, n_tok, src, row0, slot, hk, j0, j1, kv_len, pos0, mode, at, _ = r
@@ -75,9 +73,10 @@ def _check(lib, q, kv, hkv, tt, prefix, causal, ctas, layout="slots"):
         if mode == PIECE:
             assert at // 2 == cta and at not in slots
             slots.add(at)
-        load[cta] = load.get(cta, 0) + (2 if n_tok > tt else 1) * (j1 - j0)
+        load[cta] = load.get(cta, 0) + (2 if n_tok > tt else 1) * (128 * (j1 - j0))
     assert set(pieces) == set(want)
-    for key, (m, tiles) in want.items():
+    for key, (m, keys) in want.items():
+        tiles = -(-keys // 128)
         ps = sorted(pieces[key])
         assert [p[4] for p in ps][0] == 0 and ps[-1][5] == tiles
         assert all(a[5] == b[4] for a, b in zip(ps, ps[1:]))
@@ -91,14 +90,9 @@ def _check(lib, q, kv, hkv, tt, prefix, causal, ctas, layout="slots"):
             first, last = ps[0][0], ps[-1][0]
             chain = [first * 2 + 1] + [c * 2 for c in range(first + 1, last + 1) if c * 2 in slots]
             assert [p[7] for p in ps] == chain and all(p[6] == PIECE for p in ps)
-    assert all(v <= share + 1 for v in load.values())
-
-
-def test_floor_sum(lib):
-    rng = random.Random(1)
-    for _ in range(300):
-        n, a, b = rng.randint(0, 60), rng.randint(0, 256), rng.randint(0, 5000)
-        assert lib.host_floor_sum(n, a, b) == sum((a * i + b) // 128 for i in range(n))
+    # a share's keys, padded to whole tiles item by item
+    n_items = {c: sum(1 for ps in pieces.values() for p in ps if p[0] == c) for c in load}
+    assert all(v <= share + 256 * (n_items[c] + 1) for c, v in load.items())
 
 
 @pytest.mark.parametrize("ctas", [1, 7, 148])
@@ -117,7 +111,7 @@ def test_random_batches(lib, ctas):
 
 def test_one_long_sequence_is_spread_over_every_cta(lib):
     rows, units = _schedule(lib, [1], [16384], 8, 32, 0, True, 148, "slots")
-    assert len(set(rows[:, 0].tolist())) == -(-units // -(-units // 148))
+    assert set(rows[:, 0].tolist()) == set(range(148))
     _check(lib, [1], [16384], 8, 32, 0, True, 148)
     _check(lib, [16384], [16384], 8, 32, 0, True, 148)
     _check(lib, [200000], [1000000], 2, 128, 0, True, 148)
