@@ -20,12 +20,15 @@
 // atomics, the same result each run.
 //
 // One CTA, 384 threads: warps 0-3 and 4-7 are the softmax of tile slots 0 and
-// 1 (a thread owns a row), warp 8 loads (TMA), warp 9 issues the MMAs, warp
-// 10 walks the schedule into a ring of item descriptors.  A two-tile item
-// gives each slot one query tile and every key tile; a one-tile item gives
-// both slots the same query rows and every other key tile, joined in
-// registers at the end, so the tensor cores and the exponentials overlap for
-// single tokens too.  Per slot and key tile:
+// 1 (a thread owns a row), warps 8 and 11 load (TMA; K and V, and Q), warp 9
+// issues the MMAs, warp 10 walks the schedule into a ring of item descriptors.  All items of a CTA
+// form one stream of tasks u, task u on slot u % 2: a two-tile item is (tile
+// 0, key tile j), (tile 1, key tile j) for each j, the two sharing K and V; a
+// one-tile item is its key tiles in turn, joined over the slots in registers
+// at its end, and an item of one key tile takes one slot and leaves the other
+// to the next item.  The MMA warp issues S of task u + 2 behind P V of task u,
+// across item borders, so one slot's products run under the other's softmax
+// and an item's epilogue under the next one's scores.  Per task:
 //   S = Q K^T    tcgen05.mma kind::f16 into 128 fp32 TMEM columns
 //   P = 2^(S scale log2 e - m)   one thread per row, rounded to the input
 //                type and written over S in tensor memory (64 columns)
@@ -47,8 +50,7 @@ namespace hokv {
 
 constexpr int PA_THREADS = 384;
 constexpr int PA_ROWS = 128;        // rows of a tile
-constexpr int PA_QUEUE = 4;         // item descriptors in flight
-constexpr int PA_REGS_SOFTMAX = 224, PA_REGS_OTHER = 56;   // 256 * 224 + 128 * 56 = 384 * 168
+constexpr int PA_QUEUE = 8;         // item descriptors in flight
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
 template <int D>
@@ -85,31 +87,42 @@ struct PaP : PaSched {
   float4* row_o;                 // prefix only: [2][T][Hq][D / 4]
 };
 
+// A reader's place in the CTA's task stream: item fields, its task j of `tasks`.
+struct PaCursor {
+  int it = 0, n = 0, two = 0, tasks = 0, j = 0, left = 0, src = 0, hk = 0, tok0 = 0, slot = 0, row0 = 0;
+  bool done = false;
+};
+
 // ---- barriers ----------------------------------------------------------------
 
+__device__ __forceinline__ bool pa_try_wait(uint32_t bar, unsigned parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // Bounded wait of every calling thread; the first that gives up marks the CTA
-// aborted, and every other wait of the CTA then ends too.
-__device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
-  const uint32_t a = smem_u32(bar);
-  unsigned long long t0 = 0;
-  for (int i = 0;; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (done) return true;
+// aborted, and every other wait of the CTA then ends too.  The part behind the
+// first try is a call: it stands in many places and is short of time in none.
+__device__ __noinline__ bool pa_wait_more(uint32_t bar, unsigned parity, volatile uint32_t* abort_flag) {
+  const unsigned long long t0 = global_ns();
+  while (!pa_try_wait(bar, parity)) {
     if (*abort_flag) return false;
-    if (i == 0) {
-      t0 = global_ns();
-    } else if (global_ns() - t0 > TC_WAIT_NS) {
+    if (global_ns() - t0 > TC_WAIT_NS) {
       if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
       return false;
     }
   }
+  return true;
+}
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
+  return pa_try_wait(smem_u32(bar), parity) || pa_wait_more(smem_u32(bar), parity, abort_flag);
 }
 
 __device__ __forceinline__ void pa_arrive(uint64_t* bar) {
@@ -151,17 +164,30 @@ __device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a_tmem, uint32_t 
       : "memory");
 }
 
-// 32 packed columns of this thread's lane into tensor memory, without waiting.
-__device__ __forceinline__ void tmem_st32_nw(uint32_t taddr, const uint32_t (&v)[32]) {
+// 16 packed columns of this thread's lane into tensor memory, without waiting.
+__device__ __forceinline__ void tmem_st16_nw(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+// Waits for the thread's tensor-memory loads; v is not used before.
+__device__ __forceinline__ void tmem_wait_ld32(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+// Columns from `left` on do not count.
+__device__ __forceinline__ void mask32(float (&v)[32], int left) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
 }
 // Scale 8 fp32 columns of this thread's lane.
 __device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
@@ -203,20 +229,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   unsigned char* sKV = sQ + 2 * PG::Q_BYTES;
   unsigned char* sOut = sKV + ST * PG::KV_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + PG::OUT_BYTES);
-  uint64_t* q_full = bars;                 // TMA bytes
-  uint64_t* q_empty = bars + 1;            // MMA commit after the item's last S
-  uint64_t* s_full = bars + 2;             // [2] MMA commit
-  uint64_t* p_full = bars + 4;             // [2] 4 softmax warps
-  uint64_t* o_full = bars + 6;             // [2] MMA commit after the item's last P V
-  uint64_t* o_empty = bars + 8;            // [2] 4 softmax warps: O read
-  uint64_t* it_full = bars + 10;           // [PA_QUEUE] scheduler
-  uint64_t* it_empty = it_full + PA_QUEUE; // [PA_QUEUE] load + MMA + 8 softmax warps
+  uint64_t* q_full = bars;                 // [2] query buffers: TMA bytes
+  uint64_t* q_empty = bars + 2;            // [2] MMA commit after the last S that reads the buffer
+  uint64_t* s_full = bars + 4;             // [2] MMA commit
+  uint64_t* p_full = bars + 6;             // [2] 4 softmax warps
+  uint64_t* o_full = bars + 8;             // [2] MMA commit after the slot's last P V of an item
+  uint64_t* o_empty = bars + 10;           // [2] 4 softmax warps: O read
+  uint64_t* ml_full = bars + 12;           // 4 warps of slot 1: (m, l) in shared memory
+  uint64_t* it_full = bars + 13;           // [PA_QUEUE] scheduler
+  uint64_t* it_empty = it_full + PA_QUEUE; // [PA_QUEUE] 2 load + MMA + 8 softmax warps
   uint64_t* kv_full = it_empty + PA_QUEUE; // [ST] TMA bytes
   uint64_t* kv_empty = kv_full + ST;       // [ST] MMA commit
-  uint64_t* ml_full = kv_empty + ST;       // 4 warps of slot 1: (m, l) in shared memory
-  PaItem* queue = reinterpret_cast<PaItem*>(bars + 40);                     // [PA_QUEUE]
-  uint32_t* ctl = reinterpret_cast<uint32_t*>(queue + PA_QUEUE);            // [0] tmem base, [1] abort
-  float2* s_ml = reinterpret_cast<float2*>(bars + 72);                      // [128] slot 1's (m, l)
+  static_assert(13 + 2 * PA_QUEUE + 2 * ST <= 48, "barriers");
+  uint32_t* ctl = reinterpret_cast<uint32_t*>(bars + 48);                   // [0] tmem base, [1] abort
+  PaItem* queue = reinterpret_cast<PaItem*>(bars + 49);                     // [PA_QUEUE]
+  float2* s_ml = reinterpret_cast<float2*>(bars + 49 + PA_QUEUE * sizeof(PaItem) / 8);   // [128] slot 1's (m, l)
+  static_assert((49 + 128) * 8 + PA_QUEUE * sizeof(PaItem) <= 2048, "control block");
   volatile uint32_t* abort_flag = &ctl[1];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -225,10 +253,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (tid == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     mbar_init(ml_full, 4);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
@@ -236,7 +264,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     }
     for (int i = 0; i < PA_QUEUE; ++i) {
       mbar_init(&it_full[i], 1);
-      mbar_init(&it_empty[i], 10);
+      mbar_init(&it_empty[i], 11);
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -253,7 +281,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 
   if (warp < 8) {
     // ---- softmax of tile slot sl, one row per thread ----------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
     const int sl = warp >> 2, row = tid & 127;
     const int row_tok = row / G, row_g = row - row_tok * G;
     const int first_tok = ((warp & 3) * 32) / G;   // lowest token of this warp's rows
@@ -263,6 +290,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     // rows of out on 32-byte boundaries and in whole 16-element steps: 32-byte stores
     const bool wide = p.D % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) % 32 | (uint64_t)(p.ost % 16) | (uint64_t)(p.osh % 16)) == 0;
     unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
+    int u = 0;   // tasks of the items so far
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int qi = it % PA_QUEUE;
@@ -271,10 +299,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       if (w.out_mode == PA_STOP) break;
       const bool two = w.n_tok > TT;
       const int n = w.j1 - w.j0;
-      const int mine = two ? n : (sl == 0 ? (n + 1) >> 1 : n >> 1);   // key tiles of this slot
+      if (two) u = (u + 1) & ~1;                           // a two-tile item begins on slot 0
+      const int skip = two ? 0 : (sl - u) & 1;             // this slot's first key tile
+      const int mine = two ? n : (n - skip + 1) >> 1;      // its number of key tiles
+      const bool join = !two && n > 1;                     // both slots hold parts of the same rows
+      const bool other = two || join || ((u & 1) != sl);   // the other slot has a part of this item
+      u += two ? 2 * n : n;
       const bool warp_ok = first_tok < TT && (two ? sl * TT : 0) + first_tok < w.n_tok;   // any row of the warp in use
       // keys this row sees, and the least such limit of the warp, counted from the slot's key tile
-      int lim = min(w.kv_len, w.pos0 + (two ? sl * TT : 0) + row_tok + 1) - (w.j0 + (two ? 0 : sl)) * PA_BN;
+      int lim = min(w.kv_len, w.pos0 + (two ? sl * TT : 0) + row_tok + 1) - (w.j0 + skip) * PA_BN;
       int wlim = __shfl_sync(0xffffffffu, lim, 0);
       const int step = two ? PA_BN : 2 * PA_BN;
       auto item_done = [&]() {
@@ -287,17 +320,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         s_ph ^= 1;
         tc_fence_after();
         if (warp_ok) {
-          float v[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, *reinterpret_cast<float(*)[32]>(&v[c * 32]));
-          tmem_wait_ld();
-          if (wlim < PA_BN) {
-#pragma unroll
-            for (int j = 0; j < 128; ++j) v[j] = j < lim ? v[j] : -INFINITY;
-          }
+          // two passes over the row, 32 columns at a time with the next 32 on their way: short loops (the roles
+          // share one instruction cache) and few registers
+          const bool masked = wlim < PA_BN;
+          float va[32], vb[32];
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto max32 = [&](float (&v)[32], int left) __attribute__((always_inline)) {
+            if (masked) mask32(v, left);
 #pragma unroll
-          for (int j = 0; j < 128; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[j], v[j + 1]);
+            for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[j], v[j + 1]);
+          };
+          tmem_ld32_nw(s_addr, va);
+#pragma unroll 1
+          for (int c = 0; c < PA_BN; c += 64) {
+            tmem_wait_ld32(va);
+            tmem_ld32_nw(s_addr + c + 32, vb);
+            max32(va, lim - c);
+            tmem_wait_ld32(vb);
+            tmem_ld32_nw(s_addr + (c + 64) % PA_BN, va);   // behind the last columns: the first again
+            max32(vb, lim - c - 32);
+          }
           const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
           const bool grow = !(mt <= m_run + 8.f);   // also for NaN, and for the first key a row sees
           if (i > 0 && __any_sync(0xffffffffu, grow)) {
@@ -312,17 +354,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           const float nm = m_run == -INFINITY ? 0.f : -m_run;
           const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
           float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          auto exp32 = [&](float (&v)[32], int left, uint32_t at) __attribute__((always_inline)) {
+            if (masked) mask32(v, left);
+            uint32_t pk[16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float2 a = __ffma2_rn(make_float2(v[h * 64 + 2 * j], v[h * 64 + 2 * j + 1]), s2, n2);
+            for (int j = 0; j < 16; ++j) {
+              const float2 a = __ffma2_rn(make_float2(v[2 * j], v[2 * j + 1]), s2, n2);
               const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
               acc[j & 1] = __fadd2_rn(acc[j & 1], e);
               pk[j] = pack2<T>(e.x, e.y);
             }
-            tmem_st32_nw(s_addr + h * 32, pk);
+            tmem_st16_nw(at, pk);   // over columns of S that were read before
+          };
+#pragma unroll 1
+          for (int c = 0; c < PA_BN; c += 64) {
+            tmem_wait_ld32(va);
+            tmem_ld32_nw(s_addr + c + 32, vb);
+            exp32(va, lim - c, s_addr + c / 2);
+            tmem_wait_ld32(vb);
+            if (c + 64 < PA_BN) tmem_ld32_nw(s_addr + c + 64, va);
+            exp32(vb, lim - c - 32, s_addr + c / 2 + 16);
           }
           acc[0] = __fadd2_rn(acc[0], acc[1]);
           l_run += acc[0].x + acc[0].y;
@@ -333,25 +384,25 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (lane == 0) pa_arrive(&p_full[sl]);
       }
       if (!ok) break;
-      // ---- epilogue: O of this slot (one-tile items: slot 0 joins both) -----------
-      const bool join = !two && n > 1;
-      if (mine > 0) {
-        if (!pa_wait(&o_full[sl], o_ph, abort_flag)) break;
-        o_ph ^= 1;
-        tc_fence_after();
+      // ---- epilogue: O of this slot (slot 0 joins both parts of a one-tile item) ------
+      if (sl == 0 && other) o1_ph ^= 1;   // slot 1 completes a phase too
+      if (mine == 0) {
+        item_done();
+        continue;
       }
-      if (!two && sl == 1) {
-        if (join) {
-          s_ml[row] = make_float2(m_run, l_run);
-          __syncwarp();
-          if (lane == 0) pa_arrive(ml_full);
-        }
+      if (!pa_wait(&o_full[sl], o_ph, abort_flag)) break;
+      o_ph ^= 1;
+      tc_fence_after();
+      if (join && sl == 1) {
+        s_ml[row] = make_float2(m_run, l_run);
+        __syncwarp();
+        if (lane == 0) pa_arrive(ml_full);
         item_done();
         continue;   // slot 0 reads O_1 and frees it
       }
       float f0 = 1.f, f1 = 0.f;
       if (join) {
-        if (!pa_wait(&o_full[1], o1_ph, abort_flag) || !pa_wait(ml_full, ml_ph, abort_flag)) break;
+        if (!pa_wait(&o_full[1], o1_ph ^ 1, abort_flag) || !pa_wait(ml_full, ml_ph, abort_flag)) break;
         ml_ph ^= 1;
         tc_fence_after();
         const float2 b = s_ml[row];
@@ -361,8 +412,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         m_run = mm;
         l_run = l_run * f0 + b.y * f1;
       }
-      if (sl == 0 && (join || (two && n > 0))) o1_ph ^= 1;   // slot 1 completed a phase too
-      const bool nothing = n == 0 || l_run == 0.f;
+      const bool nothing = l_run == 0.f;
       const float inv = nothing ? 0.f : 1.f / l_run;
       const int tok = (two ? sl * TT : 0) + row_tok;                  // this row's token in the item
       const bool row_ok = row_tok < TT && tok < w.n_tok;
@@ -382,14 +432,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 #pragma unroll 1   // short code: an item's end is often its first use
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
-          if (n > 0) {
-            tmem_ld32(o_addr + c * 32, o);
-            if (join) {
-              float o1[32];
-              tmem_ld32(o_addr + 128 + c * 32, o1);
+          tmem_ld32(o_addr + c * 32, o);
+          if (join) {
+            float o1[32];
+            tmem_ld32(o_addr + 128 + c * 32, o1);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = o[j] * f0 + o1[j] * f1;
-            }
+            for (int j = 0; j < 32; ++j) o[j] = o[j] * f0 + o1[j] * f1;
           }
           if (nothing) {
 #pragma unroll
@@ -443,13 +491,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           }
         }
       }
-      if (n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          pa_arrive(&o_empty[sl]);
-          if (join) pa_arrive(&o_empty[1]);
-        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        pa_arrive(&o_empty[sl]);
+        if (join) pa_arrive(&o_empty[1]);
       }
       item_done();
     }
@@ -457,6 +503,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
       const int used = pa_used(p);
       const int64_t total = (int64_t)(p.T - used) * p.Hq * p.D;
+#pragma unroll 1
       for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < total; i += (int64_t)gridDim.x * 256) {
         const int d = (int)(i % p.D);
         const int64_t h = i / p.D % p.Hq, t = used + i / p.D / p.Hq;
@@ -464,71 +511,76 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
+    auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
+    // Positions c at the next task on slot sl; false when there is none: at the end of the stream (c.done), or when
+    // the next item begins on slot 0 and this is slot 1.  `release`: this cursor is its warp's last reader.
+    auto next_task = [&](PaCursor& c, int sl, bool& ok, bool release, bool loads) __attribute__((always_inline)) {
+      if (c.done) return false;
+      if (c.j == c.tasks) {
+        const int qi = c.it % PA_QUEUE;
+        ok = all(pa_wait(&it_full[qi], (unsigned)((c.it / PA_QUEUE) & 1), abort_flag));
+        if (!ok) return false;
+        ++c.it;
+        const PaItem& w = queue[qi];
+        c.done = uniform(w.out_mode) == PA_STOP;
+        c.n = uniform(w.j1 - w.j0);
+        c.two = uniform(w.n_tok > TT);
+        if (loads) {
+          c.src = uniform(w.src);
+          c.hk = uniform(w.hk);
+          c.tok0 = uniform(w.tok0);
+          c.slot = uniform(w.slot);
+          c.row0 = uniform(w.row0 + w.j0 * PA_BN);
+        } else {
+          c.left = uniform(w.kv_len - w.j0 * PA_BN);
+        }
+        c.tasks = c.two ? 2 * c.n : c.n;
+        c.j = 0;
+        __syncwarp();
+        if (release && lane == 0) pa_arrive(&it_empty[qi]);
+        if (c.done) return false;
+      }
+      return !(c.two && c.j == 0 && sl == 1);
+    };
     if (warp == 8) {
-      // ---- loads: the item's query tiles, then K and V in the order of use ------------
+      // ---- loads of K and V, in the order of use -------------------------------------
       const int used = p.prefix > 0 ? 6 : 4;
       if (lane < used) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps) + lane * sizeof(CUtensorMap)) : "memory");
-      unsigned stage = 0, stage_ph = 1, loads = 0, q_ph = 1, q_uses = 0;
+      unsigned stage = 0, stage_ph = 1, loads = 0;
+      PaCursor ck, cv;
       bool ok = true;
-      auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
-      for (int it = 0; ok; ++it) {
-        const int qi = it % PA_QUEUE;
-        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
-        if (!ok) break;
-        const int mode = uniform(queue[qi].out_mode), n = uniform(queue[qi].j1 - queue[qi].j0),
-                  two = uniform(queue[qi].n_tok > TT), src = uniform(queue[qi].src), hk = uniform(queue[qi].hk),
-                  tok0 = uniform(queue[qi].tok0), slot = uniform(queue[qi].slot),
-                  row0 = uniform(queue[qi].row0 + queue[qi].j0 * PA_BN);
-        __syncwarp();
-        if (lane == 0) pa_arrive(&it_empty[qi]);
-        if (mode == PA_STOP) break;
-        if (n == 0) continue;
-        ok = all(pa_wait(q_empty, q_ph, abort_flag));   // passes at once the first time
-        if (!ok) break;
-        q_ph ^= 1;
-        ++q_uses;
+      // the K (or V) tile that S (or P V) of the next task on slot sl reads first
+      auto step = [&](PaCursor& c, int sl, bool is_v) __attribute__((always_inline)) {
+        if (!next_task(c, sl, ok, is_v, true)) return;
+        const int j = c.j++;
+        if (c.two && (j & 1)) return;
+        ok = all(pa_wait(&kv_empty[stage], stage_ph, abort_flag));
+        if (!ok) return;
+        const CUtensorMap* m = c.src ? (is_v ? &maps.pv : &maps.pk) : (is_v ? &maps.v : &maps.k);
+        const int at_t = c.src ? (is_v ? p.pv_t : p.pk_t) : (is_v ? p.v_t : p.k_t);
+        const int at_h = c.src ? (is_v ? p.pv_h : p.pk_h) : (is_v ? p.v_h : p.k_h);
+        const int row = c.row0 + (c.two ? j >> 1 : j) * PA_BN;
+        const int c1 = at_t == 1 ? row : at_h == 1 ? c.hk : c.slot, c2 = at_t == 2 ? row : at_h == 2 ? c.hk : c.slot,
+                  c3 = at_t == 3 ? row : at_h == 3 ? c.hk : c.slot;
         if (elect_one()) {
-          pf_expect_tx(q_full, (uint32_t)((two ? 2 : 1) * PG::NB * TT * G * 128));
-          for (int t = 0; t < (two ? 2 : 1); ++t)
+          pf_expect_tx(&kv_full[stage], PG::KV_BYTES);
 #pragma unroll
-            for (int a = 0; a < PG::NB; ++a)
-              pf_tma4(sQ + t * PG::Q_BYTES + a * PA_ROWS * 128, &maps.q, a * 64, 0, hk, tok0 + t * TT, q_full);
+          for (int a = 0; a < PG::NB; ++a)
+            pf_tma4(sKV + stage * PG::KV_BYTES + a * PA_BN * 128, m, a * 64, c1, c2, c3, &kv_full[stage]);
         }
         __syncwarp();
-        auto load = [&](const CUtensorMap* m, int at_t, int at_h, int j) {
-          ok = all(pa_wait(&kv_empty[stage], stage_ph, abort_flag));
-          if (!ok) return;
-          const int row = row0 + j * PA_BN;
-          const int c1 = at_t == 1 ? row : at_h == 1 ? hk : slot, c2 = at_t == 2 ? row : at_h == 2 ? hk : slot,
-                    c3 = at_t == 3 ? row : at_h == 3 ? hk : slot;
-          if (elect_one()) {
-            pf_expect_tx(&kv_full[stage], PG::KV_BYTES);
-#pragma unroll
-            for (int a = 0; a < PG::NB; ++a)
-              pf_tma4(sKV + stage * PG::KV_BYTES + a * PA_BN * 128, m, a * 64, c1, c2, c3, &kv_full[stage]);
-          }
-          __syncwarp();
-          ++loads;
-          if (++stage == ST) stage = 0, stage_ph ^= 1;
-        };
-        auto load_k = [&](int j) {
-          if (src) load(&maps.pk, p.pk_t, p.pk_h, j);
-          else load(&maps.k, p.k_t, p.k_h, j);
-        };
-        auto load_v = [&](int j) {
-          if (src) load(&maps.pv, p.pv_t, p.pv_h, j);
-          else load(&maps.v, p.v_t, p.v_h, j);
-        };
-        const int ahead = two ? 1 : 2;
-        for (int j = -ahead; ok && j < n; ++j) {
-          if (j >= 0) load_v(j);
-          if (ok && j + ahead < n) load_k(j + ahead);
-        }
+        ++loads;
+        if (++stage == ST) stage = 0, stage_ph ^= 1;
+      };
+      // K runs two tasks ahead
+#pragma unroll 1
+      for (int i = -2; ok && !cv.done; ++i) {
+        if (i >= 0) step(cv, i & 1, true);
+        if (ok) step(ck, i & 1, false);
       }
       if (*abort_flag) {   // gave up: the copies in flight land before the CTA ends
+#pragma unroll 1
         for (unsigned k = loads > ST ? loads - ST : 0; k < loads; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
-        if (q_uses > 0) (void)mbar_wait(q_full, (q_uses - 1) & 1);
       }
     } else if (warp == 9) {
       // ---- MMA issue --------------------------------------------------------------
@@ -536,79 +588,58 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       const uint32_t idesc_s = umma_idesc_f16(PA_BN, BF, 0), idesc_o = umma_idesc_f16(kd * 16, BF, 1);
       const uint32_t q_lo = pa_desc_lo(smem_u32(sQ), 16), k_lo = pa_desc_lo(smem_u32(sKV), 16),
                      v_lo = pa_desc_lo(smem_u32(sKV), PA_BN * 128);
-      unsigned stage = 0, stage_ph = 0, q_ph = 0, p_ph0 = 0, p_ph1 = 0, oe_ph0 = 1, oe_ph1 = 1;
+      unsigned stage = 0, stage_ph = 0, q_ph = 0, p_ph = 0, oe_ph = 3;   // a phase bit per buffer or slot
+      unsigned k_stage = 0, v_stage = 0;
+      int ks = 0, qb = 0;
+      PaCursor cs, cp;
       bool ok = true;
-      auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
       // the next tile of the ring, once its bytes have landed
-      auto next_tile = [&]() {
+      auto next_tile = [&]() __attribute__((always_inline)) {
         const unsigned st = stage;
         ok = all(pa_wait(&kv_full[st], stage_ph, abort_flag));
         if (++stage == ST) stage = 0, stage_ph ^= 1;
-        tc_fence_after();
         return st;
       };
-      // S of slot SL = Q_q K^T
-      auto issue_s = [&](auto slc, unsigned q, unsigned st, bool release, bool last) {
-        constexpr int SL = decltype(slc)::value;
-        const uint32_t a = q_lo + q * (PG::Q_BYTES >> 4), b = k_lo + st * (PG::KV_BYTES >> 4);
+      // S of the next task on slot sl
+      auto issue_s = [&](int sl) __attribute__((always_inline)) {
+        if (!next_task(cs, sl, ok, false, false)) return;
+        const int j = cs.j++;
+        if (!cs.two && j == 0) qb ^= 1;
+        const int buf = cs.two ? sl : qb ^ 1;
+        if (!cs.two || sl == 0) k_stage = next_tile();
+        if (cs.two ? j < 2 : j == 0) {
+          ok = all(ok && pa_wait(&q_full[buf], q_ph >> buf & 1, abort_flag));
+          q_ph ^= 1u << buf;
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t a = q_lo + buf * (PG::Q_BYTES >> 4), b = k_lo + k_stage * (PG::KV_BYTES >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int kc = 0; kc < D / 16; ++kc) {   // 16 dims = 32 bytes inside a 64-dim column block
             const uint32_t off = (uint32_t)(((kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32) >> 4);
-            if (kc < kd) pa_mma_ss(SL * 128, a + off, b + off, idesc_s, kc > 0);
+            if (kc < kd) pa_mma_ss(sl * 128, a + off, b + off, idesc_s, kc > 0);
           }
-          umma_commit(&s_full[SL]);
-          if (release) umma_commit(&kv_empty[st]);
-          if (last) umma_commit(q_empty);
+          umma_commit(&s_full[sl]);
+          if (!cs.two || sl == 1) umma_commit(&kv_empty[k_stage]);
+          if (j >= cs.tasks - 1 - cs.two) umma_commit(&q_empty[buf]);
         }
         __syncwarp();
       };
-      // O of slot SL += P V over ks steps of 16 tokens
-      auto issue_pv = [&](auto slc, unsigned sv, int ks, bool first, bool release, bool last) {
-        constexpr int SL = decltype(slc)::value;
-        unsigned& ph = SL ? p_ph1 : p_ph0;
-        unsigned& oe = SL ? oe_ph1 : oe_ph0;
-        ok = all(pa_wait(&p_full[SL], ph, abort_flag));
-        ph ^= 1;
-        if (first) {   // the epilogue of the slot's last item has read O (passes at once the first time)
-          ok = all(ok && pa_wait(&o_empty[SL], oe, abort_flag));
-          oe ^= 1;
-        }
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t b = v_lo + sv * (PG::KV_BYTES >> 4);
-        if (elect_one()) {
-#pragma unroll
-          for (int kc = 0; kc < PA_BN / 16; ++kc)
-            if (kc < ks) pa_mma_ts(256 + SL * 128, SL * 128 + kc * 8, b + kc * (2048 >> 4), idesc_o, !first || kc > 0);
-          if (last) umma_commit(&o_full[SL]);
-          if (release) umma_commit(&kv_empty[sv]);
-        }
-        __syncwarp();
-      };
-      constexpr std::integral_constant<int, 0> S0;
-      constexpr std::integral_constant<int, 1> S1;
-      for (int it = 0; ok; ++it) {
-        const int qi = it % PA_QUEUE;
-        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
-        if (!ok) break;
-        const int mode = uniform(queue[qi].out_mode), n = uniform(queue[qi].j1 - queue[qi].j0),
-                  two = uniform(queue[qi].n_tok > TT), left = uniform(queue[qi].kv_len - queue[qi].j0 * PA_BN);
-        __syncwarp();
-        if (lane == 0) pa_arrive(&it_empty[qi]);
-        if (mode == PA_STOP) break;
-        if (n == 0) continue;
-        ok = all(pa_wait(q_full, q_ph, abort_flag));
-        q_ph ^= 1;
-        if (!ok) break;
-        // V(j) ready: its stage and 16-token steps; rows behind the sequence inside the last step are zeroed
-        auto ready_v = [&](int j, int& ks) {
-          const unsigned sv = next_tile();
-          const int valid = min(PA_BN, left - j * PA_BN);
+      // P V of the next task on slot sl
+      auto issue_pv = [&](int sl) __attribute__((always_inline)) {
+        if (!next_task(cp, sl, ok, true, false)) return;
+        const int j = cp.j++;
+        const bool first = j < 2, last = j >= cp.tasks - 2;   // of the item on this slot
+        if (!cp.two || sl == 0) {
+          v_stage = next_tile();
+          // 16-token steps of the tile; rows behind the sequence inside the last one are zeroed
+          const int valid = min(PA_BN, cp.left - (cp.two ? j >> 1 : j) * PA_BN);
           ks = (valid + 15) >> 4;
           if (ok && (valid & 15)) {
-            unsigned char* tile = sKV + sv * PG::KV_BYTES;
+            unsigned char* tile = sKV + v_stage * PG::KV_BYTES;
             const int rows = ks * 16 - valid;
+#pragma unroll 1
             for (int e = lane; e < rows * PG::NB * 8; e += 32) {
               const int r = valid + e / (PG::NB * 8), c = e % (PG::NB * 8);
               *reinterpret_cast<uint4*>(tile + (c >> 3) * PA_BN * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -616,45 +647,113 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             fence_async_smem();
             __syncwarp();
           }
-          return sv;
-        };
-        unsigned st = next_tile();
-        if (!ok) break;
-        int ks = 0;
-        if (two) {
-          issue_s(S0, 0, st, false, false);
-          issue_s(S1, 1, st, true, n == 1);
-          for (int j = 0; ok && j < n; ++j) {
-            const unsigned sv = ready_v(j, ks);
-            if (!ok) break;
-            issue_pv(S0, sv, ks, j == 0, false, j == n - 1);
-            if (ok && j + 1 < n) {
-              st = next_tile();
-              if (ok) issue_s(S0, 0, st, false, false);
-            }
-            if (ok) issue_pv(S1, sv, ks, j == 0, true, j == n - 1);
-            if (ok && j + 1 < n) issue_s(S1, 1, st, true, j + 1 == n - 1);
-          }
-        } else {
-          issue_s(S0, 0, st, true, n == 1);
-          if (n > 1) {
-            st = next_tile();
-            if (ok) issue_s(S1, 0, st, true, n == 2);
-          }
-          auto half = [&](auto slc, int j) {
-            const unsigned sv = ready_v(j, ks);
-            if (ok) issue_pv(slc, sv, ks, j < 2, true, j >= n - 2);
-            if (ok && j + 2 < n) {
-              st = next_tile();
-              if (ok) issue_s(slc, 0, st, true, j + 2 == n - 1);
-            }
-          };
-          for (int j = 0; ok && j < n; j += 2) {
-            half(S0, j);
-            if (ok && j + 1 < n) half(S1, j + 1);
-          }
         }
+        bool got = ok && pa_wait(&p_full[sl], p_ph >> sl & 1, abort_flag);
+        p_ph ^= 1u << sl;
+        if (first) {   // the epilogue of the slot's last item has read O (passes at once the first time)
+          got = got && pa_wait(&o_empty[sl], oe_ph >> sl & 1, abort_flag);
+          oe_ph ^= 1u << sl;
+        }
+        ok = all(got);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t b = v_lo + v_stage * (PG::KV_BYTES >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int kc = 0; kc < PA_BN / 16; ++kc)
+            if (kc < ks) pa_mma_ts(256 + sl * 128, sl * 128 + kc * 8, b + kc * (2048 >> 4), idesc_o, !first || kc > 0);
+          if (last) umma_commit(&o_full[sl]);
+          if (!cp.two || sl == 1) umma_commit(&kv_empty[v_stage]);
+        }
+        __syncwarp();
+      };
+      // Tasks well inside one item, from slot 0 on: P V and the S behind it are issued together, with nothing to look
+      // up in between.  The tensor pipe takes a few instructions ahead, so it idles for all that this warp does
+      // between two of them.
+      auto steady = [&]() __attribute__((always_inline)) {
+        const int m = cs.it == cp.it && cp.j >= 2 ? (cs.tasks - cs.j - 2) & ~1 : 0;
+        if (m <= 0) return;
+        const uint32_t q_at = q_lo + (cs.two ? 0 : (qb ^ 1) * (PG::Q_BYTES >> 4)), q_step = cs.two ? PG::Q_BYTES >> 4 : 0;
+#pragma unroll 1
+        for (int i = 0; i < m; ++i) {
+          const int sl = i & 1;
+          bool got = true;
+          if (!cs.two || sl == 0) {
+            v_stage = stage;
+            got = pa_wait(&kv_full[stage], stage_ph, abort_flag);
+            if (++stage == ST) stage = 0, stage_ph ^= 1;
+            k_stage = stage;
+            got = pa_wait(&kv_full[stage], stage_ph, abort_flag) && got;
+            if (++stage == ST) stage = 0, stage_ph ^= 1;
+          }
+          got = pa_wait(&p_full[sl], p_ph >> sl & 1, abort_flag) && got;
+          p_ph ^= 1u << sl;
+          ok = all(got);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t bv = v_lo + v_stage * (PG::KV_BYTES >> 4), bk = k_lo + k_stage * (PG::KV_BYTES >> 4);
+          const uint32_t a = q_at + sl * q_step, d = sl * 128;
+          if (elect_one()) {
+#pragma unroll
+            for (int kc = 0; kc < PA_BN / 16; ++kc) pa_mma_ts(256 + d, d + kc * 8, bv + kc * (2048 >> 4), idesc_o, 1);
+#pragma unroll
+            for (int kc = 0; kc < D / 16; ++kc) {
+              const uint32_t off = (uint32_t)(((kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32) >> 4);
+              if (kc < kd) pa_mma_ss(d, a + off, bk + off, idesc_s, kc > 0);
+            }
+            umma_commit(&s_full[sl]);
+            if (!cs.two || sl == 1) {
+              umma_commit(&kv_empty[v_stage]);
+              umma_commit(&kv_empty[k_stage]);
+            }
+          }
+          __syncwarp();
+        }
+        cs.j += m;
+        cp.j += m;
+      };
+      // S runs two tasks ahead.  One copy of this code for all cases: it competes for the instruction cache.
+#pragma unroll 1
+      for (int i = -2; ok && !cp.done; ++i) {
+        const int sl = i & 1;
+        if (sl == 0) steady();
+        if (i >= 0 && ok) issue_pv(sl);
+        if (ok) issue_s(sl);
       }
+    } else if (warp == 11) {
+      // ---- loads of the query tiles: both buffers for a two-tile item, else one, in turn --------
+      unsigned q_ph = 3, q_uses = 0;   // a phase bit per buffer
+      int qb = 0;
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        const int qi = it % PA_QUEUE;
+        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
+        if (!ok) break;
+        const int mode = uniform(queue[qi].out_mode), two = uniform(queue[qi].n_tok > TT), hk = uniform(queue[qi].hk),
+                  tok0 = uniform(queue[qi].tok0);
+        __syncwarp();
+        if (lane == 0) pa_arrive(&it_empty[qi]);
+        if (mode == PA_STOP) break;
+#pragma unroll 1
+        for (int t = 0; t < (two ? 2 : 1); ++t) {
+          const int buf = two ? t : qb;
+          ok = all(pa_wait(&q_empty[buf], q_ph >> buf & 1, abort_flag));   // passes at once the first time
+          if (!ok) break;
+          q_ph ^= 1u << buf;
+          q_uses |= 1u << buf;
+          if (elect_one()) {
+            pf_expect_tx(&q_full[buf], (uint32_t)(PG::NB * TT * G * 128));
+#pragma unroll
+            for (int a = 0; a < PG::NB; ++a)
+              pf_tma4(sQ + buf * PG::Q_BYTES + a * PA_ROWS * 128, &maps.q, a * 64, 0, hk, tok0 + t * TT, &q_full[buf]);
+          }
+          __syncwarp();
+        }
+        if (!two) qb ^= 1;
+      }
+      if (*abort_flag)
+        for (int i = 0; i < 2; ++i)
+          if (q_uses >> i & 1) (void)mbar_wait(&q_full[i], q_ph >> i & 1);
     } else if (warp == 10) {
       // ---- schedule: this CTA's share of the unit line ------------------------------
       const int n_s = pa_n_seqs(p);
@@ -662,6 +761,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       const int s_lo = min(lane * per, n_s), s_hi = min(s_lo + per, n_s);
       int64_t mine = 0;
       bool bad = false;
+#pragma unroll 1
       for (int s = s_lo; s < s_hi; ++s) {
         const PaSeq q = pa_seq(p, s);
         bad = bad || q.bad;
@@ -693,13 +793,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       };
       bool ok = true;
       if (begin < end) {
-        // the sequence that holds unit `begin`, and the units before it
+        // the lane whose sequences hold unit `begin`, its first one and the units before that
         const int owner = __ffs(__ballot_sync(0xffffffffu, incl > begin)) - 1;
         int s = 0;
         int64_t at = 0;
         if (lane == owner) {
           at = incl - mine;
-          s = pa_find(p, s_lo, s_hi, begin, at);
+          s = s_lo;
         }
         s = __shfl_sync(0xffffffffu, s, owner);
         at = __shfl_sync(0xffffffffu, at, owner);
@@ -714,9 +814,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
             p.desc[w.out_at] = d;
           }
           if (p.prefix > 0 && begins)   // where k_packed_combine_rows finds this item's rows
+#pragma unroll 1
             for (int i = lane; i < w.n_tok; i += 32)
               p.tok_info[((int64_t)w.src * p.T + w.tok0 + i) * p.Hkv + w.hk] =
                   make_int2(ends ? -1 : (int)blockIdx.x, i);
+          if (w.j0 == w.j1) {   // nothing to see: zeros, or an empty part of a row
+#pragma unroll 1
+            for (int e = lane; e < w.n_tok * G * (p.D / 8); e += 32) {
+              const int r = e / (p.D / 8), tok = r / G;
+              const int64_t t = w.tok0 + tok;
+              const int h = w.hk * G + r - tok * G;
+              if (w.out_mode == PA_ROWWISE) p.row_ml[((int64_t)w.src * p.T + t) * p.Hq + h] = make_float2(-INFINITY, 0.f);
+              else *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + t * p.ost + h * p.osh + e % (p.D / 8) * 8) = make_uint4(0, 0, 0, 0);
+            }
+            return true;
+          }
           return push(w);
         });
       }

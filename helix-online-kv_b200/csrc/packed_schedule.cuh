@@ -15,6 +15,16 @@
 
 namespace hokv {
 
+// Loops are kept rolled and the shared arithmetic is a call on the device: the
+// roles of the kernel share one instruction cache.
+#if defined(__CUDACC__)
+#define HD_CALL __host__ __device__ __noinline__
+#define ROLLED _Pragma("unroll 1")
+#else
+#define HD_CALL inline
+#define ROLLED
+#endif
+
 constexpr int PA_BN = 128;          // keys of a tile
 constexpr int PA_ITEM = 256;        // units of an item besides its keys (start and epilogue): one two-tile key tile
 constexpr int PA_MIN_SHARE = 512;   // smallest share of a CTA: an item's start and two key tiles of a one-tile item
@@ -99,11 +109,12 @@ HD int pa_keys(const PaSeq& s, int W, int pr) {
   return (int)pa_max(s.kv - s.nq + last, 0);
 }
 
-// Units, of one KV head, of the first n pairs (none of them the last).
-HD int64_t pa_units_before(const PaSeq& s, int W, int n) {
-  int64_t keys = (int64_t)n * s.kv;
-  if (s.causal) {
-    const int64_t off = (int64_t)s.kv - s.nq;
+// Units, of one KV head, of the first n pairs (none of them the last) of nq
+// tokens against kv keys.
+HD_CALL int64_t pa_units_before(int kv, int nq, int causal, int W, int n) {
+  int64_t keys = (int64_t)n * kv;
+  if (causal) {
+    const int64_t off = (int64_t)kv - nq;
     const int skip = off < 0 ? (int)pa_min(n, (int)-off / W) : 0;   // pairs that see nothing
     const int64_t m = n - skip;
     keys = m * off + W * (m * (m + 1) / 2 + m * skip);
@@ -120,7 +131,7 @@ HD int64_t pa_seq_units(const PaSched& p, const PaSeq& s) {
   const int W = 2 * p.TT;
   if (s.nq <= 0) return 0;
   const int last = (s.nq + W - 1) / W - 1;
-  return (int64_t)p.Hkv * (pa_units_before(s, W, last) + pa_item_units(s, W, last));
+  return (int64_t)p.Hkv * (pa_units_before(s.kv, s.nq, s.causal, W, last) + pa_item_units(s, W, last));
 }
 
 // A share of at least total / n_ctas (the same value in every CTA; the product
@@ -129,48 +140,39 @@ HD int64_t pa_share(const PaSched& p, int64_t total) {
   return pa_max((int64_t)((double)total * (1.0 / p.n_ctas)) + 1, PA_MIN_SHARE);
 }
 
-// The sequence of [lo, hi) that holds unit `unit`; `at`: units before lo, on
-// return before that sequence.
-HD int pa_find(const PaSched& p, int lo, int hi, int64_t unit, int64_t& at) {
-  int s = lo;
-  for (; s < hi - 1; ++s) {
-    const int64_t u = pa_seq_units(p, pa_seq(p, s));
-    if (at + u > unit) break;
-    at += u;
-  }
-  return s;
-}
-
 // CTA `cta`'s items: units [begin, end), which start in sequence s (`at` units
-// before it).  emit(item, begins, ends): whether the piece holds the item's
+// before it) or behind it.  emit(item, begins, ends): whether the piece holds the item's
 // first and its last key tile; false stops the walk.
 template <typename Emit>
 HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, int64_t at, Emit emit) {
   const int W = 2 * p.TT, n_s = pa_n_seqs(p);
   int64_t pos = begin;
-  for (; s < n_s && pos < end; ++s) {
+  ROLLED for (; s < n_s && pos < end; ++s) {
     const PaSeq q = pa_seq(p, s);
     const int64_t units = pa_seq_units(p, q);
-    if (units == 0) continue;
+    if (at + units <= pos) {
+      at += units;
+      continue;
+    }
     const int np = (q.nq + W - 1) / W;
     int pr = 0;
     if (pos > at) {   // the last pair that starts at or before pos
       int hi = np - 1;
-      while (pr < hi) {
+      ROLLED while (pr < hi) {
         const int mid = (pr + hi + 1) >> 1;
-        if (at + (int64_t)p.Hkv * pa_units_before(q, W, mid) <= pos) pr = mid;
+        if (at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, mid) <= pos) pr = mid;
         else hi = mid - 1;
       }
     }
-    int64_t item_at = at + (int64_t)p.Hkv * pa_units_before(q, W, pr);
-    for (; pr < np && pos < end; ++pr) {
+    int64_t item_at = at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, pr);
+    ROLLED for (; pr < np && pos < end; ++pr) {
       const int left = q.nq - pr * W;
       const int n_tok = left < W ? left : W;
       const int keys = pa_keys(q, W, pr);
       const int tiles = (keys + PA_BN - 1) / PA_BN;
       const int sh = n_tok > p.TT ? 8 : 7;          // units of a key tile: 2^sh
       const int64_t iu = pa_item_units(q, W, pr);
-      for (int hk = 0; hk < p.Hkv; ++hk, item_at += iu) {
+      ROLLED for (int hk = 0; hk < p.Hkv; ++hk, item_at += iu) {
         if (item_at + iu <= pos) continue;
         if (pos >= end) break;
         // a tile belongs to the piece in which its units start

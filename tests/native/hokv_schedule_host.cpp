@@ -19,9 +19,7 @@ int64_t host_schedule(const int* cu_q, const int* cu_k, const int* kv_len, int n
   for (int c = 0; c < n_ctas; ++c) {
     const int64_t begin = pa_min(c * share, total), end = pa_min(begin + share, total);
     if (begin >= end) continue;
-    int64_t at = 0;
-    const int s = pa_find(p, 0, n_s, begin, at);
-    const bool ok = pa_walk(p, c, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends) {
+    const bool ok = pa_walk(p, c, begin, end, 0, 0, [&](const PaItem& w, bool begins, bool ends) {
       if (n == cap) return false;
       int* o = out + 16 * n++;
       const int f[16] = {c, begins, ends, w.tok0, w.n_tok, w.src, w.row0, w.slot, w.hk, w.j0, w.j1, w.kv_len, w.pos0,
