@@ -31,7 +31,7 @@
 // and an item's epilogue under the next one's scores.  Per task:
 //   S = Q K^T    tcgen05.mma kind::f16 into 128 fp32 TMEM columns
 //   P = 2^(S scale log2 e - m)   one thread per row, rounded to the input
-//                type and written over S in tensor memory (64 columns)
+//                type, in tensor memory (64 columns)
 //   O += P V     tcgen05.mma with P as the tensor-memory A operand
 // The running maximum m is raised only when it grows by more than 8 (log2
 // units): P stays below 2^8, and normalising by the same m is exact.  P is
@@ -56,6 +56,10 @@ constexpr float PA_LOG2E = 1.4426950408889634f;
 template <int D>
 struct PaGeo {
   static constexpr int NB = D / 64;                       // 64-dim column blocks
+  // Tensor memory: S of the slots in columns 0 and 128, O in 256 and 384; P in 64 columns of its own behind a 64-dim
+  // O, over S otherwise.
+  static constexpr bool OWN_P = D == 64;
+  static constexpr int P0 = OWN_P ? 256 + 64 : 0;
   static constexpr int Q_BYTES = PA_ROWS * D * 2;         // one query tile
   static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
   static constexpr int STAGES = D == 64 ? 8 : 4;          // ring of K and V tiles
@@ -287,6 +291,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     const uint32_t lane_sel = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_sel + (uint32_t)(sl * 128);
     const uint32_t o_addr = tmem + lane_sel + (uint32_t)(256 + sl * 128);
+    const uint32_t p_addr = tmem + lane_sel + (uint32_t)(PG::P0 + sl * 128);
     // rows of out on 32-byte boundaries and in whole 16-element steps: 32-byte stores
     const bool wide = p.D % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) % 32 | (uint64_t)(p.ost % 16) | (uint64_t)(p.osh % 16)) == 0;
     unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
@@ -320,60 +325,77 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         s_ph ^= 1;
         tc_fence_after();
         if (warp_ok) {
-          // two passes over the row, 32 columns at a time with the next 32 on their way: short loops (the roles
-          // share one instruction cache) and few registers
+          // Two passes over the row, 32 columns at a time with the next 32 on their way: the maximum, then the weights
+          // (short loops: the roles share one instruction cache).  Where P has columns of its own (head dims up to 64),
+          // an item's later tiles go without the first pass: the weights are formed with the running maximum as it
+          // stands and the tile's own maximum beside them, and again in the rare case that it rises by more than 8.
           const bool masked = wlim < PA_BN;
+          const float2 s2 = make_float2(p.sl2, p.sl2);
           float va[32], vb[32];
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          auto max32 = [&](float (&v)[32], int left) __attribute__((always_inline)) {
-            if (masked) mask32(v, left);
+          float2 acc[2];
+          float mx[4];
+          auto max32 = [&](const float (&v)[32]) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[j], v[j + 1]);
           };
-          tmem_ld32_nw(s_addr, va);
-#pragma unroll 1
-          for (int c = 0; c < PA_BN; c += 64) {
-            tmem_wait_ld32(va);
-            tmem_ld32_nw(s_addr + c + 32, vb);
-            max32(va, lim - c);
-            tmem_wait_ld32(vb);
-            tmem_ld32_nw(s_addr + (c + 64) % PA_BN, va);   // behind the last columns: the first again
-            max32(vb, lim - c - 32);
-          }
-          const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
-          const bool grow = !(mt <= m_run + 8.f);   // also for NaN, and for the first key a row sees
-          if (i > 0 && __any_sync(0xffffffffu, grow)) {
-            // O was last written by this slot's previous P V, complete before this S
-            const float f = grow ? pf_ex2(m_run - mt) : 1.f;
-            l_run *= f;
-#pragma unroll 1
-            for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
-            tmem_wait_st();
-          }
-          if (grow) m_run = mt + (mt - mt);         // an infinite maximum gives NaN, as inf - inf does
-          const float nm = m_run == -INFINITY ? 0.f : -m_run;
-          const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
-          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto exp32 = [&](float (&v)[32], int left, uint32_t at) __attribute__((always_inline)) {
-            if (masked) mask32(v, left);
-            uint32_t pk[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 a = __ffma2_rn(make_float2(v[2 * j], v[2 * j + 1]), s2, n2);
-              const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
-              acc[j & 1] = __fadd2_rn(acc[j & 1], e);
-              pk[j] = pack2<T>(e.x, e.y);
-            }
-            tmem_st16_nw(at, pk);   // over columns of S that were read before
+          auto above = [&](float& mt) __attribute__((always_inline)) {   // also for NaN, and for the first key a row sees
+            mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
+            return !(mt <= m_run + 8.f);
           };
+          for (bool known = !PG::OWN_P || i == 0;; known = true) {
+            float mt;
+            tmem_ld32_nw(s_addr, va);
+            mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
+            if (known) {
 #pragma unroll 1
-          for (int c = 0; c < PA_BN; c += 64) {
-            tmem_wait_ld32(va);
-            tmem_ld32_nw(s_addr + c + 32, vb);
-            exp32(va, lim - c, s_addr + c / 2);
-            tmem_wait_ld32(vb);
-            if (c + 64 < PA_BN) tmem_ld32_nw(s_addr + c + 64, va);
-            exp32(vb, lim - c - 32, s_addr + c / 2 + 16);
+              for (int c = 0; c < PA_BN; c += 64) {
+                tmem_wait_ld32(va);
+                tmem_ld32_nw(s_addr + c + 32, vb);
+                if (masked) mask32(va, lim - c);
+                max32(va);
+                tmem_wait_ld32(vb);
+                tmem_ld32_nw(s_addr + (c + 64) % PA_BN, va);   // behind the last columns: the first again
+                if (masked) mask32(vb, lim - c - 32);
+                max32(vb);
+              }
+              const bool grow = above(mt);
+              if (i > 0 && __any_sync(0xffffffffu, grow)) {
+                // O was last written by this slot's previous P V, complete before this S
+                const float f = grow ? pf_ex2(m_run - mt) : 1.f;
+                l_run *= f;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
+                tmem_wait_st();
+              }
+              if (grow) m_run = mt + (mt - mt);         // an infinite maximum gives NaN, as inf - inf does
+            }
+            const float nm = m_run == -INFINITY ? 0.f : -m_run;
+            const float2 n2 = make_float2(nm, nm);
+            acc[0] = acc[1] = make_float2(0.f, 0.f);
+            auto exp32 = [&](const float (&v)[32], uint32_t at) __attribute__((always_inline)) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float2 a = __ffma2_rn(make_float2(v[2 * j], v[2 * j + 1]), s2, n2);
+                const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
+                acc[j & 1] = __fadd2_rn(acc[j & 1], e);
+                pk[j] = pack2<T>(e.x, e.y);
+              }
+              if (PG::OWN_P) max32(v);
+              tmem_st16_nw(at, pk);   // columns of their own, or of S that were read before
+            };
+#pragma unroll 1
+            for (int c = 0; c < PA_BN; c += 64) {
+              tmem_wait_ld32(va);
+              tmem_ld32_nw(s_addr + c + 32, vb);
+              if (masked) mask32(va, lim - c);
+              exp32(va, p_addr + c / 2);
+              tmem_wait_ld32(vb);
+              if (c + 64 < PA_BN) tmem_ld32_nw(s_addr + c + 64, va);
+              if (masked) mask32(vb, lim - c - 32);
+              exp32(vb, p_addr + c / 2 + 16);
+            }
+            if (!PG::OWN_P || known || !__any_sync(0xffffffffu, above(mt))) break;
           }
           acc[0] = __fadd2_rn(acc[0], acc[1]);
           l_run += acc[0].x + acc[0].y;
@@ -661,7 +683,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (elect_one()) {
 #pragma unroll
           for (int kc = 0; kc < PA_BN / 16; ++kc)
-            if (kc < ks) pa_mma_ts(256 + sl * 128, sl * 128 + kc * 8, b + kc * (2048 >> 4), idesc_o, !first || kc > 0);
+            if (kc < ks) pa_mma_ts(256 + sl * 128, PG::P0 + sl * 128 + kc * 8, b + kc * (2048 >> 4), idesc_o, !first || kc > 0);
           if (last) umma_commit(&o_full[sl]);
           if (!cp.two || sl == 1) umma_commit(&kv_empty[v_stage]);
         }
@@ -695,7 +717,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           const uint32_t a = q_at + sl * q_step, d = sl * 128;
           if (elect_one()) {
 #pragma unroll
-            for (int kc = 0; kc < PA_BN / 16; ++kc) pa_mma_ts(256 + d, d + kc * 8, bv + kc * (2048 >> 4), idesc_o, 1);
+            for (int kc = 0; kc < PA_BN / 16; ++kc) pa_mma_ts(256 + d, PG::P0 + d + kc * 8, bv + kc * (2048 >> 4), idesc_o, 1);
 #pragma unroll
             for (int kc = 0; kc < D / 16; ++kc) {
               const uint32_t off = (uint32_t)(((kc >> 2) * PA_ROWS * 128 + (kc & 3) * 32) >> 4);

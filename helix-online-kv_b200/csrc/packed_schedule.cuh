@@ -26,8 +26,8 @@ namespace hokv {
 #endif
 
 constexpr int PA_BN = 128;          // keys of a tile
-constexpr int PA_ITEM = 256;        // units of an item besides its keys (start and epilogue): one two-tile key tile
-constexpr int PA_MIN_SHARE = 512;   // smallest share of a CTA: an item's start and two key tiles of a one-tile item
+constexpr int PA_ITEM = 448;        // units of an item besides its keys (start and epilogue; measured)
+constexpr int PA_MIN_SHARE = 704;   // smallest share of a CTA: an item's start and two key tiles of a one-tile item
 
 enum { PA_DIRECT = 0, PA_PIECE = 1, PA_ROWWISE = 2, PA_STOP = 3 };
 
