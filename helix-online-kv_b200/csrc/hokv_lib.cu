@@ -13,6 +13,8 @@
 #include "packed_attn.cuh"
 #include "norm_rotate.cuh"
 
+#include <atomic>
+#include <chrono>
 #include <map>
 #include <mutex>
 #include <string>
@@ -918,7 +920,7 @@ static int pa_ctas() {
 
 // Workspace layout (offsets in bytes; total in `bytes`).
 struct PaWs {
-  size_t desc, ml, o, info, row_ml, row_o, bytes;
+  size_t desc, ready, ml, o, info, row_ml, row_o, bytes;
 };
 static PaWs pa_ws(const hokv_packed_args* a, int ctas) {
   PaWs w;
@@ -926,6 +928,8 @@ static PaWs pa_ws(const hokv_packed_args* a, int ctas) {
   size_t at = 0;
   w.desc = at;
   at += pa_up((size_t)ctas * 2 * sizeof(PaDesc));
+  w.ready = at;
+  at += pa_up((size_t)ctas * 2 * 8 * 8);
   w.ml = at;
   at += pa_up((size_t)ctas * 2 * 256 * 8);
   w.o = at;
@@ -965,30 +969,33 @@ static int launch_packed(const PaMaps& maps, const PaP& p, cudaStream_t st) {
   if (int e = ensure_smem(k_packed_attn<D, T>, PaGeo<D>::SMEM)) return e;
   k_packed_attn<D, T><<<p.n_ctas, PA_THREADS, PaGeo<D>::SMEM, st>>>(maps, p);
   if (int e = check_launch("k_packed_attn")) return e;
-  // the combine starts behind the last CTAs of the attention (programmatic launch; it waits for the grid's results)
+  if (p.prefix == 0) return HOKV_OK;
+  // the join starts behind the last CTAs of the attention (programmatic launch; it waits for the grid's results)
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)p.T, (unsigned)p.Hkv, (unsigned)cdiv(p.G, PA_JOIN));
   cfg.blockDim = dim3(256);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e;
-  if (p.prefix > 0) {
-    cfg.gridDim = dim3((unsigned)p.T, (unsigned)p.Hkv, (unsigned)cdiv(p.G, PA_JOIN));
-    e = cudaLaunchKernelEx(&cfg, k_packed_combine_rows<D, T>, p);
-  } else {
-    const int64_t most = std::min<int64_t>(p.T, 2 * p.TT) * p.G;   // rows of the largest item
-    // few blocks: most items are whole, and a block without one still costs its start
-    cfg.gridDim = dim3((unsigned)p.n_ctas, (unsigned)std::min<int64_t>(8, cdiv(most, PA_JOIN)));
-    e = cudaLaunchKernelEx(&cfg, k_packed_combine<D, T>, p);
-  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_packed_combine_rows<D, T>, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
-    return fail(HOKV_ERR_CUDA, "k_packed_combine launch: %s", cudaGetErrorString(e));
+    return fail(HOKV_ERR_CUDA, "k_packed_combine_rows launch: %s", cudaGetErrorString(e));
   }
-  return check_launch("k_packed_combine");
+  return check_launch("k_packed_combine_rows");
+}
+
+// Marks one call's pieces in its workspace: never the same twice in a process
+// and far from what memory may hold by chance, 0 excluded (a graph replays its
+// call's value; each call takes its marks back).
+static unsigned long long pa_token() {
+  static std::atomic<unsigned long long> count{(unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  unsigned long long x = ++count * 0x9e3779b97f4a7c15ull;   // odd factor: one to one
+  x ^= x >> 29;
+  return x ? x : 1;
 }
 
 static int packed_attention(const hokv_packed_args* a, void* stream) {
@@ -1092,6 +1099,8 @@ static int packed_attention(const hokv_packed_args* a, void* stream) {
   p.sl2 = a->scale * PA_LOG2E;
   unsigned char* w = reinterpret_cast<unsigned char*>(a->workspace);
   p.desc = reinterpret_cast<PaDesc*>(w + ws.desc);
+  p.ready = reinterpret_cast<unsigned long long*>(w + ws.ready);
+  p.token = pa_token();
   p.ml = reinterpret_cast<float2*>(w + ws.ml);
   p.o = reinterpret_cast<float4*>(w + ws.o);
   p.tok_info = reinterpret_cast<int2*>(w + ws.info);

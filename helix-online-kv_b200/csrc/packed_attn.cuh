@@ -16,8 +16,11 @@
 // schedule from them (packed_schedule.cuh): the work of all items forms one
 // line that the CTAs, one per SM, cut into equal shares.  An item cut by a
 // share's border leaves pieces (running maximum, sum and unnormalised output,
-// fp32) in the workspace, which k_packed_combine joins in CTA order: no
-// atomics, the same result each run.
+// fp32) in the workspace.  A CTA takes the item that earlier CTAs began last,
+// and the one that holds an item's last piece joins all of them in CTA order:
+// no atomics on results, the same result each run.  It waits for marks of
+// lower CTAs only, which never wait for it.  With a shared prefix, rows have
+// two items and k_packed_combine_rows joins all their parts.
 //
 // One CTA, 384 threads: warps 0-3 and 4-7 are the softmax of tile slots 0 and
 // 1 (a thread owns a row), warps 8 and 11 load (TMA; K and V, and Q), warp 9
@@ -64,7 +67,7 @@ struct PaGeo {
   static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
   static constexpr int STAGES = D == 64 ? 8 : 4;          // ring of K and V tiles
   static constexpr int OUT_BYTES = 8 * 4096;              // 32 rows x 64 dims of O per softmax warp, on their way out
-  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + OUT_BYTES + 2048;
+  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + OUT_BYTES + 3072;
 };
 
 // Piece descriptors of a CTA: [0] the piece that continues an earlier CTA's
@@ -86,9 +89,18 @@ struct PaP : PaSched {
   PaDesc* desc;                  // [n_ctas][2]
   float2* ml;                    // [n_ctas][2][256] (running maximum, sum)
   float4* o;                     // [n_ctas][2][D / 4][256]
+  unsigned long long* ready;     // [n_ctas][2][8] the call's token when 32 rows of a piece are written, then 0 again
+  unsigned long long token;      // this call's
   int2* tok_info;                // prefix only: [2][T][Hkv] (first CTA or -1: row-wise, token in item)
   float2* row_ml;                // prefix only: [2][T][Hq]
   float4* row_o;                 // prefix only: [2][T][Hq][D / 4]
+};
+
+// The item that this CTA joins at its end: the one whose last piece it holds.
+struct PaJoinList {
+  int n, tok0, n_tok, hk;      // pieces (0: none to join), rows
+  int left;                    // softmax warps that have joined their part
+  uint16_t slot[240];
 };
 
 // A reader's place in the CTA's task stream: item fields, its task j of `tasks`.
@@ -127,6 +139,25 @@ __device__ __noinline__ bool pa_wait_more(uint32_t bar, unsigned parity, volatil
 }
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
   return pa_try_wait(smem_u32(bar), parity) || pa_wait_more(smem_u32(bar), parity, abort_flag);
+}
+
+// The same for a mark in global memory.
+__device__ __noinline__ bool pa_wait_ready(const unsigned long long* mark, unsigned long long token,
+                                           volatile uint32_t* abort_flag) {
+  const unsigned long long t0 = global_ns();
+  while (true) {
+    unsigned long long v;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(mark) : "memory");
+    if (v == token) return true;
+    if (*abort_flag) return false;
+    if (global_ns() - t0 > TC_WAIT_NS) {
+      if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void store_release(unsigned long long* p, unsigned long long v) {
+  asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 
 __device__ __forceinline__ void pa_arrive(uint64_t* bar) {
@@ -248,7 +279,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   uint32_t* ctl = reinterpret_cast<uint32_t*>(bars + 48);                   // [0] tmem base, [1] abort
   PaItem* queue = reinterpret_cast<PaItem*>(bars + 49);                     // [PA_QUEUE]
   float2* s_ml = reinterpret_cast<float2*>(bars + 49 + PA_QUEUE * sizeof(PaItem) / 8);   // [128] slot 1's (m, l)
-  static_assert((49 + 128) * 8 + PA_QUEUE * sizeof(PaItem) <= 2048, "control block");
+  PaJoinList* s_join = reinterpret_cast<PaJoinList*>(s_ml + 128);
+  static_assert((49 + 128) * 8 + PA_QUEUE * sizeof(PaItem) + sizeof(PaJoinList) <= 3072, "control block");
   volatile uint32_t* abort_flag = &ctl[1];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -275,6 +307,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       mbar_init(&kv_empty[i], 1);
     }
     ctl[1] = 0u;
+    s_join->n = s_join->left = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -518,8 +551,73 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       if (lane == 0) {
         pa_arrive(&o_empty[sl]);
         if (join) pa_arrive(&o_empty[1]);
+        if (out_mode == PA_PIECE && p.prefix == 0) {   // these rows of the piece are written
+          __threadfence();
+          store_release(&p.ready[(int64_t)out_at * 8 + (prow >> 5)], p.token);
+        }
       }
       item_done();
+    }
+    // ---- the item whose last piece this CTA holds: join its pieces, in CTA order --------
+    if (ok && s_join->n > 0) {
+      const int n = s_join->n, words = s_join->n_tok > TT ? 8 : 4;
+      // the other pieces belong to CTAs before this one, and were the last of their whole items
+      bool got = true;
+#pragma unroll 1
+      for (int e = lane; got && e < n * words; e += 32)
+        got = pa_wait_ready(&p.ready[s_join->slot[e / words] * 8 + e % words], p.token, abort_flag);
+      __syncwarp();
+      __threadfence();
+      if (__all_sync(0xffffffffu, got)) {
+        // a thread owns a row (of the next power of two) and every so many 16-dim units of it
+        const int rows = s_join->n_tok * G, shift = 32 - __clz(rows - 1 | 1);
+        const int r = tid & ((1 << shift) - 1), tok = r / G, g = r - tok * G, tile = tok >= TT ? 1 : 0;
+        const int prow = tile * PA_ROWS + (tok - tile * TT) * G + g;
+        float m = -INFINITY, l = 0.f;
+        if (r < rows) {
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) {
+            const float2 ml = p.ml[s_join->slot[i] * 256 + prow];
+            const float mn = fmaxf(m, ml.x);
+            l = l * (m == -INFINITY ? 0.f : pf_ex2(m - mn)) + ml.y * (ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - mn));
+            m = mn;
+          }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* og = reinterpret_cast<T*>(p.out) + (int64_t)(s_join->tok0 + tok) * p.ost + (int64_t)(s_join->hk * G + g) * p.osh;
+#pragma unroll 1
+        for (int u = tid >> shift; r < rows && u * 16 < p.D; u += 256 >> shift) {
+          float4 a[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (int i = 0; i < n; ++i) {
+            const int at = s_join->slot[i];
+            const float4* src = p.o + ((int64_t)at * (D / 4) + u * 4) * 256 + prow;
+            const float x = p.ml[at * 256 + prow].x;
+            float4 o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __ldcg(src + j * 256);
+            const float f = x == -INFINITY ? 0.f : pf_ex2(x - m);
+            if (f != 0.f) {   // a piece that saw nothing holds no values
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                a[j].x += o[j].x * f; a[j].y += o[j].y * f; a[j].z += o[j].z * f; a[j].w += o[j].w * f;
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j += 2)
+            if (u * 16 + j * 4 < p.D)
+              *reinterpret_cast<uint4*>(og + u * 16 + j * 4) =
+                  make_uint4(pack2<T>(a[j].x * inv, a[j].y * inv), pack2<T>(a[j].z * inv, a[j].w * inv),
+                             pack2<T>(a[j + 1].x * inv, a[j + 1].y * inv), pack2<T>(a[j + 1].z * inv, a[j + 1].w * inv));
+        }
+        __syncwarp();
+        // the last warp takes the marks back: a replayed call starts without them
+        if (__shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&s_join->left, 1) : 0, 0) == 7)
+          for (int e = lane; e < n * words; e += 32) p.ready[s_join->slot[e / words] * 8 + e % words] = 0;
+      }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the last rows are written
     if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
@@ -799,7 +897,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
       const int64_t share = pa_share(p, total);
       const int64_t begin = min((int64_t)blockIdx.x * share, total), end = min(begin + share, total);
-      if (lane < 2) p.desc[blockIdx.x * 2 + lane].valid = 0;
+      if (p.prefix > 0 && lane < 2) p.desc[blockIdx.x * 2 + lane].valid = 0;
       __syncwarp();
       int n_items = 0;
       auto push = [&](const PaItem& w) {
@@ -814,6 +912,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         return true;
       };
       bool ok = true;
+      PaItem tail = {};
       if (begin < end) {
         // the lane whose sequences hold unit `begin`, its first one and the units before that
         const int owner = __ffs(__ballot_sync(0xffffffffu, incl > begin)) - 1;
@@ -825,8 +924,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         }
         s = __shfl_sync(0xffffffffu, s, owner);
         at = __shfl_sync(0xffffffffu, at, owner);
-        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends) {
-          if (w.out_mode == PA_PIECE && lane == 0) {
+        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends, int64_t item_at,
+                                                                int sh, int tiles) {
+          if (w.out_mode == PA_PIECE && p.prefix == 0 && !begins) {
+            // an item that earlier CTAs began comes last: its other pieces are done by then, and whoever holds its
+            // last piece joins them (waiting for lower CTAs only)
+            tail = w;
+            if (ends && lane == 0) {
+              int n = 0;
+              pa_pieces(share, item_at, sh, tiles, (int)blockIdx.x, [&](int slot) { s_join->slot[n++] = (uint16_t)slot; });
+              s_join->tok0 = w.tok0;
+              s_join->n_tok = w.n_tok;
+              s_join->hk = w.hk;
+              s_join->n = n;
+            }
+            return true;
+          }
+          if (w.out_mode == PA_PIECE && p.prefix > 0 && lane == 0) {
             PaDesc d;
             d.valid = 1;
             d.end = ends;
@@ -854,10 +968,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           return push(w);
         });
       }
+      if (ok && tail.out_mode == PA_PIECE) ok = push(tail);
       if (ok) {
-        PaItem w = {};
-        w.out_mode = PA_STOP;
-        push(w);
+        tail.out_mode = PA_STOP;
+        push(tail);
       }
     }
   }
@@ -990,33 +1104,6 @@ __device__ __forceinline__ void pa_join_rows(const PaP& p, Join& j, int rows, Ro
 __device__ __forceinline__ int pa_piece_row(const PaP& p, int tok, int g) {
   const int tile = tok / p.TT;
   return tile * PA_ROWS + (tok - tile * p.TT) * p.G + g;
-}
-
-// Items cut by a share's border: blockIdx.x is the CTA that began the item, its
-// rows are taken PA_JOIN at a time over blockIdx.y.
-template <int D, typename T>
-__global__ void __launch_bounds__(256) k_packed_combine(const PaP p) {
-  __shared__ __align__(16) PaJoin<PA_MAX_PIECES> j;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const PaDesc d = p.desc[blockIdx.x * 2 + 1];
-  if (!d.valid) return;
-  if (threadIdx.x < 32) {
-    const int n = pa_chain(p, j, 0, blockIdx.x, 0);
-    if (threadIdx.x == 0) j.n = n;
-  }
-  for (int r0 = blockIdx.y * PA_JOIN; r0 < d.n_tok * p.G; r0 += gridDim.y * PA_JOIN) {
-    const int rows = min(d.n_tok * p.G - r0, PA_JOIN);
-    __syncthreads();
-    if (threadIdx.x < rows) {
-      const int r = r0 + threadIdx.x, tok = r / p.G;
-      j.prow[threadIdx.x].x = pa_piece_row(p, tok, r - tok * p.G);
-    }
-    __syncthreads();
-    pa_join_rows<D, T>(p, j, rows, [&](int r) {
-      const int tok = (r0 + r) / p.G;
-      return make_int2(d.tok0 + tok, d.hk * p.G + r0 + r - tok * p.G);
-    });
-  }
 }
 
 // With a shared prefix every row joins its prefix part and its own part, each

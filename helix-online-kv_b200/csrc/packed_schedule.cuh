@@ -140,9 +140,27 @@ HD int64_t pa_share(const PaSched& p, int64_t total) {
   return pa_max((int64_t)((double)total * (1.0 / p.n_ctas)) + 1, PA_MIN_SHARE);
 }
 
+// The key tile at which x units behind an item's fixed part cut it (tiles of
+// 2^sh units): a tile belongs to the piece in which its units start.
+HD int pa_cut(int64_t x, int sh, int tiles) {
+  return x <= 0 ? 0 : (int)pa_min((x + ((int64_t)1 << sh) - 1) >> sh, tiles);
+}
+
+// Workspace slots of the pieces of a cut item (at unit item_at) whose last
+// piece is CTA `last`'s, in order.
+template <typename F>
+HD void pa_pieces(int64_t share, int64_t item_at, int sh, int tiles, int last, F f) {
+  ROLLED for (int c = (int)(item_at / share); c <= last; ++c) {
+    const int64_t x = (int64_t)c * share - item_at - PA_ITEM;
+    const int t0 = pa_cut(x, sh, tiles), t1 = pa_cut(x + share, sh, tiles);
+    if (t0 < t1) f(c * 2 + (t0 == 0 ? 1 : 0));
+  }
+}
+
 // CTA `cta`'s items: units [begin, end), which start in sequence s (`at` units
-// before it) or behind it.  emit(item, begins, ends): whether the piece holds the item's
-// first and its last key tile; false stops the walk.
+// before it) or behind it.  emit(item, begins, ends, ...): whether the piece
+// holds the item's first and its last key tile, and the item's place and tiles
+// (pa_pieces); false stops the walk.
 template <typename Emit>
 HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, int64_t at, Emit emit) {
   const int W = 2 * p.TT, n_s = pa_n_seqs(p);
@@ -175,11 +193,7 @@ HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, in
       ROLLED for (int hk = 0; hk < p.Hkv; ++hk, item_at += iu) {
         if (item_at + iu <= pos) continue;
         if (pos >= end) break;
-        // a tile belongs to the piece in which its units start
-        const int64_t x0 = pos - item_at - PA_ITEM, x1 = end - item_at - PA_ITEM;
-        const int64_t mask = ((int64_t)1 << sh) - 1;
-        const int t0 = x0 <= 0 ? 0 : (int)pa_min((x0 + mask) >> sh, tiles);
-        const int t1 = x1 <= 0 ? 0 : (int)pa_min((x1 + mask) >> sh, tiles);
+        const int t0 = pa_cut(pos - item_at - PA_ITEM, sh, tiles), t1 = pa_cut(end - item_at - PA_ITEM, sh, tiles);
         const bool start = pos == item_at;
         pos = pa_min(item_at + iu, end);
         if (tiles > 0 ? t0 == t1 : !start) continue;
@@ -198,7 +212,7 @@ HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, in
         w.out_mode = !(begins && ends) ? PA_PIECE : p.prefix > 0 ? PA_ROWWISE : PA_DIRECT;
         // a CTA's share begins with at most one unfinished item and ends with at most one
         w.out_at = cta * 2 + (begins ? 1 : 0);
-        if (!emit(w, begins, ends)) return false;
+        if (!emit(w, begins, ends, item_at, sh, tiles)) return false;
       }
     }
     at += units;
