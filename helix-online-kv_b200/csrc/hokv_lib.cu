@@ -1148,13 +1148,9 @@ static int launch_norm_rotate(NraP p, bool vec, cudaStream_t st) {
     return check_launch("k_norm_rotate_scalar");
   }
   const int lpr = p.D <= 64 ? 4 : p.D <= 128 ? 8 : 16;
-  // several heads share a token's angles once that leaves every SM full (2048 threads)
-  p.hpg = 1;
-  for (int n = 8; n > 1 && p.hpg == 1; n >>= 1)
-    if ((int64_t)p.T * cdiv(heads, n) * lpr >= (int64_t)pa_ctas() * 2048) p.hpg = n;
-  p.chunks = (int)cdiv(heads, p.hpg);
-  const int64_t blocks = cdiv((int64_t)p.T * p.chunks, NRA_THREADS / lpr);
-  HOKV_REQUIRE(blocks < (1ll << 31), "norm_rotate_append: grid too large");
+  // several tokens a block (longer runs, fewer starts) once that still gives every SM a few blocks
+  p.tokens = std::max(1, std::min(NRA_TOKENS, p.T / (NRA_BLOCKS * std::max(pa_ctas(), 1))));
+  const int64_t blocks = cdiv(p.T, p.tokens);
   if (lpr == 4) k_norm_rotate<T, 4><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
   else if (lpr == 8) k_norm_rotate<T, 8><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
   else k_norm_rotate<T, 16><<<(unsigned)blocks, NRA_THREADS, 0, st>>>(p);
@@ -1202,7 +1198,7 @@ extern "C" int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* str
   const int64_t st[14] = {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h, p.out_t, p.out_h, p.ks_b, p.ks_h, p.ks_t, p.vs_b, p.vs_h, p.vs_t};
   for (int i = 0; i < 14; ++i) vec = vec && st[i] % e16 == 0;
   vec = vec && aligned(p.q, 16) && aligned(p.k, 16) && aligned(p.v, 16) && aligned(p.out, 16) && aligned(p.ks, 16) &&
-        aligned(p.vs, 16);
+        aligned(p.vs, 16) && aligned(p.qw, 16) && aligned(p.kw, 16);
   if (a->dtype == HOKV_F16) return launch_norm_rotate<__half>(p, vec, S(stream));
   if (a->dtype == HOKV_BF16) return launch_norm_rotate<__nv_bfloat16>(p, vec, S(stream));
   return launch_norm_rotate<float>(p, vec, S(stream));

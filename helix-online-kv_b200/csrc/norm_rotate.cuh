@@ -11,10 +11,10 @@
 // LPR = D / 16 lanes (rounded up to a power of two) owns a row; a lane holds
 // both elements of its pairs, as two 16-byte chunks of 8 (16-bit types), so
 // the rotation needs no exchange and the norm only the sum of squares over
-// the group.  A group keeps the cosines of its token in registers over several
-// heads.  The angle is formed in 64 bits as a fraction of a turn (a position
-// of 10^6 times an fp32 frequency loses its phase in 32 bits); norms and
-// products are fp32, rounded once at the store.
+// the group.  The cosines of a token are formed once for all its heads.  The
+// angle is formed in 64 bits as a fraction of a turn (a position of 10^6 times
+// an fp32 frequency loses its phase in 32 bits); norms and products are fp32,
+// rounded once at the store.
 #pragma once
 #include "hokv_common.cuh"
 
@@ -28,11 +28,16 @@ struct NraP {
   const float* inv_freq;
   int64_t cap;
   int n_seqs, T, Hq, Hkv, D, n_freq, interleaved, zero_tail;
-  int chunks, hpg;   // head rows of a token over `chunks` groups, `hpg` each
+  int tokens;   // tokens of a block
   float eps;
 };
 
 constexpr int NRA_THREADS = 256;
+// 4 blocks of an SM (64 registers).  A 16K-token prompt of 32 + 2 x 8 heads of 128 dims, bf16 (403 MB): 80 us, 5.0 TB/s;
+// 88 with 5 blocks (48 registers, spills), 84 to 110 with 2 to 4 rows of a group on their way and 4 to 2 blocks, 103 with
+// a token's angles formed by each group that works on it; the same reads and writes without the arithmetic take 69.
+constexpr int NRA_BLOCKS = 4;
+constexpr int NRA_TOKENS = 8;   // most tokens of a block
 
 // The sequence that holds token t, by the whole warp (t warp-uniform): 32-way
 // search of the ascending starts.  n_seqs when t lies behind the last one.
@@ -88,21 +93,30 @@ __device__ __forceinline__ void nra_angle(int pos, float f, float& c, float& s) 
 }
 
 template <typename T>
-struct Vec8 {
+struct alignas(16) Vec8 {
   T x[8];
 };
+// 8 elements as they lie in memory, and as fp32.
 template <typename T>
-__device__ __forceinline__ void nra_load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(&u);
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ void nra_load8(const T* p, Raw8<T>& r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)w.x[i];
-  } else {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+}
+template <typename T>
+__device__ __forceinline__ void nra_weight8(const T* p, Vec8<T>& w) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    reinterpret_cast<uint4*>(&w)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+}
+template <typename T>
+__device__ __forceinline__ void nra_widen(const Raw8<T>& r, float (&f)[8]) {
+  const Vec8<T> w = *reinterpret_cast<const Vec8<T>*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)w.x[i];
 }
 template <typename T>
 __device__ __forceinline__ void nra_store8(T* p, const float (&f)[8]) {
@@ -117,119 +131,140 @@ __device__ __forceinline__ void nra_store8(T* p, const float (&f)[8]) {
   }
 }
 
-// Source and destination of head row h of token t (q heads, then k, then v);
-// kind 0 q, 1 k, 2 v.
+// Source of head row h of token t (q heads, then k, then v).
 template <typename T>
-__device__ __forceinline__ int nra_row(const NraP& p, int t, int h, const NraTok& k, const T*& src, T*& dst) {
+__device__ __forceinline__ const T* nra_source(const NraP& p, int t, int h) {
+  if (h < p.Hq) return reinterpret_cast<const T*>(p.q) + t * p.q_t + h * p.q_h;
+  h -= p.Hq;
+  if (h < p.Hkv) return reinterpret_cast<const T*>(p.k) + t * p.k_t + h * p.k_h;
+  return reinterpret_cast<const T*>(p.v) + t * p.v_t + (h - p.Hkv) * p.v_h;
+}
+// Its destination; returns 0 for q, 1 for k, 2 for v.
+template <typename T>
+__device__ __forceinline__ int nra_target(const NraP& p, int t, int h, const NraTok& k, T*& dst) {
   if (h < p.Hq) {
-    src = reinterpret_cast<const T*>(p.q) + t * p.q_t + h * p.q_h;
     dst = reinterpret_cast<T*>(p.out) + t * p.out_t + h * p.out_h;
     return 0;
   }
   h -= p.Hq;
-  if (h < p.Hkv) {
-    src = reinterpret_cast<const T*>(p.k) + t * p.k_t + h * p.k_h;
-    dst = reinterpret_cast<T*>(p.ks) + k.b * p.ks_b + h * p.ks_h + k.row * p.ks_t;
-    return 1;
-  }
-  h -= p.Hkv;
-  src = reinterpret_cast<const T*>(p.v) + t * p.v_t + h * p.v_h;
-  dst = reinterpret_cast<T*>(p.vs) + k.b * p.vs_b + h * p.vs_h + k.row * p.vs_t;
-  return 2;
+  const bool is_v = h >= p.Hkv;
+  dst = is_v ? reinterpret_cast<T*>(p.vs) + k.b * p.vs_b + (h - p.Hkv) * p.vs_h + k.row * p.vs_t
+             : reinterpret_cast<T*>(p.ks) + k.b * p.ks_b + h * p.ks_h + k.row * p.ks_t;
+  return is_v ? 2 : 1;
 }
 
 // Vector form: D a multiple of 16, and of the rotated dims too unless
-// interleaved.  grid (ceil(T chunks / groups of a block)).
+// interleaved.  A block takes p.tokens tokens with all their head rows: their
+// slots and angles once, through shared memory, then rows by groups of LPR
+// lanes, the next row on its way while one is worked on.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(NRA_THREADS) k_norm_rotate(const NraP p) {
-  constexpr int GROUPS = NRA_THREADS / LPR, WG = 32 / LPR;
-  const int lane = threadIdx.x & 31, l = threadIdx.x % LPR;
-  const int64_t unit = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR;
-  const int64_t units = (int64_t)p.T * p.chunks;
-  const bool live = unit < units;
-  const int t = live ? (int)(unit / p.chunks) : p.T - 1, chunk = (int)(unit % p.chunks);
-  // this lane's chunks of 8: both halves of its pairs
-  const int nl = p.D / 16, lr = p.interleaved ? 0 : p.n_freq / 8;   // lanes in use, lanes of the half-split rotation
-  const bool on = live && l < nl;
-  const int ca = l < lr ? l : 2 * lr + 2 * (l - lr), cb = l < lr ? l + lr : ca + 1;
+__global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const NraP p) {
+  constexpr int GROUPS = NRA_THREADS / LPR;
+  __shared__ NraTok s_tok[NRA_TOKENS];
+  __shared__ __align__(16) float2 s_cs[NRA_TOKENS][128 + 8];   // cos, sin
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = threadIdx.x % LPR;
+  const int t0 = (int)blockIdx.x * p.tokens, n_tok = min(p.tokens, p.T - t0);
   const int heads = p.Hq + 2 * p.Hkv;
-
-  // the token of each of the warp's groups (usually one for all of them)
-  NraTok tok;
-  if (p.chunks >= WG && __all_sync(0xffffffffu, t == __shfl_sync(0xffffffffu, t, 0))) {
-    tok = nra_token(p, __shfl_sync(0xffffffffu, t, 0));
-  } else {
-    for (int g = 0; g < WG; ++g) {
-      const NraTok k = nra_token(p, __shfl_sync(0xffffffffu, t, g * LPR));
-      if (lane / LPR == g) tok = k;
+  // this lane's chunks of 8: both halves of its pairs
+  const int lr = p.interleaved ? 0 : p.n_freq / 8;   // lanes of the half-split rotation
+  const bool on = l < p.D / 16;
+  const int ca = l < lr ? l : 2 * lr + 2 * (l - lr), cb = l < lr ? l + lr : ca + 1;
+  Raw8<T> next[2];
+  int fk = 0, fh = threadIdx.x / LPR;   // the next row to fetch: token and head
+  auto fetch = [&](Raw8<T> (&x)[2]) __attribute__((always_inline)) {
+    while (fh >= heads) fh -= heads, ++fk;
+    if (on && fk < n_tok) {
+      const T* src = nra_source<T>(p, t0 + fk, fh);
+      nra_load8(src + ca * 8, x[0]);
+      nra_load8(src + cb * 8, x[1]);
     }
+    fh += GROUPS;
+  };
+  fetch(next);
+  if (warp < n_tok) {
+    const NraTok k = nra_token(p, t0 + warp);
+    if (lane == 0) s_tok[warp] = k;
   }
-  float c[8], s[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    c[j] = 1.f;
-    s[j] = 0.f;
-    const int f = 8 * l + j;
-    if (on && f < p.n_freq) nra_angle(tok.pos, p.inv_freq[f], c[j], s[j]);
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_tok * p.n_freq; e += NRA_THREADS) {
+    const int k = e / p.n_freq, f = e - k * p.n_freq;
+    float2 cs;
+    nra_angle(s_tok[k].pos, p.inv_freq[f], cs.x, cs.y);
+    s_cs[k][f] = cs;
   }
-  for (int i = 0; i < p.hpg; ++i) {
-    const int h = chunk + i * p.chunks;
-    const bool row_on = on && h < heads;
-    const T* src = nullptr;
-    T* dst = nullptr;
-    const int kind = nra_row<T>(p, t, min(h, heads - 1), tok, src, dst);
-    float a[8] = {}, b[8] = {};
-    if (row_on) {
-      nra_load8(src + ca * 8, a);
-      nra_load8(src + cb * 8, b);
-    }
+  __syncthreads();
+  const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
+  int k = 0, h = threadIdx.x / LPR;
+#pragma unroll 1
+  while (true) {
+    while (h >= heads) h -= heads, ++k;
+    if (k >= n_tok) break;
+    float a[8], b[8];
+    nra_widen(next[0], a);
+    nra_widen(next[1], b);
+    fetch(next);
+    const NraTok tok = s_tok[k];
+    T* dst;
+    const int kind = nra_target<T>(p, t0 + k, h, tok, dst);
+    h += GROUPS;
     if (kind < 2) {
       const T* w = reinterpret_cast<const T*>(kind == 0 ? p.qw : p.kw);
       if (w) {   // uniform over the group: its lanes share the row
         float ss = 0.f;
+        if (on) {
+          float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += a[j] * a[j] + b[j] * b[j];
-        const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
+          for (int j = 0; j < 8; ++j) s2 = __ffma2_rn(make_float2(a[j], b[j]), make_float2(a[j], b[j]), s2);
+          ss = s2.x + s2.y;
+        }
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float r = rsqrtf(ss / (float)p.D + p.eps);
-        if (row_on) {
+        const float q = rsqrtf(ss / (float)p.D + p.eps);
+        if (on) {
+          Vec8<T> wa, wb;
+          nra_weight8(w + ca * 8, wa);
+          nra_weight8(w + cb * 8, wb);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            a[j] *= r * (float)w[ca * 8 + j];
-            b[j] *= r * (float)w[cb * 8 + j];
+            const float2 y = __fmul2_rn(make_float2(a[j], b[j]),
+                                        __fmul2_rn(make_float2((float)wa.x[j], (float)wb.x[j]), make_float2(q, q)));
+            a[j] = y.x;
+            b[j] = y.y;
           }
         }
       }
+      const float2* cs = &s_cs[k][8 * l];
       if (p.interleaved) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (8 * l + j < p.n_freq) {
             const float x = a[2 * j], y = a[2 * j + 1];
-            a[2 * j] = x * c[j] - y * s[j];
-            a[2 * j + 1] = y * c[j] + x * s[j];
+            a[2 * j] = x * cs[j].x - y * cs[j].y;
+            a[2 * j + 1] = y * cs[j].x + x * cs[j].y;
           }
           if (8 * l + 4 + j < p.n_freq) {
             const float x = b[2 * j], y = b[2 * j + 1];
-            b[2 * j] = x * c[j + 4] - y * s[j + 4];
-            b[2 * j + 1] = y * c[j + 4] + x * s[j + 4];
+            b[2 * j] = x * cs[j + 4].x - y * cs[j + 4].y;
+            b[2 * j + 1] = y * cs[j + 4].x + x * cs[j + 4].y;
           }
         }
       } else if (l < lr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = a[j], y = b[j];
-          a[j] = x * c[j] - y * s[j];
-          b[j] = y * c[j] + x * s[j];
+        for (int j = 0; j < 8; j += 2) {
+          const float4 c = *reinterpret_cast<const float4*>(cs + j);
+          const float x0 = a[j], y0 = b[j], x1 = a[j + 1], y1 = b[j + 1];
+          a[j] = x0 * c.x - y0 * c.y;
+          b[j] = y0 * c.x + x0 * c.y;
+          a[j + 1] = x1 * c.z - y1 * c.w;
+          b[j + 1] = y1 * c.z + x1 * c.w;
         }
       }
-    }
-    const bool store = kind == 0 ? tok.b >= 0 || p.zero_tail : tok.keep;
-    if (kind == 0 && tok.b < 0) {
+      if (kind == 0 && tok.b < 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+        for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+      }
     }
-    if (row_on && store) {
+    if (on && (kind == 0 ? tok.b >= 0 || p.zero_tail : tok.keep)) {
       nra_store8(dst + ca * 8, a);
       nra_store8(dst + cb * 8, b);
     }
@@ -246,9 +281,9 @@ __global__ void __launch_bounds__(NRA_THREADS) k_norm_rotate_scalar(const NraP p
   if (row >= (int64_t)p.T * heads) return;
   const int t = (int)(row / heads), h = (int)(row % heads);
   const NraTok tok = nra_token(p, t);
-  const T* src;
+  const T* src = nra_source<T>(p, t, h);
   T* dst;
-  const int kind = nra_row<T>(p, t, h, tok, src, dst);
+  const int kind = nra_target<T>(p, t, h, tok, dst);
   // pair e: rotated for e < n_freq, then the dims left over, two by two
   float a[4], b[4];
   float ss = 0.f;
