@@ -915,19 +915,17 @@ static int pa_ctas() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return std::min(sms, 240);   // the piece lists of the combine kernels hold 256
+  return std::min(sms, 255);   // k_packed_combine_rows takes CTA numbers of 8 bits
 }
 
 // Workspace layout (offsets in bytes; total in `bytes`).
 struct PaWs {
-  size_t desc, ready, ml, o, info, row_ml, row_o, bytes;
+  size_t ready, ml, o, info, row_ml, row_o, bytes;
 };
 static PaWs pa_ws(const hokv_packed_args* a, int ctas) {
   PaWs w;
   const size_t dp = a->head_dim <= 64 ? 64 : 128;
   size_t at = 0;
-  w.desc = at;
-  at += pa_up((size_t)ctas * 2 * sizeof(PaDesc));
   w.ready = at;
   at += pa_up((size_t)ctas * 2 * 8 * 8);
   w.ml = at;
@@ -1098,7 +1096,6 @@ static int packed_attention(const hokv_packed_args* a, void* stream) {
   p.n_ctas = ctas;
   p.sl2 = a->scale * PA_LOG2E;
   unsigned char* w = reinterpret_cast<unsigned char*>(a->workspace);
-  p.desc = reinterpret_cast<PaDesc*>(w + ws.desc);
   p.ready = reinterpret_cast<unsigned long long*>(w + ws.ready);
   p.token = pa_token();
   p.ml = reinterpret_cast<float2*>(w + ws.ml);

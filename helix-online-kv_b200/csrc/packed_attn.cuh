@@ -67,13 +67,7 @@ struct PaGeo {
   static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
   static constexpr int STAGES = D == 64 ? 8 : 4;          // ring of K and V tiles
   static constexpr int OUT_BYTES = 8 * 4096;              // 32 rows x 64 dims of O per softmax warp, on their way out
-  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + OUT_BYTES + 3072;
-};
-
-// Piece descriptors of a CTA: [0] the piece that continues an earlier CTA's
-// item, [1] the piece that begins an item it does not finish.
-struct PaDesc {
-  int valid, end, tok0, n_tok, hk, pad[3];
+  static constexpr int SMEM = 2 * Q_BYTES + STAGES * KV_BYTES + OUT_BYTES + 2048;
 };
 
 struct alignas(64) PaMaps {
@@ -86,22 +80,22 @@ struct PaP : PaSched {
   int Hq, G, D, zero_tail, tma_out;   // tma_out: tokens of a warp's 32 rows, 0 when they are not whole tokens
   float sl2;                     // scale * log2(e)
   int k_t, k_h, k_b, v_t, v_h, v_b, pk_t, pk_h, pk_b, pv_t, pv_h, pv_b;   // coordinate slots of the maps
-  PaDesc* desc;                  // [n_ctas][2]
   float2* ml;                    // [n_ctas][2][256] (running maximum, sum)
   float4* o;                     // [n_ctas][2][D / 4][256]
   unsigned long long* ready;     // [n_ctas][2][8] the call's token when 32 rows of a piece are written, then 0 again
   unsigned long long token;      // this call's
-  int2* tok_info;                // prefix only: [2][T][Hkv] (first CTA or -1: row-wise, token in item)
+  int2* tok_info;                // prefix only: [2][T][Hkv] (first | last CTA << 8 or -1: row-wise, token in item)
   float2* row_ml;                // prefix only: [2][T][Hq]
   float4* row_o;                 // prefix only: [2][T][Hq][D / 4]
 };
 
 // The item that this CTA joins at its end: the one whose last piece it holds.
-struct PaJoinList {
-  int n, tok0, n_tok, hk;      // pieces (0: none to join), rows
-  int left;                    // softmax warps that have joined their part
-  uint16_t slot[240];
+struct PaJoinItem {
+  int n, first, tok0, n_tok, hk;   // pieces (0: none to join) from CTA `first` on, rows
+  int left;                        // softmax warps that have joined their part
 };
+// Workspace slot of piece i of an item whose first one is CTA `first`'s.
+__device__ __forceinline__ int pa_slot(int first, int i) { return (first + i) * 2 + (i == 0 ? 1 : 0); }
 
 // A reader's place in the CTA's task stream: item fields, its task j of `tasks`.
 struct PaCursor {
@@ -279,8 +273,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   uint32_t* ctl = reinterpret_cast<uint32_t*>(bars + 48);                   // [0] tmem base, [1] abort
   PaItem* queue = reinterpret_cast<PaItem*>(bars + 49);                     // [PA_QUEUE]
   float2* s_ml = reinterpret_cast<float2*>(bars + 49 + PA_QUEUE * sizeof(PaItem) / 8);   // [128] slot 1's (m, l)
-  PaJoinList* s_join = reinterpret_cast<PaJoinList*>(s_ml + 128);
-  static_assert((49 + 128) * 8 + PA_QUEUE * sizeof(PaItem) + sizeof(PaJoinList) <= 3072, "control block");
+  PaJoinItem* s_join = reinterpret_cast<PaJoinItem*>(s_ml + 128);
+  static_assert((49 + 128) * 8 + PA_QUEUE * sizeof(PaItem) + sizeof(PaJoinItem) <= 2048, "control block");
   volatile uint32_t* abort_flag = &ctl[1];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -560,12 +554,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     }
     // ---- the item whose last piece this CTA holds: join its pieces, in CTA order --------
     if (ok && s_join->n > 0) {
-      const int n = s_join->n, words = s_join->n_tok > TT ? 8 : 4;
+      const int n = s_join->n, first = s_join->first, words = s_join->n_tok > TT ? 8 : 4;
       // the other pieces belong to CTAs before this one, and were the last of their whole items
       bool got = true;
 #pragma unroll 1
       for (int e = lane; got && e < n * words; e += 32)
-        got = pa_wait_ready(&p.ready[s_join->slot[e / words] * 8 + e % words], p.token, abort_flag);
+        got = pa_wait_ready(&p.ready[pa_slot(first, e / words) * 8 + e % words], p.token, abort_flag);
       __syncwarp();
       __threadfence();
       if (__all_sync(0xffffffffu, got)) {
@@ -577,7 +571,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (r < rows) {
 #pragma unroll 4
           for (int i = 0; i < n; ++i) {
-            const float2 ml = p.ml[s_join->slot[i] * 256 + prow];
+            const float2 ml = p.ml[pa_slot(first, i) * 256 + prow];
             const float mn = fmaxf(m, ml.x);
             l = l * (m == -INFINITY ? 0.f : pf_ex2(m - mn)) + ml.y * (ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - mn));
             m = mn;
@@ -592,7 +586,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           for (int j = 0; j < 4; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
           for (int i = 0; i < n; ++i) {
-            const int at = s_join->slot[i];
+            const int at = pa_slot(first, i);
             const float4* src = p.o + ((int64_t)at * (D / 4) + u * 4) * 256 + prow;
             const float x = p.ml[at * 256 + prow].x;
             float4 o[4];
@@ -616,7 +610,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         __syncwarp();
         // the last warp takes the marks back: a replayed call starts without them
         if (__shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&s_join->left, 1) : 0, 0) == 7)
-          for (int e = lane; e < n * words; e += 32) p.ready[s_join->slot[e / words] * 8 + e % words] = 0;
+          for (int e = lane; e < n * words; e += 32) p.ready[pa_slot(first, e / words) * 8 + e % words] = 0;
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the last rows are written
@@ -897,8 +891,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
       const int64_t share = pa_share(p, total);
       const int64_t begin = min((int64_t)blockIdx.x * share, total), end = min(begin + share, total);
-      if (p.prefix > 0 && lane < 2) p.desc[blockIdx.x * 2 + lane].valid = 0;
-      __syncwarp();
       int n_items = 0;
       auto push = [&](const PaItem& w) {
         const int qi = n_items % PA_QUEUE, use = n_items / PA_QUEUE;
@@ -924,36 +916,40 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         }
         s = __shfl_sync(0xffffffffu, s, owner);
         at = __shfl_sync(0xffffffffu, at, owner);
-        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, [&](const PaItem& w, bool begins, bool ends, int64_t item_at,
-                                                                int sh, int tiles) {
+        PaSeq q = pa_seq(p, s);
+#pragma unroll 1
+        for (int64_t units; per > 1 && at + (units = pa_seq_units(p, q)) <= begin; q = pa_seq(p, ++s)) at += units;
+        // its last pair that starts at or before `begin`, 32 at a time
+        int pr = 0;
+#pragma unroll 1
+        for (int n = (q.nq + 2 * TT - 1) / (2 * TT); n > 1;) {
+          const int step = (n + 31) / 32, probe = min(pr + lane * step, pr + n - 1);
+          const bool before = at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, 2 * TT, probe) <= begin;
+          const int k = 31 - __clz(__ballot_sync(0xffffffffu, before && lane * step < n));   // lane 0 always is
+          n = min(step, n - k * step);
+          pr += k * step;
+        }
+        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, pr, [&](const PaItem& w, bool begins, bool ends,
+                                                                    int64_t item_at, int sh, int tiles) {
           if (w.out_mode == PA_PIECE && p.prefix == 0 && !begins) {
             // an item that earlier CTAs began comes last: its other pieces are done by then, and whoever holds its
             // last piece joins them (waiting for lower CTAs only)
             tail = w;
             if (ends && lane == 0) {
-              int n = 0;
-              pa_pieces(share, item_at, sh, tiles, (int)blockIdx.x, [&](int slot) { s_join->slot[n++] = (uint16_t)slot; });
+              s_join->first = pa_first_cta(share, item_at);
               s_join->tok0 = w.tok0;
               s_join->n_tok = w.n_tok;
               s_join->hk = w.hk;
-              s_join->n = n;
+              s_join->n = (int)blockIdx.x - s_join->first + 1;
             }
             return true;
           }
-          if (w.out_mode == PA_PIECE && p.prefix > 0 && lane == 0) {
-            PaDesc d;
-            d.valid = 1;
-            d.end = ends;
-            d.tok0 = w.tok0;
-            d.n_tok = w.n_tok;
-            d.hk = w.hk;
-            p.desc[w.out_at] = d;
-          }
-          if (p.prefix > 0 && begins)   // where k_packed_combine_rows finds this item's rows
+          if (p.prefix > 0 && begins) {   // where k_packed_combine_rows finds this item's rows
+            const int info = ends ? -1 : (int)blockIdx.x | pa_last_cta(share, item_at, sh, tiles) << 8;
 #pragma unroll 1
             for (int i = lane; i < w.n_tok; i += 32)
-              p.tok_info[((int64_t)w.src * p.T + w.tok0 + i) * p.Hkv + w.hk] =
-                  make_int2(ends ? -1 : (int)blockIdx.x, i);
+              p.tok_info[((int64_t)w.src * p.T + w.tok0 + i) * p.Hkv + w.hk] = make_int2(info, i);
+          }
           if (w.j0 == w.j1) {   // nothing to see: zeros, or an empty part of a row
 #pragma unroll 1
             for (int e = lane; e < w.n_tok * G * (p.D / 8); e += 32) {
@@ -985,158 +981,84 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   }
 }
 
-// ---- joining pieces ------------------------------------------------------------
-// A block joins up to PA_JOIN rows of one KV head.  Bound by latency, not
-// bytes: a long key axis cut over every SM leaves dozens of pieces of a few
-// rows each, so the statistics of all pieces are read at once, the weights
-// 2^(m - max m) go through shared memory and the sums run over independent
-// loads.  Pieces are added in CTA order (and, for half the threads' worth of
-// elements, in two interleaved halves): the same result each run.
-
-constexpr int PA_JOIN = 8;
-constexpr int PA_MAX_PIECES = 256;       // of one source: 240 CTAs at most
-
-template <int PIECES>
-struct PaJoin {
-  int n;                        // pieces
-  int piece[PIECES];            // workspace slot, or -1 - src: the row-wise result of that source
-  int2 prow[PA_JOIN];           // row in a piece, by source of the piece (x: own keys, y: prefix)
-  float m[PIECES * PA_JOIN];               // statistics; m becomes the weight
-  alignas(16) float l[PIECES * PA_JOIN];   // (reused for float4 sums)
-  float inv[PA_JOIN];
-};
-constexpr int PA_SECOND = 1 << 20;       // flag of a slot that holds the prefix's rows
-
-// Appends the pieces of an item begun by CTA `first` (its slot 1, then slot 0
-// of the valid CTAs after it, up to the one that ends it) to j; one warp.
-template <typename Join>
-__device__ __forceinline__ int pa_chain(const PaP& p, Join& j, int n, int first, int flag) {
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) j.piece[n] = (first * 2 + 1) | flag;
-  ++n;
-  for (int c = first + 1; c < p.n_ctas; c += 32) {
-    const int i = c + lane;
-    int valid = 0, end = 0;
-    if (i < p.n_ctas) {
-      valid = p.desc[i * 2].valid;
-      end = p.desc[i * 2].end;
-    }
-    const unsigned val = __ballot_sync(0xffffffffu, valid != 0);
-    const unsigned fin = __ballot_sync(0xffffffffu, valid && end);
-    const unsigned use = fin ? val & ((2u << (__ffs(fin) - 1)) - 1u) : val;
-    if (use >> lane & 1) j.piece[n + __popc(use & ((1u << lane) - 1u))] = (i * 2) | flag;
-    n += __popc(use);
-    if (fin) break;
-  }
-  return n;
-}
-
-// Rows [0, rows) of the block: row r is out row `t(r)`, head `h(r)`.
-template <int D, typename T, typename Join, typename RowOf>
-__device__ __forceinline__ void pa_join_rows(const PaP& p, Join& j, int rows, RowOf row_of) {
-  const int n = j.n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < n * PA_JOIN; e += 256) {
-    const int r = e % PA_JOIN, at = j.piece[e / PA_JOIN];
-    float2 v = make_float2(-INFINITY, 0.f);
-    if (r < rows) {
-      if (at < 0) {
-        const int2 th = row_of(r);
-        v = p.row_ml[((int64_t)(-1 - at) * p.T + th.x) * p.Hq + th.y];
-      } else {
-        v = p.ml[(int64_t)(at & (PA_SECOND - 1)) * 256 + (at & PA_SECOND ? j.prow[r].y : j.prow[r].x)];
-      }
-    }
-    j.m[e] = v.x;
-    j.l[e] = v.y;
-  }
-  __syncthreads();
-  {   // warp r: the weights of row r
-    float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, j.m[i * PA_JOIN + warp]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    for (int i = lane; i < n; i += 32) {
-      const float x = j.m[i * PA_JOIN + warp];
-      const float f = x == -INFINITY ? 0.f : pf_ex2(x - m);
-      j.m[i * PA_JOIN + warp] = f;
-      l += j.l[i * PA_JOIN + warp] * f;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) j.inv[warp] = l == 0.f ? 0.f : 1.f / l;
-  }
-  __syncthreads();
-  constexpr int E = PA_JOIN * (D / 4), HALVES = 256 / E;
-  const int e = threadIdx.x % E, half = threadIdx.x / E, r = e % PA_JOIN, d4 = e / PA_JOIN;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (r < rows && d4 * 4 < p.D) {
-    const int2 th = row_of(r);
-    const int2 pr = j.prow[r];
-#pragma unroll 8
-    for (int i = half; i < n; i += HALVES) {
-      const int at = j.piece[i];
-      const float4* src = at < 0 ? p.row_o + (((int64_t)(-1 - at) * p.T + th.x) * p.Hq + th.y) * (D / 4) + d4
-                                 : p.o + ((int64_t)(at & (PA_SECOND - 1)) * (D / 4) + d4) * 256 +
-                                       (at & PA_SECOND ? pr.y : pr.x);
-      const float4 o = *src;
-      const float f = j.m[i * PA_JOIN + r];
-      if (f != 0.f) {   // a part that saw nothing holds no values
-        a.x += o.x * f; a.y += o.y * f; a.z += o.z * f; a.w += o.w * f;
-      }
-    }
-  }
-  if (HALVES == 2) {
-    __syncthreads();
-    float4* other = reinterpret_cast<float4*>(j.l);
-    if (half == 1) other[e] = a;
-    __syncthreads();
-    const float4 b = other[e];
-    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-  }
-  if (half == 0 && r < rows && d4 * 4 < p.D) {
-    const int2 th = row_of(r);
-    const float inv = j.inv[r];
-    T* og = reinterpret_cast<T*>(p.out) + (int64_t)th.x * p.ost + (int64_t)th.y * p.osh + d4 * 4;
-    *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-  }
-}
-
-__device__ __forceinline__ int pa_piece_row(const PaP& p, int tok, int g) {
-  const int tile = tok / p.TT;
-  return tile * PA_ROWS + (tok - tile * p.TT) * p.G + g;
-}
-
+// ---- joining the parts of a row ----------------------------------------------------
 // With a shared prefix every row joins its prefix part and its own part, each
 // one row-wise result or the pieces of a cut item.  Grid (tokens, KV heads,
-// heads of a group in steps of PA_JOIN).
+// heads of a group in steps of PA_JOIN).  Bound by latency, not bytes: a long
+// prefix cut over every SM leaves dozens of pieces of a few rows.  The warps
+// take pieces in turn, each with running statistics of its own, and meet once
+// in shared memory; both orders are fixed: the same result each run.
+constexpr int PA_JOIN = 8;
+
 template <int D, typename T>
 __global__ void __launch_bounds__(256) k_packed_combine_rows(const PaP p) {
-  __shared__ __align__(16) PaJoin<2 * PA_MAX_PIECES> j;
+  constexpr int K = D / 16;   // 4-dim groups of a lane
+  __shared__ float2 s_ml[8][PA_JOIN];
+  __shared__ __align__(16) float4 s_o[8][K][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int t = blockIdx.x, hk = blockIdx.y, g0 = blockIdx.z * PA_JOIN, rows = min(p.G - g0, PA_JOIN);
+  const int t = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane % PA_JOIN, g = blockIdx.z * PA_JOIN + r, hq = hk * p.G + min(g, p.G - 1);
   if (t >= pa_used(p)) return;
-  if (threadIdx.x < 32) {
-    int n = 0;
-    for (int src = 0; src < 2; ++src) {
-      int2 info = p.tok_info[((int64_t)src * p.T + t) * p.Hkv + hk];
-      info.x = min(max(info.x, -1), p.n_ctas - 1);      // a token that no valid sequence covers has no entry
-      info.y = min(max(info.y, 0), 2 * p.TT - 1);
-      if (info.x < 0) {
-        if (threadIdx.x == 0) j.piece[n] = -1 - src;
-        ++n;
-      } else {
-        n = pa_chain(p, j, n, info.x, src ? PA_SECOND : 0);
-      }
-      if (threadIdx.x < rows) {
-        const int r = pa_piece_row(p, info.y, g0 + threadIdx.x);
-        if (src) j.prow[threadIdx.x].y = r;
-        else j.prow[threadIdx.x].x = r;
-      }
-    }
-    if (threadIdx.x == 0) j.n = n;
+  int first[2], n[2], prow[2];   // own keys, prefix
+#pragma unroll
+  for (int src = 0; src < 2; ++src) {
+    const int2 info = p.tok_info[((int64_t)src * p.T + t) * p.Hkv + hk];
+    // a token that no valid sequence covers has no entry: any value stays inside the workspace
+    const int tok = min(max(info.y, 0), 2 * p.TT - 1), tile = tok >= p.TT ? 1 : 0;
+    prow[src] = tile * PA_ROWS + (tok - tile * p.TT) * p.G + hq - hk * p.G;
+    first[src] = info.x < 0 ? -1 : min(info.x & 255, p.n_ctas - 1);
+    n[src] = info.x < 0 ? 1 : max(min(info.x >> 8, p.n_ctas - 1) - first[src] + 1, 1);
   }
+  float m = -INFINITY, l = 0.f;
+  float4 a[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int i = warp; i < n[0] + n[1]; i += 8) {
+    const int src = i < n[0] ? 0 : 1, piece = src ? i - n[0] : i;
+    const int64_t rw = ((int64_t)src * p.T + t) * p.Hq + hq;
+    const int64_t at = pa_slot(first[src], piece);
+    const bool rowwise = first[src] < 0;
+    const float2 ml = rowwise ? p.row_ml[rw] : p.ml[at * 256 + prow[src]];
+    const float4* base = rowwise ? p.row_o + rw * (D / 4) : p.o + at * (D / 4) * 256 + prow[src];
+    const int step = rowwise ? 1 : 256;
+    float4 o[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) o[k] = base[(int64_t)((lane >> 3) + 4 * k) * step];
+    if (ml.x != -INFINITY) {   // a part that saw nothing holds no values
+      const float mn = fmaxf(m, ml.x);
+      const float fa = m == -INFINITY ? 0.f : pf_ex2(m - mn), fb = pf_ex2(ml.x - mn);
+      l = l * fa + ml.y * fb;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        a[k].x = a[k].x * fa + o[k].x * fb; a[k].y = a[k].y * fa + o[k].y * fb;
+        a[k].z = a[k].z * fa + o[k].z * fb; a[k].w = a[k].w * fa + o[k].w * fb;
+      }
+      m = mn;
+    }
+  }
+  if (lane < PA_JOIN) s_ml[warp][r] = make_float2(m, l);
+#pragma unroll
+  for (int k = 0; k < K; ++k) s_o[warp][k][lane] = a[k];
   __syncthreads();
-  pa_join_rows<D, T>(p, j, rows, [&](int r) { return make_int2(t, hk * p.G + g0 + r); });
+  const int d = ((lane >> 3) + 4 * warp) * 4;   // warp k takes the lanes' group k
+  if (warp >= K || g >= p.G || d >= p.D) return;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, s_ml[w][r].x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float2 ml = s_ml[w][r];
+    const float f = ml.x == -INFINITY ? 0.f : pf_ex2(ml.x - m);
+    const float4 x = s_o[w][warp][lane];
+    l += ml.y * f;
+    o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* og = reinterpret_cast<T*>(p.out) + (int64_t)t * p.ost + (int64_t)hq * p.osh + d;
+  *reinterpret_cast<uint2*>(og) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
 }  // namespace hokv

@@ -146,42 +146,42 @@ HD int pa_cut(int64_t x, int sh, int tiles) {
   return x <= 0 ? 0 : (int)pa_min((x + ((int64_t)1 << sh) - 1) >> sh, tiles);
 }
 
-// Workspace slots of the pieces of a cut item (at unit item_at) whose last
-// piece is CTA `last`'s, in order.
-template <typename F>
-HD void pa_pieces(int64_t share, int64_t item_at, int sh, int tiles, int last, F f) {
-  ROLLED for (int c = (int)(item_at / share); c <= last; ++c) {
-    const int64_t x = (int64_t)c * share - item_at - PA_ITEM;
-    const int t0 = pa_cut(x, sh, tiles), t1 = pa_cut(x + share, sh, tiles);
-    if (t0 < t1) f(c * 2 + (t0 == 0 ? 1 : 0));
-  }
+// The CTAs that hold the first and the last piece of a cut item at unit
+// item_at: its pieces are slot 1 of the first and slot 0 of every CTA behind it
+// up to the last (a share is longer than a key tile, so none is empty).
+HD int pa_first_cta(int64_t share, int64_t item_at) {
+  const int c = (int)(item_at / share);   // unless only the units ahead of its keys lie there
+  return (int64_t)(c + 1) * share - item_at - PA_ITEM > 0 ? c : c + 1;
+}
+HD int pa_last_cta(int64_t share, int64_t item_at, int sh, int tiles) {
+  return (int)((item_at + PA_ITEM + ((int64_t)(tiles - 1) << sh)) / share);
 }
 
-// CTA `cta`'s items: units [begin, end), which start in sequence s (`at` units
-// before it) or behind it.  emit(item, begins, ends, ...): whether the piece
+// The last pair of sequence q (`at` units before it) that starts at or before
+// unit pos.
+HD int pa_find_pair(const PaSched& p, const PaSeq& q, int64_t at, int64_t pos) {
+  const int W = 2 * p.TT;
+  int lo = 0, hi = (q.nq + W - 1) / W - 1;
+  ROLLED while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, mid) <= pos) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// CTA `cta`'s items: units [begin, end), which start in pair `pr` of sequence s
+// (`at` units before it).  emit(item, begins, ends, ...): whether the piece
 // holds the item's first and its last key tile, and the item's place and tiles
-// (pa_pieces); false stops the walk.
+// (pa_first_cta, pa_last_cta); false stops the walk.
 template <typename Emit>
-HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, int64_t at, Emit emit) {
+HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, int64_t at, int pr, Emit emit) {
   const int W = 2 * p.TT, n_s = pa_n_seqs(p);
   int64_t pos = begin;
   ROLLED for (; s < n_s && pos < end; ++s) {
     const PaSeq q = pa_seq(p, s);
-    const int64_t units = pa_seq_units(p, q);
-    if (at + units <= pos) {
-      at += units;
-      continue;
-    }
+    if (q.nq <= 0) continue;
     const int np = (q.nq + W - 1) / W;
-    int pr = 0;
-    if (pos > at) {   // the last pair that starts at or before pos
-      int hi = np - 1;
-      ROLLED while (pr < hi) {
-        const int mid = (pr + hi + 1) >> 1;
-        if (at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, mid) <= pos) pr = mid;
-        else hi = mid - 1;
-      }
-    }
     int64_t item_at = at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, pr);
     ROLLED for (; pr < np && pos < end; ++pr) {
       const int left = q.nq - pr * W;
@@ -215,7 +215,8 @@ HD bool pa_walk(const PaSched& p, int cta, int64_t begin, int64_t end, int s, in
         if (!emit(w, begins, ends, item_at, sh, tiles)) return false;
       }
     }
-    at += units;
+    at = item_at;
+    pr = 0;
   }
   return true;
 }

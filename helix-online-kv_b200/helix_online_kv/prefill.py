@@ -192,7 +192,7 @@ def _packed(what, query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
     device = geometry[0][3]
     with L.on_device(device):
         if out is None:
-            out = query.new_empty(query.shape)
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         if not query.numel():
             return out
         a = L.PackedArgs.from_buffer_copy(known[0])

@@ -103,7 +103,7 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     device = geometry[0][3]
     with L.on_device(device):
         if out is None:
-            out = query.new_empty(query.shape)
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         if not known.n_tokens:
             return out
         a = L.NormRotateArgs.from_buffer_copy(known)

@@ -19,14 +19,16 @@ int64_t host_schedule(const int* cu_q, const int* cu_k, const int* kv_len, int n
   for (int c = 0; c < n_ctas; ++c) {
     const int64_t begin = pa_min(c * share, total), end = pa_min(begin + share, total);
     if (begin >= end) continue;
-    const bool ok = pa_walk(p, c, begin, end, 0, 0, [&](const PaItem& w, bool begins, bool ends, int64_t item_at, int sh, int tiles) {
+    int s = 0;
+    int64_t at = 0;
+    for (; at + pa_seq_units(p, pa_seq(p, s)) <= begin; ++s) at += pa_seq_units(p, pa_seq(p, s));
+    const bool ok = pa_walk(p, c, begin, end, s, at, pa_find_pair(p, pa_seq(p, s), at, begin), [&](const PaItem& w, bool begins, bool ends, int64_t item_at, int sh, int tiles) {
       if (n == cap) return false;
       int* o = out + 16 * n++;
       const int f[16] = {c, begins, ends, w.tok0, w.n_tok, w.src, w.row0, w.slot, w.hk, w.j0, w.j1, w.kv_len, w.pos0,
                          w.out_mode, w.out_at, 0};
       for (int i = 0; i < 16; ++i) o[i] = f[i];
-      if (!begins && ends)   // the chain of its pieces: their number and a hash of their slots, in order
-        pa_pieces(share, item_at, sh, tiles, c, [&](int at) { o[15] = o[15] * 31 + at + 1; });
+      if (tiles > 0) o[15] = pa_first_cta(share, item_at) * 1000 + pa_last_cta(share, item_at, sh, tiles);
       return true;
     });
     if (!ok) return -1;

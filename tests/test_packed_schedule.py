@@ -86,14 +86,12 @@ def _check(lib, q, kv, hkv, tt, prefix, causal, ctas, layout="slots"):
         if len(ps) == 1:
             assert ps[0][6] == (ROWWISE if prefix else DIRECT)
         else:
-            # the chain that the joins follow: slot 1 of the first CTA, then slot 0 of the valid ones after it
+            # the chain that the joins follow: slot 1 of the first CTA, slot 0 of those behind it up to the last
             first, last = ps[0][0], ps[-1][0]
-            chain = [first * 2 + 1] + [c * 2 for c in range(first + 1, last + 1) if c * 2 in slots]
-            assert [p[7] for p in ps] == chain and all(p[6] == PIECE for p in ps)
-            h = 0
-            for at in chain:
-                h = (h * 31 + at + 1) & 0xffffffff
-            assert ps[-1][8] & 0xffffffff == h   # pa_pieces lists the same slots
+            assert [p[7] for p in ps] == [first * 2 + 1] + [c * 2 for c in range(first + 1, last + 1)]
+            assert all(p[6] == PIECE for p in ps)
+        if tiles:
+            assert all(p[8] == ps[0][0] * 1000 + ps[-1][0] for p in ps)   # pa_first_cta, pa_last_cta
     # a share's keys, padded to whole tiles item by item
     n_items = {c: sum(1 for ps in pieces.values() for p in ps if p[0] == c) for c in load}
     assert all(v <= share + 256 * (n_items[c] + 1) for c, v in load.items())
