@@ -1003,7 +1003,7 @@ static int packed_attention(const hokv_packed_args* a, void* stream) {
   HOKV_REQUIRE(a->q && a->out, "packed_attention: null pointer");
   HOKV_REQUIRE(a->cu_seqlens_q || a->n_tokens == a->n_seqs,
                "packed_attention: %lld tokens for %d sequences of one token", (long long)a->n_tokens, a->n_seqs);
-  HOKV_REQUIRE(a->kv_in_slots ? a->kv_len != nullptr : a->cu_seqlens_k != nullptr,
+  HOKV_REQUIRE(a->n_seqs == 0 || (a->kv_in_slots ? a->kv_len != nullptr : a->cu_seqlens_k != nullptr),
                "packed_attention: null key lengths");
   const int64_t rows_k = a->kv_in_slots ? a->kv_rows * a->n_seqs : a->kv_rows;
   HOKV_REQUIRE(rows_k == 0 || (a->k && a->v), "packed_attention: null pointer");
@@ -1172,7 +1172,7 @@ extern "C" int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* str
                a->n_freq, a->head_dim);
   HOKV_REQUIRE(a->eps >= 0.f && a->eps < INFINITY, "norm_rotate_append: eps %g", a->eps);
   if (a->n_tokens == 0) return HOKV_OK;
-  HOKV_REQUIRE(a->q && a->k && a->v && a->out && a->kv_len && (a->n_freq == 0 || a->inv_freq),
+  HOKV_REQUIRE(a->q && a->k && a->v && a->out && (a->kv_len || a->n_seqs == 0) && (a->n_freq == 0 || a->inv_freq),
                "norm_rotate_append: null pointer");
   HOKV_REQUIRE((a->k_slots && a->v_slots) || a->capacity == 0 || a->n_seqs == 0, "norm_rotate_append: null slots");
   HOKV_REQUIRE(a->cu_seqlens || a->n_tokens == a->n_seqs, "norm_rotate_append: %lld tokens for %d sequences of one token",

@@ -135,7 +135,9 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile
   return pa_try_wait(smem_u32(bar), parity) || pa_wait_more(smem_u32(bar), parity, abort_flag);
 }
 
-// The same for a mark in global memory.
+// The same for a mark in global memory, which another CTA sets: shares are
+// equal but a long call's CTAs may end some way apart.
+constexpr unsigned long long PA_MARK_NS = 10 * TC_WAIT_NS;
 __device__ __noinline__ bool pa_wait_ready(const unsigned long long* mark, unsigned long long token,
                                            volatile uint32_t* abort_flag) {
   const unsigned long long t0 = global_ns();
@@ -144,7 +146,7 @@ __device__ __noinline__ bool pa_wait_ready(const unsigned long long* mark, unsig
     asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(mark) : "memory");
     if (v == token) return true;
     if (*abort_flag) return false;
-    if (global_ns() - t0 > TC_WAIT_NS) {
+    if (global_ns() - t0 > PA_MARK_NS) {
       if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
       return false;
     }

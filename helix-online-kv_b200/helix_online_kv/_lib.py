@@ -202,32 +202,17 @@ def stream():
     return _vp(torch.cuda.current_stream().cuda_stream)
 
 
-def raw_stream(index: int) -> int:
-    """Address of the current stream of device `index` (what ``stream`` wraps, without a Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-class on_device:
-    """Makes device `index` current for a block; nothing to do when it already is."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def call_on(index: int, fn, args) -> int:
+    """fn(byref(args), current stream) with device `index` current; the status."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
 
 
 def signature(t):
     """What an argument check goes by: everything of a tensor but its data."""
-    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
+    return t.dtype, t.shape, t.stride(), t.get_device()
 
 
 class Checked(dict):

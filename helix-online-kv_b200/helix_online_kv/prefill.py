@@ -169,7 +169,7 @@ def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
         a.pv_stride_h, a.pv_stride_t = prefix_value.stride()[:2]
         a.prefix_len = prefix_key.shape[1]
     need = ctypes.c_size_t(0)
-    with L.on_device(dev.index):
+    with torch.cuda.device(dev):
         L.check(L.lib().hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), "packed_attention")
     return a, need.value
 
@@ -183,35 +183,35 @@ def _packed(what, query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
     if cu_seqlens_k is None and kv_len is None:
         cu_seqlens_k = cu_seqlens_q
     sig = L.signature
-    geometry = (sig(query), sig(key), sig(value), sig(cu_seqlens_q), sig(cu_seqlens_k), sig(kv_len), scaling, is_causal,
-                sig(out), sig(prefix_key), sig(prefix_value))
+    geometry = (sig(query), sig(key), sig(value), cu_seqlens_q is not None and sig(cu_seqlens_q),
+                cu_seqlens_k is not None and sig(cu_seqlens_k), kv_len is not None and sig(kv_len), scaling, is_causal,
+                out is not None and sig(out), prefix_key is not None and (sig(prefix_key), sig(prefix_value)))
     known = _checked.get(geometry)
     if known is None:
         known = _checked.keep(geometry, _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling,
                                                       is_causal, out, prefix_key, prefix_value))
-    device = geometry[0][3]
-    with L.on_device(device):
-        if out is None:
-            out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        if not query.numel():
-            return out
-        a = L.PackedArgs.from_buffer_copy(known[0])
-        ws = torch.empty(known[1], dtype=torch.uint8, device=query.device)
-        a.q, a.k, a.v, a.out, a.workspace, a.workspace_bytes = (query.data_ptr(), key.data_ptr(), value.data_ptr(),
-                                                                out.data_ptr(), ws.data_ptr(), known[1])
-        if prefix_key is not None:
-            a.prefix_k, a.prefix_v = prefix_key.data_ptr(), prefix_value.data_ptr()
-        if cu_seqlens_q is not None:
-            a.cu_seqlens_q = cu_seqlens_q.data_ptr()
-        if kv_len is not None:
-            a.kv_len = kv_len.data_ptr()
-        else:
-            a.cu_seqlens_k = cu_seqlens_k.data_ptr()
-        status = L.lib().hokv_packed_attention(ctypes.byref(a), L.raw_stream(device))
-        if status:
-            if status == L.ERR_INVALID:   # what the signatures do not show: addresses
-                raise ValueError(f"{what}: {L.lib().hokv_last_error().decode(errors='replace')}")
-            L.check(status, what)
+    args, need = known
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    if not args.n_tokens:
+        return out
+    a = L.PackedArgs.from_buffer_copy(args)
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    a.q, a.k, a.v, a.out, a.workspace, a.workspace_bytes = (query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                                                            out.data_ptr(), ws.data_ptr(), need)
+    if prefix_key is not None:
+        a.prefix_k, a.prefix_v = prefix_key.data_ptr(), prefix_value.data_ptr()
+    if cu_seqlens_q is not None:
+        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+    if kv_len is not None:
+        a.kv_len = kv_len.data_ptr()
+    else:
+        a.cu_seqlens_k = cu_seqlens_k.data_ptr()
+    status = L.call_on(geometry[0][3], L.lib().hokv_packed_attention, a)
+    if status:
+        if status == L.ERR_INVALID:   # what the signatures do not show: addresses
+            raise ValueError(f"{what}: {L.lib().hokv_last_error().decode(errors='replace')}")
+        L.check(status, what)
     return out
 
 

@@ -94,29 +94,29 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     even head dims up to 256.  ``out`` may be the query itself; rows behind the last sequence are zeros, or left
     as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
     sig = L.signature
-    geometry = (sig(query), sig(key), sig(value), sig(key_slots), sig(value_slots), sig(cu_seqlens), sig(kv_len),
-                sig(inv_freq), sig(q_weight), sig(k_weight), eps, interleaved, sig(positions), sig(out))
+    geometry = (sig(query), sig(key), sig(value), sig(key_slots), sig(value_slots), sig(kv_len), sig(inv_freq), eps,
+                interleaved, cu_seqlens is not None and sig(cu_seqlens), q_weight is not None and sig(q_weight),
+                k_weight is not None and sig(k_weight), positions is not None and sig(positions),
+                out is not None and sig(out))
     known = _checked.get(geometry)
     if known is None:
         known = _checked.keep(geometry, _check(query, key, value, key_slots, value_slots, cu_seqlens, kv_len, inv_freq,
                                                q_weight, k_weight, eps, interleaved, positions, out))
-    device = geometry[0][3]
-    with L.on_device(device):
-        if out is None:
-            out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        if not known.n_tokens:
-            return out
-        a = L.NormRotateArgs.from_buffer_copy(known)
-        a.q, a.k, a.v, a.out, a.k_slots, a.v_slots, a.kv_len, a.inv_freq = (
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(), key_slots.data_ptr(),
-            value_slots.data_ptr(), kv_len.data_ptr(), inv_freq.data_ptr())
-        if cu_seqlens is not None:
-            a.cu_seqlens = cu_seqlens.data_ptr()
-        if positions is not None:
-            a.positions = positions.data_ptr()
-        if q_weight is not None:
-            a.q_weight = q_weight.data_ptr()
-        if k_weight is not None:
-            a.k_weight = k_weight.data_ptr()
-        L.check(L.lib().hokv_norm_rotate_append(ctypes.byref(a), L.raw_stream(device)), "norm_rotate_append")
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    if not known.n_tokens:
+        return out
+    a = L.NormRotateArgs.from_buffer_copy(known)
+    a.q, a.k, a.v, a.out, a.k_slots, a.v_slots, a.kv_len, a.inv_freq = (
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr(), key_slots.data_ptr(), value_slots.data_ptr(),
+        kv_len.data_ptr(), inv_freq.data_ptr())
+    if cu_seqlens is not None:
+        a.cu_seqlens = cu_seqlens.data_ptr()
+    if positions is not None:
+        a.positions = positions.data_ptr()
+    if q_weight is not None:
+        a.q_weight = q_weight.data_ptr()
+    if k_weight is not None:
+        a.k_weight = k_weight.data_ptr()
+    L.check(L.call_on(geometry[0][3], L.lib().hokv_norm_rotate_append, a), "norm_rotate_append")
     return out

@@ -260,3 +260,91 @@ def test_shared_prefix_of_another_store_and_no_prefix():
     _verify(out, *reference(query, [1, 1], keys, values, 64 ** -0.5, True, (pk, pv)))
     none = shared_prefix_attention(query, pk[:, :0], pv[:, :0], k, v, kl)
     assert torch.equal(none, packed_attention(query, k, v, kv_len=kl))
+
+
+def test_no_sequences_and_no_keys():
+    """A batch of no sequences, tensors without rows: nothing to attend, zeros behind the last sequence."""
+    from helix_online_kv import _lib as L
+    from helix_online_kv.prefill import packed_attention
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    z = lambda *s: torch.zeros(s, dtype=F16, device="cuda")   # noqa: E731
+    query = torch.ones(3, 4, 64, dtype=F16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert (packed_attention(query, z(0, 2, 64), z(0, 2, 64), lens_tensor([]), lens_tensor([])) == 0).all()
+    assert (packed_attention(query, z(0, 2, 8, 64), z(0, 2, 8, 64), lens_tensor([]), kv_len=none) == 0).all()
+    assert (packed_attention(query, z(0, 2, 64), z(0, 2, 64), lens_tensor([1, 2]), lens_tensor([0, 0])) == 0).all()
+    assert (packed_attention(query, z(2, 2, 0, 64), z(2, 2, 0, 64), lens_tensor([1, 2]), kv_len=lens_tensor([0])) == 0).all()
+    # only the prefix to see
+    g = _gen(31)
+    pk, pv = _randn(g, 2, 200, 64, dtype=F16), _randn(g, 2, 200, 64, dtype=F16)
+    query = _randn(g, 3, 4, 64, dtype=F16)
+    out = shared_prefix_attention(query, pk, pv, z(0, 2, 64), z(0, 2, 64), cu_seqlens_q=lens_tensor([1, 2]),
+                                  cu_seqlens_k=lens_tensor([0, 0]))
+    empty = [torch.zeros(0, 2, 64, dtype=F16, device="cuda")] * 2
+    _verify(out, *reference(query, [1, 2], empty, empty, 64 ** -0.5, True, (pk, pv)))
+    torch.cuda.synchronize()
+    L.device_status()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (6, 2)])
+def test_outputs_in_any_layout(Hq, Hkv):
+    """out as a transposed view (heads outside tokens) and with rows off 32-byte boundaries."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(32)
+    q, D = [300, 5], 64
+    query, k, v = _randn(g, 305, Hq, D, dtype=BF16), _randn(g, 305, Hkv, D, dtype=BF16), _randn(g, 305, Hkv, D, dtype=BF16)
+    want = packed_attention(query, k, v, lens_tensor(q))
+    out = torch.full((Hq, 305, D), 3.0, dtype=BF16, device="cuda").transpose(0, 1)
+    assert torch.equal(packed_attention(query, k, v, lens_tensor(q), out=out), want)
+    wide = torch.full((305, Hq, D + 8), 3.0, dtype=BF16, device="cuda")
+    assert torch.equal(packed_attention(query, k, v, lens_tensor(q), out=wide[:, :, 8:]), want)
+    assert (wide[:, :, :8] == 3).all()
+    # values with strides of their own, and slots whose heads lie outside the batch
+    k4 = torch.empty(Hkv, 2, 320, D, dtype=BF16, device="cuda").fill_(float("nan")).transpose(0, 1)
+    v4 = torch.empty(2, 320, Hkv, D, dtype=BF16, device="cuda").fill_(float("nan")).transpose(1, 2)
+    for b, (a, n) in enumerate(((0, 300), (300, 5))):
+        k4[b, :, :n], v4[b, :, :n] = k[a:a + n].transpose(0, 1), v[a:a + n].transpose(0, 1)
+    assert torch.equal(packed_attention(query, k4, v4, lens_tensor(q), kv_len=torch.tensor(q, dtype=torch.int32, device="cuda")), want)
+
+
+def test_many_short_sequences_and_long_tables():
+    """More sequences than the schedule's lanes hold one each; items of one key tile share the slots in turn."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(33)
+    kv = [1 + (i * 37) % 190 for i in range(700)]
+    q = [0 if i % 13 == 5 else 1 + (i % 7 == 3) for i in range(700)]
+    q = [min(a, b) for a, b in zip(q, kv)]
+    query = _randn(g, sum(q), 4, 128, dtype=BF16)
+    k, v = _randn(g, sum(kv), 1, 128, dtype=BF16), _randn(g, sum(kv), 1, 128, dtype=BF16)
+    out = packed_attention(query, k, v, lens_tensor(q), lens_tensor(kv))
+    _verify(out, *reference(query, q, k.split(kv), v.split(kv), 128 ** -0.5))
+
+
+def test_one_and_two_tile_items_in_turn():
+    """Single tokens, prompts and short chunks one after the other: each CTA changes between the item forms."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(34)
+    q = [1, 65, 1, 1, 33, 200, 1, 32, 3, 64, 1, 97] * 12
+    kv = [n + (i * 113) % 700 for i, n in enumerate(q)]
+    for D, dtype in ((128, F16), (64, BF16)):
+        query = _randn(g, sum(q), 8, D, dtype=dtype)
+        k, v = _randn(g, sum(kv), 2, D, dtype=dtype), _randn(g, sum(kv), 2, D, dtype=dtype)
+        out = packed_attention(query, k, v, lens_tensor(q), lens_tensor(kv))
+        _verify(out, *reference(query, q, k.split(kv), v.split(kv), D ** -0.5))
+
+
+def test_non_finite_scores_propagate():
+    """A NaN or infinite score of a key that a row sees makes that row NaN, as the formula does, also where the running
+    maximum was taken before; other rows of the tile stay right."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(35)
+    for D in (64, 128):
+        query = _randn(g, 300, 2, D, dtype=BF16)
+        k, v = _randn(g, 300, 2, D, dtype=BF16), _randn(g, 300, 2, D, dtype=BF16)
+        clean = packed_attention(query, k, v, lens_tensor([300]))
+        k2 = k.clone()
+        k2[250, 0, 3] = float("nan")
+        k2[270, 1] = float("inf")
+        out = packed_attention(query, k2, v, lens_tensor([300]))
+        assert torch.equal(out[:250, 0], clean[:250, 0]) and out[250:, 0].isnan().all()
+        assert torch.equal(out[:270, 1], clean[:270, 1]) and out[270:, 1].isnan().all()

@@ -221,3 +221,11 @@ def test_model_step_in_one_graph():
         ref, tol = reference(query, [1, 1], [st.k[0, b, :, :n].transpose(0, 1) for b, n in enumerate(held)],
                              [st.v[0, b, :, :n].transpose(0, 1) for b, n in enumerate(held)], D ** -0.5)
         assert ((out.double() - ref).abs() <= tol).all()
+
+
+def test_no_sequences():
+    from helix_online_kv.rotary import norm_rotate_append
+    x = torch.ones(3, 2, 64, dtype=F16, device="cuda")
+    ks = torch.zeros(0, 2, 8, 64, dtype=F16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert (norm_rotate_append(x, x, x, ks, ks, lens_tensor([]), none, _freqs(32)) == 0).all()
