@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "helix-online-kv_b200", "csrc")
 OUT = os.path.join(HERE, "native", "_build", "libhokv_schedule_host.so")
 DIRECT, PIECE, ROWWISE = 0, 1, 2
-ITEM, MIN_SHARE = 448, 704
+ITEM, MIN_SHARE, WHOLE = 448, 704, 1472
 
 
 @pytest.fixture(scope="module")
@@ -90,11 +90,13 @@ def _check(lib, q, kv, hkv, tt, prefix, causal, ctas, layout="slots"):
             first, last = ps[0][0], ps[-1][0]
             assert [p[7] for p in ps] == [first * 2 + 1] + [c * 2 for c in range(first + 1, last + 1)]
             assert all(p[6] == PIECE for p in ps)
-        if tiles:
+        units_of = ITEM + (2 if m > tt else 1) * keys
+        assert len(ps) == 1 or units_of > WHOLE
+        if tiles and units_of > WHOLE:
             assert all(p[8] == ps[0][0] * 1000 + ps[-1][0] for p in ps)   # pa_first_cta, pa_last_cta
     # a share's keys, padded to whole tiles item by item
     n_items = {c: sum(1 for ps in pieces.values() for p in ps if p[0] == c) for c in load}
-    assert all(v <= share + 256 * (n_items[c] + 1) for c, v in load.items())
+    assert all(v <= share + WHOLE + 256 * (n_items[c] + 1) for c, v in load.items())
 
 
 @pytest.mark.parametrize("ctas", [1, 7, 148])
