@@ -1189,6 +1189,7 @@ extern "C" int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* str
   p.n_seqs = a->n_seqs; p.T = (int)a->n_tokens; p.Hq = a->q_heads; p.Hkv = a->kv_heads; p.D = a->head_dim;
   p.n_freq = a->n_freq; p.interleaved = a->interleaved ? 1 : 0; p.zero_tail = a->zero_tail ? 1 : 0;
   p.eps = a->eps;
+  p.inv_dim = 1.f / (float)p.D;
   // 16-byte rows and whole 8-element chunks of both halves: the vector form
   const int e16 = a->dtype == HOKV_F32 ? 4 : 8;
   bool vec = p.D % 16 == 0 && (p.interleaved || p.n_freq % 8 == 0);

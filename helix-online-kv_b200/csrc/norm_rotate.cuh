@@ -29,12 +29,12 @@ struct NraP {
   int64_t cap;
   int n_seqs, T, Hq, Hkv, D, n_freq, interleaved, zero_tail;
   int tokens;   // tokens of a block
-  float eps;
+  float eps, inv_dim;   // inv_dim: 1 / D
 };
 
 constexpr int NRA_THREADS = 256;
-// 4 blocks of an SM (64 registers).  A 16K-token prompt of 32 + 2 x 8 heads of 128 dims, bf16 (403 MB): 80 us, 5.0 TB/s;
-// 88 with 5 blocks (48 registers, spills), 84 to 110 with 2 to 4 rows of a group on their way and 4 to 2 blocks, 103 with
+// 4 blocks of an SM (64 registers).  A 16K-token prompt of 32 + 2 x 8 heads of 128 dims, bf16 (403 MB): 79 us, 5.1 TB/s;
+// 82 with 5 blocks (48 registers, spills), 84 to 110 with 2 to 4 rows of a group on their way and 4 to 2 blocks, 103 with
 // a token's angles formed by each group that works on it; the same reads and writes without the arithmetic take 69.
 constexpr int NRA_BLOCKS = 4;
 constexpr int NRA_TOKENS = 8;   // most tokens of a block
@@ -90,6 +90,13 @@ __device__ __forceinline__ void nra_angle(int pos, float f, float& c, float& s) 
   const double turns = (double)pos * (double)f * 0.15915494309189533577;   // 1 / (2 pi)
   const float frac = (float)(turns - rint(turns));
   sincospif(2.f * frac, &s, &c);
+}
+
+// Two pairs (a, b) turned by their angles: packed fp32.
+__device__ __forceinline__ void turn2(float& a0, float& a1, float& b0, float& b1, float2 c, float2 s) {
+  const float2 a = make_float2(a0, a1), b = make_float2(b0, b1);
+  const float2 x = __ffma2_rn(b, make_float2(-s.x, -s.y), __fmul2_rn(a, c)), y = __ffma2_rn(a, s, __fmul2_rn(b, c));
+  a0 = x.x; a1 = x.y; b0 = y.x; b1 = y.y;
 }
 
 template <typename T>
@@ -161,7 +168,7 @@ template <typename T, int LPR>
 __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const NraP p) {
   constexpr int GROUPS = NRA_THREADS / LPR;
   __shared__ NraTok s_tok[NRA_TOKENS];
-  __shared__ __align__(16) float2 s_cs[NRA_TOKENS][128 + 8];   // cos, sin
+  __shared__ __align__(16) float s_cos[NRA_TOKENS][128 + 8], s_sin[NRA_TOKENS][128 + 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = threadIdx.x % LPR;
   const int t0 = (int)blockIdx.x * p.tokens, n_tok = min(p.tokens, p.T - t0);
   const int heads = p.Hq + 2 * p.Hkv;
@@ -188,9 +195,7 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
   __syncthreads();
   for (int e = threadIdx.x; e < n_tok * p.n_freq; e += NRA_THREADS) {
     const int k = e / p.n_freq, f = e - k * p.n_freq;
-    float2 cs;
-    nra_angle(s_tok[k].pos, p.inv_freq[f], cs.x, cs.y);
-    s_cs[k][f] = cs;
+    nra_angle(s_tok[k].pos, p.inv_freq[f], s_cos[k][f], s_sin[k][f]);
   }
   __syncthreads();
   const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
         }
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float q = rsqrtf(ss / (float)p.D + p.eps);
+        const float q = rsqrtf(ss * p.inv_dim + p.eps);
         if (on) {
           Vec8<T> wa, wb;
           nra_weight8(w + ca * 8, wa);
@@ -233,30 +238,27 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
           }
         }
       }
-      const float2* cs = &s_cs[k][8 * l];
+      const float *cos = &s_cos[k][8 * l], *sin = &s_sin[k][8 * l];
       if (p.interleaved) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (8 * l + j < p.n_freq) {
             const float x = a[2 * j], y = a[2 * j + 1];
-            a[2 * j] = x * cs[j].x - y * cs[j].y;
-            a[2 * j + 1] = y * cs[j].x + x * cs[j].y;
+            a[2 * j] = x * cos[j] - y * sin[j];
+            a[2 * j + 1] = y * cos[j] + x * sin[j];
           }
           if (8 * l + 4 + j < p.n_freq) {
             const float x = b[2 * j], y = b[2 * j + 1];
-            b[2 * j] = x * cs[j + 4].x - y * cs[j + 4].y;
-            b[2 * j + 1] = y * cs[j + 4].x + x * cs[j + 4].y;
+            b[2 * j] = x * cos[j + 4] - y * sin[j + 4];
+            b[2 * j + 1] = y * cos[j + 4] + x * sin[j + 4];
           }
         }
       } else if (l < lr) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          const float4 c = *reinterpret_cast<const float4*>(cs + j);
-          const float x0 = a[j], y0 = b[j], x1 = a[j + 1], y1 = b[j + 1];
-          a[j] = x0 * c.x - y0 * c.y;
-          b[j] = y0 * c.x + x0 * c.y;
-          a[j + 1] = x1 * c.z - y1 * c.w;
-          b[j + 1] = y1 * c.z + x1 * c.w;
+        for (int j = 0; j < 8; j += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(cos + j), d = *reinterpret_cast<const float4*>(sin + j);
+          turn2(a[j], a[j + 1], b[j], b[j + 1], make_float2(c.x, c.y), make_float2(d.x, d.y));
+          turn2(a[j + 2], a[j + 3], b[j + 2], b[j + 3], make_float2(c.z, c.w), make_float2(d.z, d.w));
         }
       }
       if (kind == 0 && tok.b < 0) {
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(NRA_THREADS) k_norm_rotate_scalar(const NraP p
   if (kind < 2 && w) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    r = rsqrtf(ss / (float)p.D + p.eps);
+    r = rsqrtf(ss * p.inv_dim + p.eps);
   }
   if (kind == 0 ? tok.b < 0 && !p.zero_tail : !tok.keep) return;
 #pragma unroll
