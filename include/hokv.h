@@ -228,8 +228,9 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
  * fp32 sums; the softmax weights are rounded to the input type before the
  * second product.  Non-finite keys or values that a causal mask hides from a
  * query may still reach it when they share its 128-key tile.  Results are the
- * same on every run (no atomics).  Calls that overlap on the GPU need
- * workspaces of their own. */
+ * same on every run (no atomics on them).  The workspace needs no
+ * initialisation; calls that overlap on the GPU need workspaces of their
+ * own. */
 typedef struct hokv_packed_args {
   int dtype, n_seqs, q_heads, kv_heads, head_dim, causal, kv_in_slots, zero_tail;
   float scale;

@@ -348,3 +348,84 @@ def test_non_finite_scores_propagate():
         out = packed_attention(query, k2, v, lens_tensor([300]))
         assert torch.equal(out[:250, 0], clean[:250, 0]) and out[250:, 0].isnan().all()
         assert torch.equal(out[:270, 1], clean[:270, 1]) and out[270:, 1].isnan().all()
+
+
+def test_shared_prefix_in_a_graph_and_on_two_streams():
+    """Both launches captured and replayed with other lengths; eager calls on two streams at once."""
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(41)
+    Hq, Hkv, D, P = 8, 2, 128, 3000
+    k, v, kl = _slots(g, [700, 90, 1], Hkv, D, BF16, 2100, stale=0.25)
+    pk, pv = _randn(g, Hkv, P, D, dtype=BF16), _randn(g, Hkv, P, D, dtype=BF16)
+    query, cu = _randn(g, 6, Hq, D, dtype=BF16), lens_tensor([2, 3, 1])
+    call = lambda: shared_prefix_attention(query, pk, pv, k, v, kl, cu)   # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for q, kv in (([2, 3, 1], [700, 90, 1]), ([1, 1, 4], [5, 2000, 130]), ([6, 0, 0], [6, 0, 40])):
+        cu.copy_(lens_tensor(q))
+        kl.copy_(torch.tensor(kv, dtype=torch.int32))
+        query.copy_(_randn(g, 6, Hq, D, dtype=BF16))
+        graph.replay()
+        _verify(out, *reference(query, q, [k[b, :, :n].transpose(0, 1) for b, n in enumerate(kv)],
+                                [v[b, :, :n].transpose(0, 1) for b, n in enumerate(kv)], D ** -0.5, True, (pk, pv)))
+    alone = call()
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, alone) for o in outs)
+
+
+def test_two_graphs_and_replays_of_cut_items():
+    """Two captured calls whose items are cut between CTAs, replayed in turn many times: every replay starts from
+    clean marks of its own workspace."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(42)
+    k, v, kl = _slots(g, [9000, 12000], 2, 64, F16)
+    q1, q2 = _randn(g, 2, 8, 64, dtype=F16), _randn(g, 2, 8, 64, dtype=F16)
+    w1, w2 = packed_attention(q1, k, v, kv_len=kl), packed_attention(q2, k, v, kv_len=kl)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in (q1, q2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(packed_attention(q, k, v, kv_len=kl))
+    for _ in range(20):
+        for graph, o in zip(graphs, outs):
+            o.zero_()
+            graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], w1) and torch.equal(outs[1], w2)
+
+
+def test_workspace_contents_do_not_matter():
+    """The C entry point on a workspace full of ones, NaN patterns, and what the call before left there."""
+    import ctypes
+
+    from helix_online_kv import _lib as L
+    from helix_online_kv import prefill as F
+    g = _gen(43)
+    k, v, kl = _slots(g, [9000, 40, 3000], 2, 128, BF16)
+    query = _randn(g, 3, 8, 128, dtype=BF16)
+    want = F.packed_attention(query, k, v, kv_len=kl)
+    args, need = F._packed_check(query, k, v, None, None, kl, None, True, None, None, None)
+    a = L.PackedArgs.from_buffer_copy(args)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(query)
+    a.q, a.k, a.v, a.out, a.kv_len = query.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), kl.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    for fill in (1, 255, None, None):
+        if fill is not None:
+            ws.fill_(fill)
+        out.zero_()
+        L.check(L.lib().hokv_packed_attention(ctypes.byref(a), L.stream()))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    a.workspace_bytes = need - 1
+    assert L.lib().hokv_packed_attention(ctypes.byref(a), L.stream()) == L.ERR_WORKSPACE
