@@ -429,3 +429,47 @@ def test_workspace_contents_do_not_matter():
         assert torch.equal(out, want)
     a.workspace_bytes = need - 1
     assert L.lib().hokv_packed_attention(ctypes.byref(a), L.stream()) == L.ERR_WORKSPACE
+
+
+def test_bad_lengths_behind_a_prefix():
+    """A slot longer than its capacity, starts outside the batch: reported, without waiting; later calls are unharmed."""
+    import time
+
+    from helix_online_kv import _lib as L
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(44)
+    k, v, kl = _slots(g, [50, 60, 70], 2, 64, F16, cap=80)
+    pk, pv = _randn(g, 2, 300, 64, dtype=F16), _randn(g, 2, 300, 64, dtype=F16)
+    query, cu = _randn(g, 6, 4, 64, dtype=F16), lens_tensor([2, 2, 2])
+    good = shared_prefix_attention(query, pk, pv, k, v, kl, cu)
+    torch.cuda.synchronize()
+    kl[1] = 81
+    out = shared_prefix_attention(query, pk, pv, k, v, kl, cu)
+    with pytest.raises(L.HokvError) as e:
+        L.device_status()
+    assert e.value.status == L.ERR_DEVICE_INPUT
+    assert torch.equal(out[:2], good[:2]) and torch.equal(out[4:], good[4:])
+    kl[1] = 60
+    cu[1] = 9
+    t = time.time()
+    shared_prefix_attention(query, pk, pv, k, v, kl, cu)
+    with pytest.raises(L.HokvError) as e:
+        L.device_status()
+    assert e.value.status == L.ERR_DEVICE_INPUT and time.time() - t < 1
+    cu.copy_(lens_tensor([2, 2, 2]))
+    assert torch.equal(shared_prefix_attention(query, pk, pv, k, v, kl, cu), good)
+
+
+def test_many_pairs_behind_a_prefix():
+    """Many whole and cut prefix items a CTA: 300 sequences of up to three tokens behind prefixes of 40 and 2,000."""
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(45)
+    q = [1 + i % 3 for i in range(300)]
+    kv = [max(n, (i * 61) % 400) for i, n in enumerate(q)]
+    kv[7], q[7] = 9000, 3   # one own part cut over CTAs
+    query = _randn(g, sum(q), 8, 64, dtype=F16)
+    k, v = _randn(g, sum(kv), 2, 64, dtype=F16), _randn(g, sum(kv), 2, 64, dtype=F16)
+    for P in (40, 2000):
+        pk, pv = _randn(g, 2, P, 64, dtype=F16), _randn(g, 2, P, 64, dtype=F16)
+        out = shared_prefix_attention(query, pk, pv, k, v, cu_seqlens_q=lens_tensor(q), cu_seqlens_k=lens_tensor(kv))
+        _verify(out, *reference(query, q, k.split(kv), v.split(kv), 64 ** -0.5, True, (pk, pv)))
