@@ -965,6 +965,12 @@ static int pa_check(const hokv_packed_args* a) {
 template <int D, typename T>
 static int launch_packed(const PaMaps& maps, const PaP& p, cudaStream_t st) {
   if (int e = ensure_smem(k_packed_attn<D, T>, PaGeo<D>::SMEM)) return e;
+  // its warps share out the registers it was launched with: a build with fewer would wait for more for good
+  static const int regs = [] {
+    cudaFuncAttributes a = {};
+    return cudaFuncGetAttributes(&a, k_packed_attn<D, T>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != PA_REGS) return fail(HOKV_ERR_CUDA, "k_packed_attn: built with %d registers a thread, not %d", regs, PA_REGS);
   k_packed_attn<D, T><<<p.n_ctas, PA_THREADS, PaGeo<D>::SMEM, st>>>(maps, p);
   if (int e = check_launch("k_packed_attn")) return e;
   if (p.prefix == 0) return HOKV_OK;

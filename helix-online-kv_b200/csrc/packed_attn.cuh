@@ -62,6 +62,11 @@ namespace hokv {
 
 constexpr int PA_THREADS = 384;
 constexpr int PA_ROWS = 128;        // rows of a tile
+// Registers of a thread: 168 at launch, then 200 for the 8 softmax warps, which hold a row of 128 scores, and 104 for
+// the other 4.  The sum may not pass what the block was launched with, or the raise would wait for good: the launch
+// checks the build's count.  (208 and 88: 1 % slower, 192 and 120: 0.5 %, both with more spills.)
+constexpr int PA_REGS = 168, PA_REGS_ROW = 200, PA_REGS_ISSUE = 104;
+static_assert(256 * PA_REGS_ROW + 128 * PA_REGS_ISSUE <= PA_THREADS * PA_REGS, "register split");
 constexpr int PA_QUEUE = 8;         // item descriptors in flight
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
@@ -70,8 +75,7 @@ struct PaGeo {
   static constexpr int NB = D / 64;                       // 64-dim column blocks
   // Tensor memory: S of the slots in columns 0 and 128, O in 256 and 384; P in 64 columns of its own behind a 64-dim
   // O, over S otherwise.
-  static constexpr bool OWN_P = D == 64;
-  static constexpr int P0 = OWN_P ? 256 + 64 : 0;
+  static constexpr int P0 = D == 64 ? 256 + 64 : 0;
   static constexpr int Q_BYTES = PA_ROWS * D * 2;         // one query tile
   static constexpr int KV_BYTES = PA_BN * D * 2;          // one K or V tile
   static constexpr int STAGES = D == 64 ? 8 : 4;          // ring of K and V tiles
@@ -127,9 +131,8 @@ __device__ __forceinline__ bool pa_try_wait(uint32_t bar, unsigned parity) {
 }
 
 // Bounded wait of every calling thread; the first that gives up marks the CTA
-// aborted, and every other wait of the CTA then ends too.  The part behind the
-// first try is a call: it stands in many places and is short of time in none.
-__device__ __noinline__ bool pa_wait_more(uint32_t bar, unsigned parity, volatile uint32_t* abort_flag) {
+// aborted, and every other wait of the CTA then ends too.
+__device__ __forceinline__ bool pa_wait_more(uint32_t bar, unsigned parity, volatile uint32_t* abort_flag) {
   const unsigned long long t0 = global_ns();
   while (!pa_try_wait(bar, parity)) {
     if (*abort_flag) return false;
@@ -147,8 +150,8 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile
 // The same for a mark in global memory, which another CTA sets: shares are
 // equal but a long call's CTAs may end some way apart.
 constexpr unsigned long long PA_MARK_NS = 10 * TC_WAIT_NS;
-__device__ __noinline__ bool pa_wait_ready(const unsigned long long* mark, unsigned long long token,
-                                           volatile uint32_t* abort_flag) {
+__device__ __forceinline__ bool pa_wait_ready(const unsigned long long* mark, unsigned long long token,
+                                              volatile uint32_t* abort_flag) {
   const unsigned long long t0 = global_ns();
   while (true) {
     unsigned long long v;
@@ -322,6 +325,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   const int TT = p.TT, G = p.G;
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_ROW));
     // ---- softmax of tile slot sl, one row per thread ----------------------------
     const int sl = warp >> 2, row = tid & 127;
     const int row_tok = row / G, row_g = row - row_tok * G;
@@ -363,77 +367,50 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         s_ph ^= 1;
         tc_fence_after();
         if (warp_ok) {
-          // Two passes over the row, 32 columns at a time with the next 32 on their way: the maximum, then the weights
-          // (short loops: the roles share one instruction cache).  Where P has columns of its own (head dims up to 64),
-          // an item's later tiles go without the first pass: the weights are formed with the running maximum as it
-          // stands and the tile's own maximum beside them, and again in the rare case that it rises by more than 8.
+          // The row stays in registers between its maximum and its weights, which a pass of its own from tensor memory
+          // for each would cost 4 to 8 % of (16K prompt 1,862 -> 1,772 us, 4 x 4,096 tokens of 64 dims 797 -> 726).
           const bool masked = wlim < PA_BN;
-          const float2 s2 = make_float2(p.sl2, p.sl2);
-          float va[32], vb[32];
+          float v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, v[c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_wait_ld32(v[c]);
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mask32(v[c], lim - c * 32);
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[c][j], v[c][j + 1]);
+          }
+          const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
+          const bool grow = !(mt <= m_run + 8.f);     // also for NaN, and for the first key a row sees
+          if (i > 0 && __any_sync(0xffffffffu, grow)) {
+            // O was last written by this slot's previous P V, complete before this S
+            const float f = grow ? pf_ex2(m_run - mt) : 1.f;
+            l_run *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
+            tmem_wait_st();
+          }
+          if (grow) m_run = mt + (mt - mt);           // an infinite maximum gives NaN, as inf - inf does
+          const float nm = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
           float2 acc[2];
-          float mx[4];
-          auto max32 = [&](const float (&v)[32]) __attribute__((always_inline)) {
+          acc[0] = acc[1] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[j], v[j + 1]);
-          };
-          auto above = [&](float& mt) __attribute__((always_inline)) {   // also for NaN, and for the first key a row sees
-            mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
-            return !(mt <= m_run + 8.f);
-          };
-          for (bool known = !PG::OWN_P || i == 0;; known = true) {
-            float mt;
-            tmem_ld32_nw(s_addr, va);
-            mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
-            if (known) {
-#pragma unroll 1
-              for (int c = 0; c < PA_BN; c += 64) {
-                tmem_wait_ld32(va);
-                tmem_ld32_nw(s_addr + c + 32, vb);
-                if (masked) mask32(va, lim - c);
-                max32(va);
-                tmem_wait_ld32(vb);
-                tmem_ld32_nw(s_addr + (c + 64) % PA_BN, va);   // behind the last columns: the first again
-                if (masked) mask32(vb, lim - c - 32);
-                max32(vb);
-              }
-              const bool grow = above(mt);
-              if (i > 0 && __any_sync(0xffffffffu, grow)) {
-                // O was last written by this slot's previous P V, complete before this S
-                const float f = grow ? pf_ex2(m_run - mt) : 1.f;
-                l_run *= f;
-#pragma unroll 1
-                for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
-                tmem_wait_st();
-              }
-              if (grow) m_run = mt + (mt - mt);         // an infinite maximum gives NaN, as inf - inf does
-            }
-            const float nm = m_run == -INFINITY ? 0.f : -m_run;
-            const float2 n2 = make_float2(nm, nm);
-            acc[0] = acc[1] = make_float2(0.f, 0.f);
-            auto exp32 = [&](const float (&v)[32], uint32_t at) __attribute__((always_inline)) {
-              uint32_t pk[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float2 a = __ffma2_rn(make_float2(v[2 * j], v[2 * j + 1]), s2, n2);
-                const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
-                acc[j & 1] = __fadd2_rn(acc[j & 1], e);
-                pk[j] = pack2<T>(e.x, e.y);
-              }
-              if (PG::OWN_P) max32(v);
-              tmem_st16_nw(at, pk);   // columns of their own, or of S that were read before
-            };
-#pragma unroll 1
-            for (int c = 0; c < PA_BN; c += 64) {
-              tmem_wait_ld32(va);
-              tmem_ld32_nw(s_addr + c + 32, vb);
-              if (masked) mask32(va, lim - c);
-              exp32(va, p_addr + c / 2);
-              tmem_wait_ld32(vb);
-              if (c + 64 < PA_BN) tmem_ld32_nw(s_addr + c + 64, va);
-              if (masked) mask32(vb, lim - c - 32);
-              exp32(vb, p_addr + c / 2 + 16);
+            for (int j = 0; j < 16; ++j) {
+              const float2 a = __ffma2_rn(make_float2(v[c][2 * j], v[c][2 * j + 1]), s2, n2);
+              const float2 e = make_float2(pf_ex2(a.x), pf_ex2(a.y));
+              acc[j & 1] = __fadd2_rn(acc[j & 1], e);
+              pk[j] = pack2<T>(e.x, e.y);
             }
-            if (!PG::OWN_P || known || !__any_sync(0xffffffffu, above(mt))) break;
+            tmem_st16_nw(p_addr + c * 16, pk);   // columns of their own, or of S that were read before
           }
           acc[0] = __fadd2_rn(acc[0], acc[1]);
           l_run += acc[0].x + acc[0].y;
@@ -636,6 +613,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       }
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_ISSUE));
     auto all = [&](bool x) { return (bool)__all_sync(0xffffffffu, x); };
     // Positions c at the next task on slot sl; false when there is none: at the end of the stream (c.done), or when
     // the next item begins on slot 0 and this is slot 1.  `release`: this cursor is its warp's last reader.

@@ -16,13 +16,11 @@
 
 namespace hokv {
 
-// Loops are kept rolled and the shared arithmetic is a call on the device: the
-// roles of the kernel share one instruction cache.
+// Loops are kept rolled on the device: the roles of the kernel share one
+// instruction cache.
 #if defined(__CUDACC__)
-#define HD_CALL __host__ __device__ __noinline__
 #define ROLLED _Pragma("unroll 1")
 #else
-#define HD_CALL inline
 #define ROLLED
 #endif
 
@@ -115,7 +113,7 @@ HD int pa_keys(const PaSeq& s, int W, int pr) {
 
 // Units, of one KV head, of the first n pairs (none of them the last) of nq
 // tokens against kv keys.
-HD_CALL int64_t pa_units_before(int kv, int nq, int causal, int W, int n) {
+HD int64_t pa_units_before(int kv, int nq, int causal, int W, int n) {
   int64_t keys = (int64_t)n * kv;
   if (causal) {
     const int64_t off = (int64_t)kv - nq;
