@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "helix-online-kv_b200", "csrc")
 OUT = os.path.join(HERE, "native", "_build", "libhokv_schedule_host.so")
 DIRECT, PIECE, ROWWISE = 0, 1, 2
-ITEM, MIN_SHARE, WHOLE = 448, 704, 1472
+ITEM, MIN_SHARE, WHOLE = 512, 768, 1536
 
 
 @pytest.fixture(scope="module")
