@@ -48,8 +48,8 @@
 //
 // What bounds it (B200, 32 query / 8 KV heads of 128 dims, bf16): prompts by a
 // slot's chain of scores, softmax and products, 3,300 cycles a two-tile step
-// against 2,048 of products, and at 16K tokens by the board's power (1.96 ms =
-// 1,120 TFLOP/s cool, 1,010 at the 1,000 W cap); single tokens by memory (8 at
+// against 2,048 of products, and at 16K tokens by the board's power (1.71 ms =
+// 1,285 TFLOP/s cool, 1,107 at the 1,000 W cap); single tokens by memory (8 at
 // 16K keys: 92 us, 5.8 TB/s of K and V); short calls by latency, 4.5 us to the
 // first scores.  Rolled loops and one copy of each role's code are deliberate:
 // with unrolled roles (20 KB more) the instruction cache missed 20 % of its
@@ -64,7 +64,7 @@ constexpr int PA_THREADS = 384;
 constexpr int PA_ROWS = 128;        // rows of a tile
 // Registers of a thread: 168 at launch, then 200 for the 8 softmax warps, which hold a row of 128 scores, and 104 for
 // the other 4.  The sum may not pass what the block was launched with, or the raise would wait for good: the launch
-// checks the build's count.  (208 and 88: 1 % slower, 192 and 120: 0.5 %, both with more spills.)
+// checks the build's count.  (208 and 88: 1 to 3 % slower, 192 and 120: 0.5 %.)
 constexpr int PA_REGS = 168, PA_REGS_ROW = 200, PA_REGS_ISSUE = 104;
 static_assert(256 * PA_REGS_ROW + 128 * PA_REGS_ISSUE <= PA_THREADS * PA_REGS, "register split");
 constexpr int PA_QUEUE = 8;         // item descriptors in flight
@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         s_ph ^= 1;
         tc_fence_after();
         if (warp_ok) {
-          // The row stays in registers between its maximum and its weights, which a pass of its own from tensor memory
-          // for each would cost 4 to 8 % of (16K prompt 1,862 -> 1,772 us, 4 x 4,096 tokens of 64 dims 797 -> 726).
+          // The row stays in registers between its maximum and its weights (a pass from tensor memory for each: 16K
+          // prompt 1,862 us against 1,772, 4 x 4,096 tokens of 64 dims 797 against 726).
           const bool masked = wlim < PA_BN;
           float v[4][32];
 #pragma unroll
