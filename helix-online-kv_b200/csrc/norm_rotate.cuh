@@ -33,9 +33,10 @@ struct NraP {
 };
 
 constexpr int NRA_THREADS = 256;
-// 4 blocks of an SM (64 registers).  A 16K-token prompt of 32 + 2 x 8 heads of 128 dims, bf16 (403 MB): 79 us, 5.1 TB/s;
+// 4 blocks of an SM (64 registers).  A 16K-token prompt of 32 + 2 x 8 heads of 128 dims, bf16 (403 MB): 78 us, 5.2 TB/s;
 // 82 with 5 blocks (48 registers, spills), 84 to 110 with 2 to 4 rows of a group on their way and 4 to 2 blocks, 103 with
 // a token's angles formed by each group that works on it; the same reads and writes without the arithmetic take 69.
+// With addresses multiplied out for each row 79, and 4,196 tokens of 3 sequences 27.6 instead of 25.3.
 constexpr int NRA_BLOCKS = 4;
 constexpr int NRA_TOKENS = 8;   // most tokens of a block
 
@@ -97,6 +98,13 @@ __device__ __forceinline__ void turn2(float& a0, float& a1, float& b0, float& b1
   const float2 a = make_float2(a0, a1), b = make_float2(b0, b1);
   const float2 x = __ffma2_rn(b, make_float2(-s.x, -s.y), __fmul2_rn(a, c)), y = __ffma2_rn(a, s, __fmul2_rn(b, c));
   a0 = x.x; a1 = x.y; b0 = y.x; b1 = y.y;
+}
+
+// Two elements times their weights and the row's factor.
+template <typename T>
+__device__ __forceinline__ void scale2(float& x, float& y, T wx, T wy, float q) {
+  const float2 r = __fmul2_rn(make_float2(x, y), __fmul2_rn(make_float2((float)wx, (float)wy), make_float2(q, q)));
+  x = r.x; y = r.y;
 }
 
 template <typename T>
@@ -162,12 +170,15 @@ __device__ __forceinline__ int nra_target(const NraP& p, int t, int h, const Nra
 
 // Vector form: D a multiple of 16, and of the rotated dims too unless
 // interleaved.  A block takes p.tokens tokens with all their head rows: their
-// slots and angles once, through shared memory, then rows by groups of LPR
-// lanes, the next row on its way while one is worked on.
+// slots, row addresses and angles once, through shared memory, then rows by
+// groups of LPR lanes, the next row on its way while one is worked on.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const NraP p) {
   constexpr int GROUPS = NRA_THREADS / LPR;
   __shared__ NraTok s_tok[NRA_TOKENS];
+  __shared__ T* s_dst[NRA_TOKENS][3];          // the token's rows: of q, k and v
+  __shared__ const T* s_src[NRA_TOKENS][3];
+  __shared__ int64_t s_step[2][3];             // head strides: source, destination
   __shared__ __align__(16) float s_cos[NRA_TOKENS][128 + 8], s_sin[NRA_TOKENS][128 + 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = threadIdx.x % LPR;
   const int t0 = (int)blockIdx.x * p.tokens, n_tok = min(p.tokens, p.T - t0);
@@ -177,20 +188,34 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
   const bool on = l < p.D / 16;
   const int ca = l < lr ? l : 2 * lr + 2 * (l - lr), cb = l < lr ? l + lr : ca + 1;
   Raw8<T> next[2];
-  int fk = 0, fh = threadIdx.x / LPR;   // the next row to fetch: token and head
-  auto fetch = [&](Raw8<T> (&x)[2]) __attribute__((always_inline)) {
+  int fk = 0, fh = threadIdx.x / LPR, kind = 0, head = 0;   // the next row: token, head row; kind and head of its own
+  auto locate = [&]() __attribute__((always_inline)) {
     while (fh >= heads) fh -= heads, ++fk;
-    if (on && fk < n_tok) {
-      const T* src = nra_source<T>(p, t0 + fk, fh);
-      nra_load8(src + ca * 8, x[0]);
-      nra_load8(src + cb * 8, x[1]);
-    }
-    fh += GROUPS;
+    kind = (fh >= p.Hq) + (fh >= p.Hq + p.Hkv);
+    head = fh - (kind > 0 ? p.Hq : 0) - (kind > 1 ? p.Hkv : 0);
   };
-  fetch(next);
+  locate();
+  if (on && fk < n_tok) {
+    const T* src = nra_source<T>(p, t0 + fk, fh);
+    nra_load8(src + ca * 8, next[0]);
+    nra_load8(src + cb * 8, next[1]);
+  }
   if (warp < n_tok) {
     const NraTok k = nra_token(p, t0 + warp);
-    if (lane == 0) s_tok[warp] = k;
+    const int64_t t = t0 + warp;
+    if (lane == 0) {
+      s_tok[warp] = k;
+      s_src[warp][0] = reinterpret_cast<const T*>(p.q) + t * p.q_t;
+      s_src[warp][1] = reinterpret_cast<const T*>(p.k) + t * p.k_t;
+      s_src[warp][2] = reinterpret_cast<const T*>(p.v) + t * p.v_t;
+      s_dst[warp][0] = reinterpret_cast<T*>(p.out) + t * p.out_t;
+      s_dst[warp][1] = reinterpret_cast<T*>(p.ks) + (k.keep ? k.b * p.ks_b + k.row * p.ks_t : 0);
+      s_dst[warp][2] = reinterpret_cast<T*>(p.vs) + (k.keep ? k.b * p.vs_b + k.row * p.vs_t : 0);
+    }
+  }
+  if (threadIdx.x == 0) {
+    s_step[0][0] = p.q_h; s_step[0][1] = p.k_h; s_step[0][2] = p.v_h;
+    s_step[1][0] = p.out_h; s_step[1][1] = p.ks_h; s_step[1][2] = p.vs_h;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < n_tok * p.n_freq; e += NRA_THREADS) {
@@ -199,27 +224,33 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
   }
   __syncthreads();
   const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane / LPR * LPR);
-  int k = 0, h = threadIdx.x / LPR;
 #pragma unroll 1
-  while (true) {
-    while (h >= heads) h -= heads, ++k;
-    if (k >= n_tok) break;
+  while (fk < n_tok) {
     float a[8], b[8];
     nra_widen(next[0], a);
     nra_widen(next[1], b);
-    fetch(next);
+    const int k = fk, row_kind = kind;
     const NraTok tok = s_tok[k];
-    T* dst;
-    const int kind = nra_target<T>(p, t0 + k, h, tok, dst);
-    h += GROUPS;
-    if (kind < 2) {
-      const T* w = reinterpret_cast<const T*>(kind == 0 ? p.qw : p.kw);
+    T* dst = s_dst[k][kind] + head * s_step[1][kind];
+    fh += GROUPS;
+    locate();
+    if (on && fk < n_tok) {
+      const T* src = s_src[fk][kind] + head * s_step[0][kind];
+      nra_load8(src + ca * 8, next[0]);
+      nra_load8(src + cb * 8, next[1]);
+    }
+    if (row_kind < 2) {
+      const T* w = reinterpret_cast<const T*>(row_kind == 0 ? p.qw : p.kw);
       if (w) {   // uniform over the group: its lanes share the row
         float ss = 0.f;
         if (on) {
-          float2 s2 = make_float2(0.f, 0.f);
+          float2 s2 = make_float2(0.f, 0.f), r2 = s2;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s2 = __ffma2_rn(make_float2(a[j], b[j]), make_float2(a[j], b[j]), s2);
+          for (int j = 0; j < 8; j += 2) {
+            s2 = __ffma2_rn(make_float2(a[j], a[j + 1]), make_float2(a[j], a[j + 1]), s2);
+            r2 = __ffma2_rn(make_float2(b[j], b[j + 1]), make_float2(b[j], b[j + 1]), r2);
+          }
+          s2 = __fadd2_rn(s2, r2);
           ss = s2.x + s2.y;
         }
 #pragma unroll
@@ -230,11 +261,9 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
           nra_weight8(w + ca * 8, wa);
           nra_weight8(w + cb * 8, wb);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 y = __fmul2_rn(make_float2(a[j], b[j]),
-                                        __fmul2_rn(make_float2((float)wa.x[j], (float)wb.x[j]), make_float2(q, q)));
-            a[j] = y.x;
-            b[j] = y.y;
+          for (int j = 0; j < 8; j += 2) {
+            scale2(a[j], a[j + 1], wa.x[j], wa.x[j + 1], q);
+            scale2(b[j], b[j + 1], wb.x[j], wb.x[j + 1], q);
           }
         }
       }
@@ -261,12 +290,12 @@ __global__ void __launch_bounds__(NRA_THREADS, NRA_BLOCKS) k_norm_rotate(const N
           turn2(a[j + 2], a[j + 3], b[j + 2], b[j + 3], make_float2(c.z, c.w), make_float2(d.z, d.w));
         }
       }
-      if (kind == 0 && tok.b < 0) {
+      if (row_kind == 0 && tok.b < 0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
       }
     }
-    if (on && (kind == 0 ? tok.b >= 0 || p.zero_tail : tok.keep)) {
+    if (on && (row_kind == 0 ? tok.b >= 0 || p.zero_tail : tok.keep)) {
       nra_store8(dst + ca * 8, a);
       nra_store8(dst + cb * 8, b);
     }
