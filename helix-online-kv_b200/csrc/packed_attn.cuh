@@ -15,7 +15,7 @@
 // Work split.  Lengths live on the device only; every CTA derives the same
 // schedule from them (packed_schedule.cuh): the work of all items forms one
 // line that the CTAs, one per SM, cut into equal shares.  An item cut by a
-// share's border leaves pieces (running maximum, sum and unnormalised output,
+// share's border leaves pieces (reference point, sum and unnormalised output,
 // fp32) in the workspace.  A CTA takes the item that earlier CTAs began last,
 // and the one that holds an item's last piece joins all of them in CTA order:
 // no atomics on results, the same result each run.  It waits for marks of
@@ -36,10 +36,15 @@
 //   P = 2^(S scale log2 e - m)   one thread per row, rounded to the input
 //                type, in tensor memory (64 columns)
 //   O += P V     tcgen05.mma with P as the tensor-memory A operand
-// The running maximum m is raised only when it grows by more than 8 (log2
-// units): P stays below 2^8, and normalising by the same m is exact.  P is
-// rounded to the input type because the tensor cores multiply in it (half a
-// step of that type relative to each weight); sums, maxima and O are fp32.
+// The reference point m is raised only when a score passes it by more than a
+// step (log2 units), and normalising by the same m is exact.  P is rounded to
+// the input type because the tensor cores multiply in it: half a step of that
+// type relative to each weight.  bf16 has the range of fp32: m is the running
+// maximum, raised by steps above 8.  f16 is subnormal below 2^-14, and a row with
+// one dominant key may have most of its mass in thousands of weights that small:
+// m lies 11 below the running maximum and is raised by steps above 4 (P up to
+// 2^15), so a weight keeps its half step down to 2^-25 of the largest, and one
+// below that is off by 2^-36 of the largest at most.  Sums, maxima and O are fp32.
 //
 // Rows behind a sequence's end: their scores are masked by selection (any bit
 // pattern, NaN included, drops out), and the V rows of the last, partial
@@ -93,7 +98,7 @@ struct PaP : PaSched {
   int Hq, G, D, zero_tail, tma_out;   // tma_out: tokens of a warp's 32 rows, 0 when they are not whole tokens
   float sl2;                     // scale * log2(e)
   int k_t, k_h, k_b, v_t, v_h, v_b, pk_t, pk_h, pk_b, pv_t, pv_h, pv_b;   // coordinate slots of the maps
-  float2* ml;                    // [n_ctas][2][256] (running maximum, sum)
+  float2* ml;                    // [n_ctas][2][256] (m, sum)
   float4* o;                     // [n_ctas][2][D / 4][256]
   unsigned long long* ready;     // [n_ctas][2][8] the call's token when 32 rows of a piece are written, then 0 again
   unsigned long long token;      // this call's
@@ -232,15 +237,15 @@ __device__ __forceinline__ void mask32(float (&v)[32], int left) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
 }
-// Scale 8 fp32 columns of this thread's lane.
-__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
+// x f + a for 8 fp32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_fma8(uint32_t taddr, float f, float a) {
   uint32_t r[8];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
   tmem_wait_ld();
 #pragma unroll
-  for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+  for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(fmaf(__uint_as_float(r[j]), f, a));
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
@@ -252,6 +257,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));   // NaN wins
   return d;
 }
+
+// Where a row's reference point m lies below its largest score, and how far a score may pass m before m is raised.
+template <typename T>
+struct PaRange {
+  static constexpr bool NARROW = std::is_same<T, __half>::value;   // weights may leave the type's range
+  static constexpr float LIFT = NARROW ? 11.f : 0.f, MOST = NARROW ? 15.f : 8.f;
+  // From here on fp32 holds m too coarsely for f16 weights (off by a quarter at 2^22): scores are taken relative to the
+  // one that set m before they are scaled.
+  static constexpr float FAR = 0x1p22f;
+};
 
 // One 32-byte store (a whole sector): a thread's row of O.
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t* u) {
@@ -265,6 +280,7 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t* u) {
 template <int D, typename T>
 __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_constant__ PaMaps maps, const PaP p) {
   using PG = PaGeo<D>;
+  using PR = PaRange<T>;
   constexpr int ST = PG::STAGES;
   constexpr int BF = std::is_same<T, __half>::value ? 0 : 1;
   extern __shared__ __align__(1024) unsigned char pa_smem[];
@@ -336,6 +352,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     const uint32_t p_addr = tmem + lane_sel + (uint32_t)(PG::P0 + sl * 128);
     // rows of out on 32-byte boundaries and in whole 16-element steps: 32-byte stores
     const bool wide = p.D % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) % 32 | (uint64_t)(p.ost % 16) | (uint64_t)(p.osh % 16)) == 0;
+    const float raw_step = (PR::MOST - PR::LIFT - 0x1p-8f) / p.sl2;   // of a score as it stands in S
     unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
     int u = 0;   // tasks of the items so far
     bool ok = true;
@@ -361,7 +378,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         __syncwarp();
         if (lane == 0) pa_arrive(&it_empty[qi]);
       };
-      float m_run = -INFINITY, l_run = 0.f;
+      float m_run = -INFINITY, l_run = 0.f, nm = 0.f;        // nm: what is added to a scaled score
+      float raw_most = -INFINITY, m_raw = 0.f;               // f16: scores above this raise m; what is taken from scores
+      bool any_far = false;                                  // in the warp
       for (int i = 0; i < mine; ++i, lim -= step, wlim -= step) {
         if (!pa_wait(&s_full[sl], s_ph, abort_flag)) { ok = false; break; }
         s_ph ^= 1;
@@ -371,32 +390,56 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
           // prompt 1,862 us against 1,772, 4 x 4,096 tokens of 64 dims 797 against 726).
           const bool masked = wlim < PA_BN;
           float v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, v[c]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_wait_ld32(v[c]);
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mask32(v[c], lim - c * 32);
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[c][j], v[c][j + 1]);
-          }
-          const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.sl2;
-          const bool grow = !(mt <= m_run + 8.f);     // also for NaN, and for the first key a row sees
-          if (i > 0 && __any_sync(0xffffffffu, grow)) {
-            // O was last written by this slot's previous P V, complete before this S
-            const float f = grow ? pf_ex2(m_run - mt) : 1.f;
-            l_run *= f;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 8) tmem_scale8(o_addr + c, f);   // rare: few registers
+          for (bool moved = false;; moved = true) {   // once, but for scores that fp32 holds too coarsely
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32_nw(s_addr + c * 32, v[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_wait_ld32(v[c]);
+            if (masked) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mask32(v[c], lim - c * 32);
+            }
+            if (PR::NARROW && moved) break;
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) mx[j >> 1 & 3] = max3(mx[j >> 1 & 3], v[c][j], v[c][j + 1]);
+            }
+            const float raw = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), mt = raw * p.sl2;
+            // also for NaN, and for the first key a row sees
+            const bool grow = PR::NARROW ? !(raw <= raw_most) : !(mt <= m_run + PR::MOST);
+            if (i == 0 || __any_sync(0xffffffffu, grow)) {
+              const float m_new = PR::NARROW ? fmaf(raw, p.sl2, -PR::LIFT) : mt;
+              if (i > 0) {
+                // O was last written by this slot's previous P V, complete before this S
+                const float f = grow ? pf_ex2(m_run - m_new) : 1.f;
+                l_run *= f;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 8) tmem_fma8(o_addr + c, f, 0.f);   // rare: few registers
+                tmem_wait_st();
+              }
+              if (grow) {
+                m_run = m_new + (mt - mt);            // an infinite maximum gives NaN, as inf - inf does
+                if constexpr (PR::NARROW) {
+                  m_raw = raw;
+                  raw_most = __fadd_rd(raw, raw_step);
+                }
+              }
+              nm = m_run == -INFINITY ? 0.f : -m_run;
+              if constexpr (PR::NARROW) {
+                const bool far = m_run != -INFINITY && fabsf(m_run) >= PR::FAR;
+                if (far) nm = PR::LIFT;
+                else m_raw = 0.f;
+                any_far = __any_sync(0xffffffffu, far);
+              }
+            }
+            if (!PR::NARROW || !any_far) break;
+#pragma unroll 1
+            for (int c = 0; c < PA_BN; c += 8) tmem_fma8(s_addr + c, 1.f, -m_raw);   // P is not written yet
             tmem_wait_st();
           }
-          if (grow) m_run = mt + (mt - mt);           // an infinite maximum gives NaN, as inf - inf does
-          const float nm = m_run == -INFINITY ? 0.f : -m_run;
           const float2 s2 = make_float2(p.sl2, p.sl2), n2 = make_float2(nm, nm);
           float2 acc[2];
           acc[0] = acc[1] = make_float2(0.f, 0.f);

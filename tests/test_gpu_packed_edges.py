@@ -1,0 +1,114 @@
+"""packed_attention and shared_prefix_attention where a mistake hides from random
+data: keys far below a row's largest score, scores of any finite size."""
+
+import math
+
+import pytest
+import torch
+
+from packed_reference import lens_tensor, reference
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _check(out, ref, tol):
+    from helix_online_kv import _lib as L
+    torch.cuda.synchronize()
+    L.device_status()
+    err = (out.double() - ref).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (int(bad.sum()), float(err.max()), float((err / tol).max()), bad.nonzero()[:3].tolist())
+
+
+def _far_tail(g, n, Hkv, D, gap, sinks, dtype):
+    """Keys [n, H_kv, D] whose dim 0 holds the score in log2 units for a query with 1 there and scaling ln 2: `gap` for
+    the keys in `sinks`, 0 for the others, whose weights then all round the same way; values 0 for the sinks, 0.5 to 1.5
+    for the others."""
+    k = torch.zeros(n, Hkv, D, device="cuda")
+    v = torch.rand((n, Hkv, D), generator=g, device="cuda") + 0.5
+    k[sinks, :, 0], v[sinks] = gap, 0.0
+    return k.to(dtype), v.to(dtype)
+
+
+def _tail_tolerance(tol, dtype, values):
+    """Weights that the type holds below its normal range are off by up to half its smallest step, 2^-25 in f16, where a
+    row's largest weight is stored as 2^11 at least: 2^-36 sum |V| of the result (bf16 has the range of fp32)."""
+    if dtype == BF16:
+        return tol
+    return tol + 2.0 ** -36 * float(sum(v.double().abs().sum(0).max() for v in values))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q,kv,gap,sink", [
+    ([1], [131072], 25.125, 0),      # one token over every CTA: a tail of 2^-25 each holds a thousandth of the mass
+    ([1], [131072], 25.125, 131071),
+    ([1], [16384], 17.5, 9000),
+    ([1, 2], [1000, 900], 20.25, 5),  # whole items of one tile
+    ([300], [300], 19.25, 0),        # two-tile items; rows that see few keys and many
+    ([2048], [2048], 22.25, 0),
+])
+def test_keys_far_below_the_largest_score(q, kv, gap, sink, dtype):
+    """A key that dominates its row (an attention sink) takes none of the others' values away."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(sum(kv))
+    Hq, Hkv, D = 8, 2, 64
+    sinks, at = [], 0
+    for n in kv:
+        sinks.append(at + min(sink, n - 1))
+        at += n
+    k, v = _far_tail(g, sum(kv), Hkv, D, gap, sinks, dtype)
+    query = torch.zeros(sum(q), Hq, D, dtype=dtype, device="cuda")
+    query[..., 0] = 1
+    out = packed_attention(query, k, v, lens_tensor(q), lens_tensor(kv), scaling=math.log(2.0))
+    keys, values = k.split(kv), v.split(kv)
+    ref, tol = reference(query, q, keys, values, math.log(2.0))
+    _check(out, ref, _tail_tolerance(tol, dtype, values))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("P,sink", [(20000, 0), (20000, None), (700, 0)])
+def test_keys_far_below_the_largest_score_behind_a_prefix(P, sink, dtype):
+    """The same over the join of a prefix with own keys: the dominating key in the prefix, or among the own keys."""
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(P)
+    Hq, Hkv, D, kv, q = 8, 2, 64, [3000, 40], [1, 3]
+    pk, pv = _far_tail(g, P, Hkv, D, 21.25, [] if sink is None else [sink], dtype)
+    k, v = _far_tail(g, sum(kv), Hkv, D, 21.25, [7, 3001] if sink is None else [], dtype)
+    query = torch.zeros(sum(q), Hq, D, dtype=dtype, device="cuda")
+    query[..., 0] = 1
+    pk, pv = pk.transpose(0, 1), pv.transpose(0, 1)
+    out = shared_prefix_attention(query, pk, pv, k, v, cu_seqlens_q=lens_tensor(q), cu_seqlens_k=lens_tensor(kv),
+                                  scaling=math.log(2.0))
+    keys, values = k.split(kv), v.split(kv)
+    ref, tol = reference(query, q, keys, values, math.log(2.0), True, (pk, pv))
+    _check(out, ref, _tail_tolerance(tol, dtype, [pv.transpose(0, 1), *values]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rising", [False, True])
+def test_scores_of_any_finite_size(dtype, rising):
+    """Scores of 2^28, whose differences are far above the rounding of an fp32 score: each row is the value of its
+    largest key, but for the rounding of that key's weight and of the output (half a step each), and of a few fp32
+    products."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(9)
+    n, D = 900, 64
+    query = torch.zeros(n, 4, D, dtype=dtype, device="cuda")
+    query[..., 0] = 8192.0
+    rank = torch.arange(n, device="cuda") if rising else torch.randperm(n, generator=g, device="cuda")
+    k = torch.zeros(n, 2, D, dtype=dtype, device="cuda")
+    # 8 significant bits: 128 keys of one binade each; 8192 times the least step is 2^13
+    k[..., 0] = torch.ldexp(1 + (rank % 128) / 128, (rank // 128) + 8)[:, None].to(dtype)
+    v = torch.randn((n, 2, D), generator=g, device="cuda").to(dtype)
+    top = torch.stack([rank[:i + 1].argmax() for i in range(n)])
+    out = packed_attention(query, k, v, lens_tensor([n]), scaling=1.0)
+    ref = v[top].repeat_interleave(2, 1).double()
+    fi = torch.finfo(dtype)
+    _check(out, ref, ref.abs() * (fi.eps + 2.0 ** -20) + fi.smallest_normal * fi.eps)
