@@ -135,7 +135,7 @@ def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
         _lengths(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
     elif T != B:
         raise ValueError(f"without cu_seqlens_q every sequence has one query: got {T} queries for {B} sequences")
-    scale = float(scaling) if scaling is not None else D ** -0.5
+    scale = scaling if scaling is not None else D ** -0.5
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"Expected a positive finite scaling, got {scaling}")
     prefix = (("prefix_key", prefix_key), ("prefix_value", prefix_value)) if prefix_key is not None else ()
@@ -154,7 +154,7 @@ def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
                             or (out.numel() and (out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8))):
         raise ValueError(f"Expected out [{T}, {Hq}, {D}] {query.dtype} on {dev} with contiguous rows and strides in "
                          f"multiples of 8 elements, got {tuple(out.shape)} {out.dtype} on {out.device}")
-    a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim, a.causal = _DTYPES[query.dtype], B, Hq, Hkv, D, bool(is_causal)
+    a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim, a.causal = _DTYPES[query.dtype], B, Hq, Hkv, D, is_causal
     a.scale, a.n_tokens, a.zero_tail = scale, T, out is None
     a.q_stride_t, a.q_stride_h = query.stride(0), query.stride(1)
     a.out_stride_t, a.out_stride_h = (Hq * D, D) if out is None else out.stride()[:2]
@@ -182,6 +182,8 @@ def _packed(what, query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
     """Check, take the output and this call's workspace from the allocator, launch on the current stream."""
     if cu_seqlens_k is None and kv_len is None:
         cu_seqlens_k = cu_seqlens_q
+    # values, not objects: a tensor would be found again by its identity after it has changed
+    scaling, is_causal = None if scaling is None else float(scaling), bool(is_causal)
     sig = L.signature
     geometry = (sig(query), sig(key), sig(value), cu_seqlens_q is not None and sig(cu_seqlens_q),
                 cu_seqlens_k is not None and sig(cu_seqlens_k), kv_len is not None and sig(kv_len), scaling, is_causal,

@@ -63,7 +63,7 @@ def _check(query, key, value, key_slots, value_slots, cu_seqlens, kv_len, inv_fr
         raise ValueError(f"Expected a finite eps >= 0, got {eps}")
     a = L.NormRotateArgs()
     a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim = _DTYPES[dt], B, Hq, Hkv, D
-    a.n_freq, a.interleaved, a.zero_tail, a.eps, a.n_tokens = inv_freq.shape[0], bool(interleaved), out is None, eps, T
+    a.n_freq, a.interleaved, a.zero_tail, a.eps, a.n_tokens = inv_freq.shape[0], interleaved, out is None, eps, T
     a.q_stride_t, a.q_stride_h = query.stride()[:2]
     a.k_stride_t, a.k_stride_h = key.stride()[:2]
     a.v_stride_t, a.v_stride_h = value.stride()[:2]
@@ -93,6 +93,7 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     inv_freq[f]; the dims behind 2F keep their values.  f16, bf16 or f32, the same for all but lengths and inv_freq;
     even head dims up to 256.  ``out`` may be the query itself; rows behind the last sequence are zeros, or left
     as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
+    eps, interleaved = float(eps), bool(interleaved)   # values, not objects: a tensor may change behind its identity
     sig = L.signature
     geometry = (sig(query), sig(key), sig(value), sig(key_slots), sig(value_slots), sig(kv_len), sig(inv_freq), eps,
                 interleaved, cu_seqlens is not None and sig(cu_seqlens), q_weight is not None and sig(q_weight),

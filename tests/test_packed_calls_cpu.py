@@ -1,0 +1,55 @@
+"""What the packed-batch entry points keep between calls and refuse, without a
+GPU: the argument checks are stubbed, nothing is launched."""
+
+import pytest
+import torch
+
+from helix_online_kv import _lib as L
+from helix_online_kv import prefill as F
+from helix_online_kv import rotary as R
+from helix_online_kv.shared_prefix import shared_prefix_attention
+
+
+class _Nothing:
+    """A checked call that has no tokens: the entry point returns before any launch."""
+
+    n_tokens = 0
+
+
+@pytest.mark.parametrize("kind", ["packed", "prefix"])
+def test_a_scaling_changed_in_place_is_read_again(monkeypatch, kind):
+    seen = []
+    monkeypatch.setattr(F, "_checked", L.Checked())
+    monkeypatch.setattr(F, "_packed_check", lambda *a: seen.append(a[6]) or (_Nothing, 0))
+    q, cu, scale = torch.zeros(2, 2, 64), torch.zeros(3, dtype=torch.int32), torch.tensor(0.5)
+
+    def call(s):
+        if kind == "packed":
+            return F.packed_attention(q, q, q, cu, scaling=s)
+        return shared_prefix_attention(q, q, q, q, q, cu_seqlens_q=cu, scaling=s)
+
+    call(scale)
+    scale.fill_(2.0)
+    call(scale)
+    assert seen == [0.5, 2.0] and all(type(s) is float for s in seen)
+    call(2.0)
+    call(torch.tensor(2.0))
+    assert len(seen) == 2   # the same value is the same geometry
+    with pytest.raises((TypeError, ValueError)):
+        call("much")
+    with pytest.raises((TypeError, ValueError, RuntimeError)):
+        call(torch.ones(2))
+    assert all(not isinstance(x, torch.Tensor) for key in F._checked for x in key)
+
+
+def test_an_eps_changed_in_place_is_read_again(monkeypatch):
+    seen = []
+    monkeypatch.setattr(R, "_checked", L.Checked())
+    monkeypatch.setattr(R, "_check", lambda *a: seen.append(a[10]) or _Nothing)
+    q, n, eps = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32), torch.tensor(0.5)
+    call = lambda e: R.norm_rotate_append(q, q, q, q, q, None, n, q, eps=e)   # noqa: E731
+    call(eps)
+    eps.fill_(2.0)
+    call(eps)
+    assert seen == [0.5, 2.0] and all(type(e) is float for e in seen)
+    assert all(not isinstance(x, torch.Tensor) for key in R._checked for x in key)
