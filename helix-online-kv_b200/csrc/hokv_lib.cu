@@ -1162,6 +1162,17 @@ static int launch_norm_rotate(NraP p, bool vec, cudaStream_t st) {
 
 }  // namespace hokv
 
+extern "C" int hokv_hold(int what) {
+#ifdef HOKV_HOLD
+  const cudaError_t e = cudaMemcpyToSymbol(hokv::g_hold, &what, sizeof(int));
+  if (e != cudaSuccess) return hokv::fail(HOKV_ERR_CUDA, "hold: %s", cudaGetErrorString(e));
+  return HOKV_OK;
+#else
+  (void)what;
+  return hokv::fail(HOKV_ERR_UNSUPPORTED, "hold: this library was built without -DHOKV_HOLD");
+#endif
+}
+
 extern "C" int hokv_norm_rotate_append(const hokv_norm_rotate_args* a, void* stream) {
   HOKV_REQUIRE(a, "norm_rotate_append: null arguments");
   HOKV_REQUIRE(a->dtype == HOKV_F16 || a->dtype == HOKV_BF16 || a->dtype == HOKV_F32, "norm_rotate_append: dtype %d",

@@ -121,6 +121,20 @@ struct PaCursor {
   bool done = false;
 };
 
+// ---- signals kept back (instrumented build only) --------------------------------
+// Built with -DHOKV_HOLD, hokv_hold() makes CTAs 3, 11, 19, ... keep back signals that other roles or CTAs wait for,
+// and shortens the packed attention's waits, so that a test sees them run out.  The product build compiles none of it.
+enum { PA_HOLD_MARK = 1, PA_HOLD_P = 2, PA_HOLD_STOP = 4 };   // a piece's marks; the first warp's weights; the stream's end
+#ifdef HOKV_HOLD
+__device__ int g_hold = 0;
+__device__ __forceinline__ int pa_hold() { return *reinterpret_cast<volatile int*>(&g_hold); }
+__device__ __forceinline__ bool pa_held(int what) { return (pa_hold() & what) && blockIdx.x % 8 == 3; }
+__device__ __forceinline__ unsigned long long pa_limit(unsigned long long ns) { return pa_hold() ? ns / 50 : ns; }
+#else
+__device__ __forceinline__ constexpr bool pa_held(int) { return false; }
+__device__ __forceinline__ constexpr unsigned long long pa_limit(unsigned long long ns) { return ns; }
+#endif
+
 // ---- barriers ----------------------------------------------------------------
 
 __device__ __forceinline__ bool pa_try_wait(uint32_t bar, unsigned parity) {
@@ -141,7 +155,7 @@ __device__ __forceinline__ bool pa_wait_more(uint32_t bar, unsigned parity, vola
   const unsigned long long t0 = global_ns();
   while (!pa_try_wait(bar, parity)) {
     if (*abort_flag) return false;
-    if (global_ns() - t0 > TC_WAIT_NS) {
+    if (global_ns() - t0 > pa_limit(TC_WAIT_NS)) {
       if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
       return false;
     }
@@ -151,6 +165,10 @@ __device__ __forceinline__ bool pa_wait_more(uint32_t bar, unsigned parity, vola
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
   return pa_try_wait(smem_u32(bar), parity) || pa_wait_more(smem_u32(bar), parity, abort_flag);
 }
+// The whole warp's wait: near the limit its lanes may see different ends, and all of them go on or none does.
+__device__ __forceinline__ bool pa_wait_warp(uint64_t* bar, unsigned parity, volatile uint32_t* abort_flag) {
+  return __all_sync(0xffffffffu, pa_wait(bar, parity, abort_flag));
+}
 
 // The same for a mark in global memory, which another CTA sets: shares are
 // equal but a long call's CTAs may end some way apart.
@@ -159,11 +177,11 @@ __device__ __forceinline__ bool pa_wait_ready(const unsigned long long* mark, un
                                               volatile uint32_t* abort_flag) {
   const unsigned long long t0 = global_ns();
   while (true) {
+    if (*abort_flag) return false;
     unsigned long long v;
     asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(mark) : "memory");
     if (v == token) return true;
-    if (*abort_flag) return false;
-    if (global_ns() - t0 > PA_MARK_NS) {
+    if (global_ns() - t0 > pa_limit(PA_MARK_NS)) {
       if (atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u) dev_flag(HOKV_ERR_TIMEOUT);
       return false;
     }
@@ -299,7 +317,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   uint64_t* it_empty = it_full + PA_QUEUE; // [PA_QUEUE] 2 load + MMA + 8 softmax warps
   uint64_t* kv_full = it_empty + PA_QUEUE; // [ST] TMA bytes
   uint64_t* kv_empty = kv_full + ST;       // [ST] MMA commit
-  static_assert(13 + 2 * PA_QUEUE + 2 * ST <= 48, "barriers");
+  uint64_t* mma_done = kv_empty + ST;      // MMA commit at the end of a CTA that gave up
+  static_assert(14 + 2 * PA_QUEUE + 2 * ST <= 48, "barriers");
   uint32_t* ctl = reinterpret_cast<uint32_t*>(bars + 48);                   // [0] tmem base, [1] abort
   PaItem* queue = reinterpret_cast<PaItem*>(bars + 49);                     // [PA_QUEUE]
   float2* s_ml = reinterpret_cast<float2*>(bars + 49 + PA_QUEUE * sizeof(PaItem) / 8);   // [128] slot 1's (m, l)
@@ -314,6 +333,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   }
   if (tid == 0) {
     mbar_init(ml_full, 4);
+    mbar_init(mma_done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -358,7 +378,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const int qi = it % PA_QUEUE;
-      if (!pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag)) break;
+      ok = pa_wait_warp(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag);
+      if (!ok) break;
       const volatile PaItem& w = queue[qi];   // read again where needed: registers are short in the loop
       if (w.out_mode == PA_STOP) break;
       const bool two = w.n_tok > TT;
@@ -382,7 +403,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       float raw_most = -INFINITY, m_raw = 0.f;               // f16: scores above this raise m; what is taken from scores
       bool any_far = false;                                  // in the warp
       for (int i = 0; i < mine; ++i, lim -= step, wlim -= step) {
-        if (!pa_wait(&s_full[sl], s_ph, abort_flag)) { ok = false; break; }
+        // no vote here (1 % of a prompt): a CTA that gave up runs through the item on what is there, and drops it at its end
+        (void)pa_wait(&s_full[sl], s_ph, abort_flag);
+        __syncwarp();
         s_ph ^= 1;
         tc_fence_after();
         if (warp_ok) {
@@ -461,16 +484,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) pa_arrive(&p_full[sl]);
+        if (lane == 0 && !(warp == 0 && pa_held(PA_HOLD_P))) pa_arrive(&p_full[sl]);
       }
-      if (!ok) break;
       // ---- epilogue: O of this slot (slot 0 joins both parts of a one-tile item) ------
       if (sl == 0 && other) o1_ph ^= 1;   // slot 1 completes a phase too
       if (mine == 0) {
         item_done();
         continue;
       }
-      if (!pa_wait(&o_full[sl], o_ph, abort_flag)) break;
+      ok = __all_sync(0xffffffffu, pa_wait(&o_full[sl], o_ph, abort_flag) && !*abort_flag);
+      if (!ok) break;
       o_ph ^= 1;
       tc_fence_after();
       if (join && sl == 1) {
@@ -482,7 +505,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       }
       float f0 = 1.f, f1 = 0.f;
       if (join) {
-        if (!pa_wait(&o_full[1], o1_ph ^ 1, abort_flag) || !pa_wait(ml_full, ml_ph, abort_flag)) break;
+        ok = pa_wait_warp(&o_full[1], o1_ph ^ 1, abort_flag) && pa_wait_warp(ml_full, ml_ph, abort_flag);
+        if (!ok) break;
         ml_ph ^= 1;
         tc_fence_after();
         const float2 b = s_ml[row];
@@ -578,7 +602,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (join) pa_arrive(&o_empty[1]);
         if (out_mode == PA_PIECE && p.prefix == 0) {   // these rows of the piece are written
           __threadfence();
-          store_release(&p.ready[(int64_t)out_at * 8 + (prow >> 5)], p.token);
+          if (!pa_held(PA_HOLD_MARK)) store_release(&p.ready[(int64_t)out_at * 8 + (prow >> 5)], p.token);
         }
       }
       item_done();
@@ -665,7 +689,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       if (c.done) return false;
       if (c.j == c.tasks) {
         const int qi = c.it % PA_QUEUE;
-        ok = all(pa_wait(&it_full[qi], (unsigned)((c.it / PA_QUEUE) & 1), abort_flag));
+        ok = pa_wait_warp(&it_full[qi], (unsigned)((c.it / PA_QUEUE) & 1), abort_flag);
         if (!ok) return false;
         ++c.it;
         const PaItem& w = queue[qi];
@@ -701,7 +725,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (!next_task(c, sl, ok, is_v, true)) return;
         const int j = c.j++;
         if (c.two && (j & 1)) return;
-        ok = all(pa_wait(&kv_empty[stage], stage_ph, abort_flag));
+        ok = pa_wait_warp(&kv_empty[stage], stage_ph, abort_flag);
         if (!ok) return;
         const CUtensorMap* m = c.src ? (is_v ? &maps.pv : &maps.pk) : (is_v ? &maps.v : &maps.k);
         const int at_t = c.src ? (is_v ? p.pv_t : p.pk_t) : (is_v ? p.v_t : p.k_t);
@@ -725,10 +749,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (i >= 0) step(cv, i & 1, true);
         if (ok) step(ck, i & 1, false);
       }
-      if (*abort_flag) {   // gave up: the copies in flight land before the CTA ends
+      // the copies in flight land before the CTA ends, whoever gave up on them
 #pragma unroll 1
-        for (unsigned k = loads > ST ? loads - ST : 0; k < loads; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
-      }
+      for (unsigned k = loads > ST ? loads - ST : 0; k < loads; ++k) (void)mbar_wait(&kv_full[k % ST], (k / ST) & 1);
     } else if (warp == 9) {
       // ---- MMA issue --------------------------------------------------------------
       const int kd = (p.D + 15) / 16;
@@ -743,7 +766,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       // the next tile of the ring, once its bytes have landed
       auto next_tile = [&]() __attribute__((always_inline)) {
         const unsigned st = stage;
-        ok = all(pa_wait(&kv_full[st], stage_ph, abort_flag));
+        ok = pa_wait_warp(&kv_full[st], stage_ph, abort_flag);
         if (++stage == ST) stage = 0, stage_ph ^= 1;
         return st;
       };
@@ -874,7 +897,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       bool ok = true;
       for (int it = 0; ok; ++it) {
         const int qi = it % PA_QUEUE;
-        ok = all(pa_wait(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag));
+        ok = pa_wait_warp(&it_full[qi], (unsigned)((it / PA_QUEUE) & 1), abort_flag);
         if (!ok) break;
         const int mode = uniform(queue[qi].out_mode), two = uniform(queue[qi].n_tok > TT), hk = uniform(queue[qi].hk),
                   tok0 = uniform(queue[qi].tok0);
@@ -884,7 +907,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
 #pragma unroll 1
         for (int t = 0; t < (two ? 2 : 1); ++t) {
           const int buf = two ? t : qb;
-          ok = all(pa_wait(&q_empty[buf], q_ph >> buf & 1, abort_flag));   // passes at once the first time
+          ok = pa_wait_warp(&q_empty[buf], q_ph >> buf & 1, abort_flag);   // passes at once the first time
           if (!ok) break;
           q_ph ^= 1u << buf;
           q_uses |= 1u << buf;
@@ -898,9 +921,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         }
         if (!two) qb ^= 1;
       }
-      if (*abort_flag)
-        for (int i = 0; i < 2; ++i)
-          if (q_uses >> i & 1) (void)mbar_wait(&q_full[i], q_ph >> i & 1);
+      for (int i = 0; i < 2; ++i)   // as for K and V
+        if (q_uses >> i & 1) (void)mbar_wait(&q_full[i], q_ph >> i & 1);
     } else if (warp == 10) {
       // ---- schedule: this CTA's share of the unit line ------------------------------
       const int n_s = pa_n_seqs(p);
@@ -927,7 +949,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       int n_items = 0;
       auto push = [&](const PaItem& w) {
         const int qi = n_items % PA_QUEUE, use = n_items / PA_QUEUE;
-        if (use > 0 && !__all_sync(0xffffffffu, pa_wait(&it_empty[qi], (unsigned)((use - 1) & 1), abort_flag))) return false;
+        if (use > 0 && !pa_wait_warp(&it_empty[qi], (unsigned)((use - 1) & 1), abort_flag)) return false;
         if (lane == 0) {
           queue[qi] = w;
           pa_arrive(&it_full[qi]);
@@ -998,17 +1020,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         });
       }
       if (ok && tail.out_mode == PA_PIECE) ok = push(tail);
-      if (ok) {
+      if (ok && !pa_held(PA_HOLD_STOP)) {
         tail.out_mode = PA_STOP;
         push(tail);
       }
     }
   }
   // every role is done: each item's last products were awaited by its
-  // epilogue, or the CTA gave up
+  // epilogue, or the CTA gave up, and the products in flight are awaited here
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
+    if (*abort_flag) {
+      if (elect_one()) umma_commit(mma_done);
+      __syncwarp();
+      (void)mbar_wait(mma_done, 0);
+    }
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }

@@ -11,8 +11,10 @@ REPO = os.path.dirname(PKG_ROOT)
 CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(HERE, "_lib", "libhokv.so")
-# profiling variant: the same sources with phase stamps in the decode kernels
-VARIANTS = {"": (OUT, []), "stamps": (os.path.join(HERE, "_lib", "libhokv_stamps.so"), ["-DHOKV_STAMPS"])}
+# instrumented variant: the same sources with phase stamps in the decode kernels and signals of the packed attention
+# that a test can keep back
+VARIANTS = {"": (OUT, []),
+            "stamps": (os.path.join(HERE, "_lib", "libhokv_stamps.so"), ["-DHOKV_STAMPS", "-DHOKV_HOLD"])}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr", "--extended-lambda"]
@@ -44,7 +46,7 @@ def build(force: bool = False, nvcc: str = "nvcc", verbose: bool = True, variant
 
 
 def build_all(force: bool = False, verbose: bool = True):
-    """The product library and the profiling variant, compiled in parallel."""
+    """The product library and the instrumented variant, compiled in parallel."""
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(len(VARIANTS)) as ex:
         return list(ex.map(lambda v: build(force=force, verbose=verbose, variant=v), VARIANTS))

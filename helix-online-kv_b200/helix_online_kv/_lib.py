@@ -21,8 +21,9 @@ except ImportError:  # pragma: no cover - torch is a hard dependency of the devi
     torch = None
     _HAS_TORCH = False
 
-# HOKV_LIB_VARIANT=stamps loads the profiling build (phase stamps in the decode
-# kernels, hokv_phase_stamps); the default is the product library.
+# HOKV_LIB_VARIANT=stamps loads the instrumented build (phase stamps in the decode
+# kernels, hokv_phase_stamps; signals kept back for tests, hokv_hold); the default
+# is the product library.
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib",
                         "libhokv_stamps.so" if os.environ.get("HOKV_LIB_VARIANT") == "stamps" else "libhokv.so")
 
@@ -146,6 +147,7 @@ _SIGS = {
     "hokv_prefilter_mask": (_c_int, [_vp, _c_int, _vp, _c_i64, _c_int, _vp, _vp]),
     "hokv_scale_f32_to_f64": (_c_int, [_vp, _c_i64, _c_f64, _vp, _vp]),
     "hokv_phase_stamps": (_c_int, [_vp, _c_sz]),
+    "hokv_hold": (_c_int, [_c_int]),
 }
 
 _lock = threading.Lock()

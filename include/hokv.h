@@ -412,6 +412,15 @@ int hokv_age_tokens(const hokv_cdc03_args* a, const int* cold_from, const int* c
  * ---------------------------------------------------------------------- */
 int hokv_phase_stamps(uint64_t* out, size_t n_values);
 
+/* Testing.  No counterpart in the reference.  In a library built with
+ * -DHOKV_HOLD, later hokv_packed_attention calls on the current device keep
+ * back signals that their waits need, in every eighth CTA (what: 1 the marks
+ * of an item's pieces, 2 the softmax weights of a warp, 4 the end of the item
+ * stream; a sum of these), and wait for a fiftieth of the usual limits, so
+ * that they end with HOKV_ERR_TIMEOUT in the device status; 0 ends that.  The
+ * product build returns HOKV_ERR_UNSUPPORTED. */
+int hokv_hold(int what);
+
 #ifdef __cplusplus
 }
 #endif
