@@ -101,7 +101,7 @@ struct PaP : PaSched {
   float2* ml;                    // [n_ctas][2][256] (m, sum)
   float4* o;                     // [n_ctas][2][D / 4][256]
   unsigned long long* ready;     // [n_ctas][2][8] the call's token when 32 rows of a piece are written, then 0 again
-  unsigned long long token;      // this call's
+  unsigned long long token;      // this call's; a replayed call's marks also carry g_pa_failures
   int2* tok_info;                // prefix only: [2][T][Hkv] (first | last CTA << 8 or -1: row-wise, token in item)
   float2* row_ml;                // prefix only: [2][T][Hq]
   float4* row_o;                 // prefix only: [2][T][Hq][D / 4]
@@ -111,7 +111,13 @@ struct PaP : PaSched {
 struct PaJoinItem {
   int n, first, tok0, n_tok, hk;   // pieces (0: none to join) from CTA `first` on, rows
   int left;                        // softmax warps that have joined their part
+  unsigned long long token;        // what this launch's marks hold
 };
+// CTAs that gave up, since the library was loaded on the device.  One that did may leave marks behind, and a graph
+// replays its call's token: the marks of a launch carry both, so that later replays do not take old marks for theirs.
+// Every CTA reads the count at its start.  It only changes while a call fails; a call on another stream that starts at
+// that moment may see both values, and then its own waits run out.
+__device__ unsigned long long g_pa_failures = 0;
 // Workspace slot of piece i of an item whose first one is CTA `first`'s.
 __device__ __forceinline__ int pa_slot(int first, int i) { return (first + i) * 2 + (i == 0 ? 1 : 0); }
 
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (join) pa_arrive(&o_empty[1]);
         if (out_mode == PA_PIECE && p.prefix == 0) {   // these rows of the piece are written
           __threadfence();
-          if (!pa_held(PA_HOLD_MARK)) store_release(&p.ready[(int64_t)out_at * 8 + (prow >> 5)], p.token);
+          if (!pa_held(PA_HOLD_MARK)) store_release(&p.ready[(int64_t)out_at * 8 + (prow >> 5)], s_join->token);
         }
       }
       item_done();
@@ -614,7 +620,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       bool got = true;
 #pragma unroll 1
       for (int e = lane; got && e < n * words; e += 32)
-        got = pa_wait_ready(&p.ready[pa_slot(first, e / words) * 8 + e % words], p.token, abort_flag);
+        got = pa_wait_ready(&p.ready[pa_slot(first, e / words) * 8 + e % words], s_join->token, abort_flag);
       __syncwarp();
       __threadfence();
       if (__all_sync(0xffffffffu, got)) {
@@ -925,6 +931,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         if (q_uses >> i & 1) (void)mbar_wait(&q_full[i], q_ph >> i & 1);
     } else if (warp == 10) {
       // ---- schedule: this CTA's share of the unit line ------------------------------
+      unsigned long long failures = 0;   // on its way during the scan
+      if (lane == 0) failures = *reinterpret_cast<volatile unsigned long long*>(&g_pa_failures);
       const int n_s = pa_n_seqs(p);
       const int per = (n_s + 31) / 32;
       const int s_lo = min(lane * per, n_s), s_hi = min(s_lo + per, n_s);
@@ -937,6 +945,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
         mine += pa_seq_units(p, q);
       }
       if (bad) dev_flag(HOKV_ERR_DEVICE_INPUT);
+      if (lane == 0) s_join->token = p.token ^ (failures * 0xd1342543de82ef95ull);
       int64_t incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -1032,6 +1041,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
   __syncthreads();
   if (warp == 9) {
     if (*abort_flag) {
+      if (lane == 0) atomicAdd(&g_pa_failures, 1ull);
       if (elect_one()) umma_commit(mma_done);
       __syncwarp();
       (void)mbar_wait(mma_done, 0);

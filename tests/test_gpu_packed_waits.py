@@ -61,6 +61,43 @@ def run_out():
             L.device_status()
 
 
+def replay():
+    """A captured call whose waits run out, marks of some pieces left behind; its replays on new data, at once and after
+    more failures, and a graph captured before in the same pool are right."""
+    import torch
+
+    from helix_online_kv import _lib as L
+    from helix_online_kv.prefill import packed_attention
+    query, k, v, kl = _batch(torch, [9000, 7000, 12000], D=64)
+    other, *_ = _batch(torch, [1, 1, 1], D=64, seed=2)
+    first = packed_attention(query, k, v, kv_len=kl)
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            outs.append(packed_attention(query, k, v, kv_len=kl))
+        pool = graphs[0].pool()
+    for graph, out in zip(graphs, outs):
+        graph.replay()
+        assert torch.equal(out, first)
+    for round_ in range(4):
+        graph, out = graphs[round_ % 2], outs[round_ % 2]
+        _held(L, MARKS, graph.replay)
+        if round_ == 3:
+            _held(L, WEIGHTS, graph.replay)
+        # other data: a piece taken from the failed replay would show
+        query.copy_(other if round_ % 2 == 0 else query.flip(1))
+        want = packed_attention(query, k, v, kv_len=kl)
+        for graph, out in zip(graphs, outs):
+            for _ in range(3):
+                out.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want)
+        L.device_status()
+
+
 def _child(name):
     env = dict(os.environ, HOKV_LIB_VARIANT="stamps")
     r = subprocess.run([sys.executable, os.path.abspath(__file__), name], env=env, capture_output=True, text=True, timeout=240)
@@ -72,6 +109,11 @@ def test_waits_that_run_out_are_reported_and_the_next_call_is_right():
     _child("run_out")
 
 
+@pytest.mark.gpu
+def test_replays_after_a_failed_one_do_not_take_its_marks():
+    _child("replay")
+
+
 def test_the_product_keeps_nothing_back():
     from helix_online_kv import _lib as L
     if os.environ.get("HOKV_LIB_VARIANT"):
@@ -81,4 +123,4 @@ def test_the_product_keeps_nothing_back():
 
 if __name__ == "__main__":
     sys.path.insert(0, os.path.join(os.path.dirname(HERE), "helix-online-kv_b200"))
-    {f.__name__: f for f in (run_out,)}[sys.argv[1]]()
+    {f.__name__: f for f in (run_out, replay)}[sys.argv[1]]()
