@@ -64,7 +64,10 @@ HD int64_t pa_max(int64_t a, int64_t b) { return a > b ? a : b; }
 
 HD int pa_n_seqs(const PaSched& p) { return p.n_seqs + (p.prefix > 0 ? 1 : 0); }
 // Query tokens that belong to a sequence.
-HD int pa_used(const PaSched& p) { return p.cu_q ? (int)pa_min(pa_max(p.cu_q[p.n_seqs], 0), p.T) : p.n_seqs; }
+HD int pa_used(const PaSched& p) {
+  if (!p.cu_q || p.n_seqs == 0) return p.n_seqs;
+  return (int)pa_min(pa_max(p.cu_q[p.n_seqs], 0), p.T);
+}
 
 // Sequence s of the schedule (with a prefix, 0 is the prefix against all
 // tokens).  One whose lengths do not fit the tensors is `bad` and empty, so
@@ -84,7 +87,7 @@ HD PaSeq pa_seq(const PaSched& p, int s) {
     s -= 1;
   }
   const int a = p.cu_q ? p.cu_q[s] : s, e = p.cu_q ? p.cu_q[s + 1] : s + 1;
-  bool bad = a < 0 || e < a || e > p.T;
+  bool bad = a < 0 || e < a || e > p.T || (s == 0 && a > 0);   // tokens ahead of the first one would belong to none
   r.src = 0;
   r.causal = p.causal;
   if (p.cu_k) {

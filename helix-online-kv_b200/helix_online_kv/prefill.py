@@ -223,8 +223,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(query key^T * scaling [causal]) value for every sequence of a packed batch.
 
-    query [T, H_q, D]: sequence b owns tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (without cu_seqlens_q, token
-    b).  key/value either packed [S, H_kv, D] with cu_seqlens_k [B + 1] (default: cu_seqlens_q) or in slots [B,
+    query [T, H_q, D]: sequence b owns tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]), the first start being 0
+    (without cu_seqlens_q, token b).  key/value either packed [S, H_kv, D] with cu_seqlens_k [B + 1] (default: cu_seqlens_q) or in slots [B,
     H_kv, capacity, D] with kv_len [B], the keys each sequence holds, its new tokens included (a slot's rows behind
     kv_len are not used).  Lengths are int32 CUDA vectors and stay on the device.  Causal: query i of a sequence
     with n keys and m queries sits at position n - m + i; a query that sees no key gives zeros.  f16/bf16, head

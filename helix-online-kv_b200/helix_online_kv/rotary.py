@@ -85,7 +85,7 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     """Rotated queries [T, H_q, D]; keys and values appended to their slots.
 
     query [T, H_q, D], key/value [T, H_kv, D] (contiguous head dims, any other strides: parts of one projection are
-    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]) (cu_seqlens None: token b).  Token i of b sits at
+    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]), the first start being 0 (None: token b).  Token i of b sits at
     position kv_len[b] + i, or positions[t] when given (sequences behind a shared prefix), and its key and value go to
     row kv_len[b] + i of key_slots/value_slots [B, H_kv, capacity, D].  kv_len (the rows held before the call) is
     not changed.  With q_weight / k_weight [D] the head is first multiplied by weight / sqrt(mean(x^2) + eps).

@@ -112,3 +112,45 @@ def test_scores_of_any_finite_size(dtype, rising):
     ref = v[top].repeat_interleave(2, 1).double()
     fi = torch.finfo(dtype)
     _check(out, ref, ref.abs() * (fi.eps + 2.0 ** -20) + fi.smallest_normal * fi.eps)
+
+
+@pytest.mark.parametrize("kind", ["packed", "prefix", "append"])
+def test_starts_that_do_not_begin_at_the_first_token_are_reported(kind):
+    """Rows ahead of the first sequence would belong to none; the sequences behind the first one stay right, and so do
+    later calls."""
+    from helix_online_kv import _lib as L
+    from helix_online_kv.prefill import packed_attention
+    from helix_online_kv.rotary import norm_rotate_append
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(3)
+    x = lambda *s: torch.randn(s, generator=g, device="cuda").to(F16)   # noqa: E731
+    query, key, k, v, pk, pv = x(9, 4, 64), x(9, 2, 64), x(2, 2, 20, 64), x(2, 2, 20, 64), x(2, 300, 64), x(2, 300, 64)
+    kl, f = torch.tensor([8, 9], dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+
+    def call(cu):
+        if kind == "packed":
+            return packed_attention(query, k, v, cu, kv_len=kl)
+        if kind == "prefix":
+            return shared_prefix_attention(query, pk, pv, k, v, kl, cu)
+        return norm_rotate_append(query, key, key, k, v, cu, kl, f)
+
+    good = call(lens_tensor([4, 5]))
+    cu = torch.tensor([2, 4, 9], dtype=torch.int32, device="cuda")
+    out = call(cu)
+    with pytest.raises(L.HokvError) as e:
+        L.device_status()
+    assert e.value.status == L.ERR_DEVICE_INPUT
+    assert torch.equal(out[4:], good[4:])
+    assert torch.equal(call(lens_tensor([4, 5])), good)
+    L.device_status()
+
+
+def test_keys_may_start_behind_the_first_row():
+    """Packed keys have starts of their own: rows ahead of cu_seqlens_k[0] belong to no sequence."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(4)
+    query, k, v = (torch.randn((n, h, 64), generator=g, device="cuda").to(F16) for n, h in ((9, 4), (40, 2), (40, 2)))
+    k[:7], v[:7] = float("nan"), float("inf")
+    cu_k = torch.tensor([7, 20, 40], dtype=torch.int32, device="cuda")
+    out = packed_attention(query, k, v, lens_tensor([4, 5]), cu_k)
+    _check(out, *reference(query, [4, 5], [k[7:20], k[20:]], [v[7:20], v[20:]], 64 ** -0.5))
