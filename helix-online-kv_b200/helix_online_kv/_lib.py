@@ -200,6 +200,14 @@ def check(status: int, what: str = ""):
         raise HokvError(status, f"{what}: {msg}" if what else msg)
 
 
+def check_call(status: int, what: str):
+    """``check`` of an entry point that passes its caller's arguments on: what the library does not take of them (and
+    the Python checks did not see) is a ValueError too."""
+    if status in (ERR_INVALID, ERR_UNSUPPORTED):
+        raise ValueError(f"{what}: {lib().hokv_last_error().decode(errors='replace')}")
+    check(status, what)
+
+
 def stream():
     return _vp(torch.cuda.current_stream().cuda_stream)
 

@@ -170,7 +170,7 @@ def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
         a.prefix_len = prefix_key.shape[1]
     need = ctypes.c_size_t(0)
     with torch.cuda.device(dev):
-        L.check(L.lib().hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), "packed_attention")
+        L.check_call(L.lib().hokv_packed_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)), "packed_attention")
     return a, need.value
 
 
@@ -211,9 +211,7 @@ def _packed(what, query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
         a.cu_seqlens_k = cu_seqlens_k.data_ptr()
     status = L.call_on(geometry[0][3], L.lib().hokv_packed_attention, a)
     if status:
-        if status == L.ERR_INVALID:   # what the signatures do not show: addresses
-            raise ValueError(f"{what}: {L.lib().hokv_last_error().decode(errors='replace')}")
-        L.check(status, what)
+        L.check_call(status, what)   # strides that do not nest; addresses, which the signatures do not show
     return out
 
 

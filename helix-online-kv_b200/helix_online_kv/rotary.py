@@ -119,5 +119,5 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
         a.q_weight = q_weight.data_ptr()
     if k_weight is not None:
         a.k_weight = k_weight.data_ptr()
-    L.check(L.call_on(geometry[0][3], L.lib().hokv_norm_rotate_append, a), "norm_rotate_append")
+    L.check_call(L.call_on(geometry[0][3], L.lib().hokv_norm_rotate_append, a), "norm_rotate_append")
     return out

@@ -32,5 +32,7 @@ def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefi
     [B, H_kv, capacity, D] with kv_len [B], or packed [S, H_kv, D] with cu_seqlens_k, causal among its own keys (query i
     of m sits at own position n - m + i).  -> [T, H_q, D].  Scratch grows with T (about 8 H_q D bytes per token), so
     this form is for decoding and drafted tokens, not for long prompts behind a prefix."""
+    if (prefix_key is None) != (prefix_value is None):
+        raise ValueError("Expected prefix_key and prefix_value, got one of them")
     return _packed("shared_prefix_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal,
                    out, prefix_key, prefix_value)

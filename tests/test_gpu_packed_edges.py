@@ -154,3 +154,21 @@ def test_keys_may_start_behind_the_first_row():
     cu_k = torch.tensor([7, 20, 40], dtype=torch.int32, device="cuda")
     out = packed_attention(query, k, v, lens_tensor([4, 5]), cu_k)
     _check(out, *reference(query, [4, 5], [k[7:20], k[20:]], [v[7:20], v[20:]], 64 ** -0.5))
+
+
+def test_refusals_of_the_library_are_value_errors():
+    """Strides that do not nest, numbers that fp32 does not hold: refused before anything is launched."""
+    from helix_online_kv.prefill import packed_attention
+    from helix_online_kv.rotary import norm_rotate_append
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    z = lambda *s: torch.zeros(s, dtype=F16, device="cuda")   # noqa: E731
+    q, k, cu = z(4, 8, 64), z(4, 2, 64), lens_tensor([4])
+    for kw in (dict(key=z(1, 2, 64).expand(4, 2, 64)), dict(value=z(4, 1, 64).expand(4, 2, 64)), dict(scaling=1e-60),
+               dict(scaling=1e39)):
+        with pytest.raises(ValueError):
+            packed_attention(**{**dict(query=q, key=k, value=k, cu_seqlens_q=cu), **kw})
+    with pytest.raises(ValueError):
+        shared_prefix_attention(q, z(1, 9, 64).expand(2, 9, 64), z(2, 9, 64), k, k, cu_seqlens_q=cu)
+    slots, n = z(1, 2, 16, 64), lens_tensor([])
+    with pytest.raises(ValueError):
+        norm_rotate_append(q, k, k, slots, slots.clone(), cu, n, torch.ones(32, device="cuda"), eps=1e39)

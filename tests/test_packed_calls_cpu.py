@@ -53,3 +53,40 @@ def test_an_eps_changed_in_place_is_read_again(monkeypatch):
     call(eps)
     assert seen == [0.5, 2.0] and all(type(e) is float for e in seen)
     assert all(not isinstance(x, torch.Tensor) for key in R._checked for x in key)
+
+
+@pytest.mark.parametrize("status,error", [(L.ERR_INVALID, ValueError), (L.ERR_UNSUPPORTED, ValueError),
+                                          (L.ERR_CUDA, L.HokvError), (L.ERR_WORKSPACE, L.HokvError)])
+@pytest.mark.parametrize("stage", ["workspace", "call"])
+def test_arguments_that_the_library_refuses_are_value_errors(monkeypatch, status, error, stage):
+    """Refusals of the C entry points (strides that do not nest, a scaling that is 0 in fp32) are as Python's own."""
+    class Args:
+        n_tokens = 2
+
+    monkeypatch.setattr(L, "call_on", lambda *a: status)
+    q, cu = torch.zeros(2, 2, 64), torch.zeros(3, dtype=torch.int32)
+    if stage == "call":
+        with pytest.raises(error):
+            L.check_call(L.call_on(), "packed_attention")
+        from_buffer = type("A", (), {"from_buffer_copy": staticmethod(lambda a: a)})
+        monkeypatch.setattr(L, "PackedArgs", from_buffer)
+        monkeypatch.setattr(L, "NormRotateArgs", from_buffer)
+        monkeypatch.setattr(F, "_checked", L.Checked())
+        monkeypatch.setattr(R, "_checked", L.Checked())
+        monkeypatch.setattr(F, "_packed_check", lambda *a: (Args(), 16))
+        monkeypatch.setattr(R, "_check", lambda *a: Args())
+        with pytest.raises(error):
+            F.packed_attention(q, q, q, cu)
+        with pytest.raises(error):
+            R.norm_rotate_append(q, q, q, q, q, None, cu[:2], q)
+    else:
+        assert L.check_call(L.OK, "x") is None
+        with pytest.raises(error, match="packed"):
+            L.check_call(status, "packed")
+
+
+def test_half_a_prefix_is_refused():
+    q, cu = torch.zeros(2, 2, 64), torch.zeros(3, dtype=torch.int32)
+    for pk, pv in ((q, None), (None, q)):
+        with pytest.raises(ValueError, match="prefix_key and prefix_value"):
+            shared_prefix_attention(q, pk, pv, q, q, cu_seqlens_q=cu)
