@@ -49,7 +49,9 @@
 // Rows behind a sequence's end: their scores are masked by selection (any bit
 // pattern, NaN included, drops out), and the V rows of the last, partial
 // 16-token step are zeroed in shared memory before the product, steps past it
-// are not issued.
+// are not issued.  Rows of the sequence itself that the causal mask hides take
+// part in an item's products, with weight 0, up to the end of its last key tile:
+// only a value that is not finite shows, at queries up to 2 TT + 126 tokens ahead.
 //
 // What bounds it (B200, 32 query / 8 KV heads of 128 dims, bf16): prompts by a
 // slot's chain of scores, softmax and products, 3,300 cycles a two-tile step

@@ -172,3 +172,24 @@ def test_refusals_of_the_library_are_value_errors():
     slots, n = z(1, 2, 16, 64), lens_tensor([])
     with pytest.raises(ValueError):
         norm_rotate_append(q, k, k, slots, slots.clone(), cu, n, torch.ones(32, device="cuda"), eps=1e39)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 64), (8, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_non_finite_rows_that_the_mask_hides(Hq, Hkv, D, bad):
+    """A hidden key reaches no query; a hidden value reaches at most the queries W + 126 tokens ahead of it, W = 2
+    floor(128 / group), as the documentation says; whole items, two tiles each, and items cut over CTAs."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(D + Hq)
+    n, W = 1500, 2 * (128 * Hkv // Hq)
+    query, k, v = (torch.randn((n, h, D), generator=g, device="cuda").to(BF16) for h in (Hq, Hkv, Hkv))
+    clean = packed_attention(query, k, v, lens_tensor([n]))
+    for j in (200, 777, 1499):
+        k2, v2 = k.clone(), v.clone()
+        k2[j], v2[j] = bad, bad
+        out = packed_attention(query, k2, v, lens_tensor([n]))
+        assert torch.equal(out[:j], clean[:j])
+        out = packed_attention(query, k, v2, lens_tensor([n]))
+        free = max(j - (W + 126), 0)
+        assert torch.equal(out[:free], clean[:free])
+        assert not out[j:].isfinite().any()
