@@ -935,17 +935,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       // ---- schedule: this CTA's share of the unit line ------------------------------
       unsigned long long failures = 0;   // on its way during the scan
       if (lane == 0) failures = *reinterpret_cast<volatile unsigned long long*>(&g_pa_failures);
-      const int n_s = pa_n_seqs(p);
-      const int per = (n_s + 31) / 32;
-      const int s_lo = min(lane * per, n_s), s_hi = min(s_lo + per, n_s);
-      int64_t mine = 0;
       bool bad = false;
-#pragma unroll 1
-      for (int s = s_lo; s < s_hi; ++s) {
-        const PaSeq q = pa_seq(p, s);
-        bad = bad || q.bad;
-        mine += pa_seq_units(p, q);
-      }
+      const int64_t mine = pa_lane_units(p, lane, bad);
       if (bad) dev_flag(HOKV_ERR_DEVICE_INPUT);
       if (lane == 0) s_join->token = p.token ^ (failures * 0xd1342543de82ef95ull);
       int64_t incl = mine;
@@ -972,30 +963,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       bool ok = true;
       PaItem tail = {};
       if (begin < end) {
-        // the lane whose sequences hold unit `begin`, its first one and the units before that
-        const int owner = __ffs(__ballot_sync(0xffffffffu, incl > begin)) - 1;
-        int s = 0;
-        int64_t at = 0;
-        if (lane == owner) {
-          at = incl - mine;
-          s = s_lo;
-        }
-        s = __shfl_sync(0xffffffffu, s, owner);
-        at = __shfl_sync(0xffffffffu, at, owner);
-        PaSeq q = pa_seq(p, s);
-#pragma unroll 1
-        for (int64_t units; per > 1 && at + (units = pa_seq_units(p, q)) <= begin; q = pa_seq(p, ++s)) at += units;
-        // its last pair that starts at or before `begin`, 32 at a time
-        int pr = 0;
-#pragma unroll 1
-        for (int n = (q.nq + 2 * TT - 1) / (2 * TT); n > 1;) {
-          const int step = (n + 31) / 32, probe = min(pr + lane * step, pr + n - 1);
-          const bool before = at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, 2 * TT, probe) <= begin;
-          const int k = 31 - __clz(__ballot_sync(0xffffffffu, before && lane * step < n));   // lane 0 always is
-          n = min(step, n - k * step);
-          pr += k * step;
-        }
-        ok = pa_walk(p, (int)blockIdx.x, begin, end, s, at, pr, [&](const PaItem& w, bool begins, bool ends,
+        const PaStart at = pa_find_start(p, begin, [&](int) { return mine; }, [&](int) { return incl; });
+        ok = pa_walk(p, (int)blockIdx.x, begin, end, at.s, at.at, at.pr, [&](const PaItem& w, bool begins, bool ends,
                                                                     int64_t item_at, int sh, int tiles) {
           if (w.out_mode == PA_PIECE && p.prefix == 0 && !begins) {
             // an item that earlier CTAs began comes last: its other pieces are done by then, and whoever holds its

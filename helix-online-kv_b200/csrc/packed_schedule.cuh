@@ -163,17 +163,93 @@ HD int pa_last_cta(int64_t share, int64_t item_at, int sh, int tiles) {
   return (int)((item_at + PA_ITEM + ((int64_t)(tiles - 1) << sh)) / share);
 }
 
+// Where a CTA's share begins is found by a warp.  The host runs the same code
+// over 32 lanes in turn: f(lane) is each lane's value.
+template <typename F>
+HD unsigned pa_ballot(F f) {
+#if defined(__CUDA_ARCH__)
+  return __ballot_sync(0xffffffffu, f((int)(threadIdx.x & 31)));
+#else
+  unsigned votes = 0;
+  for (int lane = 0; lane < 32; ++lane) votes |= (f(lane) ? 1u : 0u) << lane;
+  return votes;
+#endif
+}
+template <typename F>
+HD int64_t pa_from(int lane, F f) {
+#if defined(__CUDA_ARCH__)
+  return __shfl_sync(0xffffffffu, f((int)(threadIdx.x & 31)), lane);
+#else
+  return f(lane);
+#endif
+}
+HD int pa_lowest(unsigned votes) {   // of at least one
+#if defined(__CUDA_ARCH__)
+  return __ffs(votes) - 1;
+#else
+  return __builtin_ctz(votes);
+#endif
+}
+HD int pa_highest(unsigned votes) {
+#if defined(__CUDA_ARCH__)
+  return 31 - __clz(votes);
+#else
+  return 31 - __builtin_clz(votes);
+#endif
+}
+
+// Units of the sequences that are one lane's to count, and whether one of them is bad.
+HD int pa_lane_first(const PaSched& p, int lane) {
+  const int n_s = pa_n_seqs(p);
+  return (int)pa_min((int64_t)lane * ((n_s + 31) / 32), n_s);
+}
+HD int64_t pa_lane_units(const PaSched& p, int lane, bool& bad) {
+  const int last = pa_lane_first(p, lane + 1);
+  int64_t units = 0;
+  ROLLED for (int s = pa_lane_first(p, lane); s < last; ++s) {
+    const PaSeq q = pa_seq(p, s);
+    bad = bad || q.bad;
+    units += pa_seq_units(p, q);
+  }
+  return units;
+}
+
 // The last pair of sequence q (`at` units before it) that starts at or before
-// unit pos.
+// unit pos, 32 probes at a time.
 HD int pa_find_pair(const PaSched& p, const PaSeq& q, int64_t at, int64_t pos) {
   const int W = 2 * p.TT;
-  int lo = 0, hi = (q.nq + W - 1) / W - 1;
-  ROLLED while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, mid) <= pos) lo = mid;
-    else hi = mid - 1;
+  int pr = 0;
+  ROLLED for (int n = (q.nq + W - 1) / W; n > 1;) {
+    const int step = (n + 31) / 32;
+    const unsigned before = pa_ballot([&](int lane) {   // lane 0's always is
+      const int probe = (int)pa_min(pr + lane * step, pr + n - 1);
+      return at + (int64_t)p.Hkv * pa_units_before(q.kv, q.nq, q.causal, W, probe) <= pos && lane * step < n;
+    });
+    const int k = pa_highest(before);
+    n = (int)pa_min(step, n - k * step);
+    pr += k * step;
   }
-  return lo;
+  return pr;
+}
+
+// The sequence and pair that hold unit `begin` (below the total), and the units
+// before the sequence.  mine(lane), upto(lane): a lane's units, and those of
+// all lanes up to it.
+struct PaStart {
+  int s, pr;
+  int64_t at;
+};
+template <typename Mine, typename Upto>
+HD PaStart pa_find_start(const PaSched& p, int64_t begin, Mine mine, Upto upto) {
+  PaStart r;
+  const int owner = pa_lowest(pa_ballot([&](int lane) { return upto(lane) > begin; }));
+  r.s = pa_lane_first(p, owner);
+  r.at = pa_from(owner, [&](int lane) { return upto(lane) - mine(lane); });
+  PaSeq q = pa_seq(p, r.s);
+  const bool several = pa_n_seqs(p) > 32;   // sequences of a lane
+  ROLLED for (int64_t units; several && r.at + (units = pa_seq_units(p, q)) <= begin; q = pa_seq(p, ++r.s)) r.at += units;
+  r.pr = pa_find_pair(p, q, r.at, begin);
+  return r;
 }
 
 // CTA `cta`'s items: units [begin, end), which start in pair `pr` of sequence s
