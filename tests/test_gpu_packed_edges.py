@@ -1,5 +1,6 @@
 """packed_attention and shared_prefix_attention where a mistake hides from random
-data: keys far below a row's largest score, scores of any finite size."""
+data: keys far below a row's largest score, scores of any finite size, starts, hidden
+rows, and results that show the loss of a single key."""
 
 import math
 
@@ -193,3 +194,108 @@ def test_non_finite_rows_that_the_mask_hides(Hq, Hkv, D, bad):
         free = max(j - (W + 126), 0)
         assert torch.equal(out[:free], clean[:free])
         assert not out[j:].isfinite().any()
+
+
+# ---- every key counts: results that show the loss of a single one ------------------
+
+
+def _counted(q, kv, ahead, step, D, Hq):
+    """Rows of equal scores: the share of each channel's keys among those a query sees, [T, H_q, D]; key j of a row
+    (`ahead` prefix keys, then the own ones) is marked in channel j // step."""
+    rows = []
+    for m, n in zip(q, kv):
+        marks = torch.nn.functional.one_hot(torch.arange(ahead + n, device="cuda") // step, D).double().cumsum(0)
+        seen = torch.arange(ahead + n - m, ahead + n, device="cuda") + 1
+        rows.append(torch.where((seen > 0)[:, None], marks[seen - 1] / seen[:, None], 0.0))
+    return torch.cat(rows)[:, None].expand(-1, Hq, -1)
+
+
+def _share_tolerance(ref, dtype):
+    """Equal scores give equal weights, exact sums of whole numbers and one quotient: half a step of the output, and
+    2^-20 for the weights' common factor and the quotient.  One key of a channel's 128 is 2^-7."""
+    return ref * (torch.finfo(dtype).eps / 2 + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q,kv,step", [
+    ([1], [9000], 128), ([1], [12345], 128), ([1, 1, 1], [5000, 1, 16384], 128),   # one token over many CTAs
+    ([1, 3], [1030, 2047], 16),
+    ([2048], [2048], 16), ([300, 1], [2000, 2041], 16),                           # causal prompts, cut and whole
+    ([40, 3], [7000, 6001], 128),
+])
+def test_equal_scores_count_every_key(q, kv, step, dtype):
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(sum(kv))
+    Hq, Hkv, D = 8, 2, 128
+    query = torch.zeros(sum(q), Hq, D, dtype=dtype, device="cuda")
+    k = torch.randn((sum(kv), Hkv, D), generator=g, device="cuda").to(dtype)
+    v = torch.cat([torch.nn.functional.one_hot(torch.arange(n, device="cuda") // step, D) for n in kv])
+    v = v[:, None].expand(-1, Hkv, -1).to(dtype).contiguous()
+    out = packed_attention(query, k, v, lens_tensor(q), lens_tensor(kv))
+    ref = _counted(q, kv, 0, step, D, Hq)
+    _check(out, ref, _share_tolerance(ref, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("P,q,kv", [(8000, [1, 2, 1], [40, 300, 1]), (129, [1, 3], [900, 5]),
+                                    (5001, [1] * 40, [7 * i + 1 for i in range(40)])])
+def test_equal_scores_count_every_key_behind_a_prefix(P, q, kv, dtype):
+    from helix_online_kv.shared_prefix import shared_prefix_attention
+    g = _gen(P)
+    Hq, Hkv, D = 8, 2, 128
+    query = torch.zeros(sum(q), Hq, D, dtype=dtype, device="cuda")
+    k, pk = (torch.randn(s, generator=g, device="cuda").to(dtype) for s in ((sum(kv), Hkv, D), (Hkv, P, D)))
+    one_hot = lambda j: torch.nn.functional.one_hot(j // 128, D).to(dtype)   # noqa: E731
+    pv = one_hot(torch.arange(P, device="cuda"))[None].expand(Hkv, -1, -1).contiguous()
+    v = torch.cat([one_hot(P + torch.arange(n, device="cuda")) for n in kv])[:, None].expand(-1, Hkv, -1).contiguous()
+    out = shared_prefix_attention(query, pk, pv, k, v, cu_seqlens_q=lens_tensor(q), cu_seqlens_k=lens_tensor(kv))
+    ref = _counted(q, kv, P, 128, D, Hq)
+    _check(out, ref, _share_tolerance(ref, dtype))
+
+
+def _codes(n, D, dtype):
+    """Keys [n, D] of +-1: the 14 bits of the key's number, nine times over; two keys whose numbers differ in d bits have
+    the product 126 - 18 d."""
+    bits = (torch.arange(n, device="cuda")[:, None] >> torch.arange(14, device="cuda")) & 1
+    k = torch.zeros(n, D, device="cuda")
+    k[:, :126] = (2 * bits - 1).float().repeat(1, 9)
+    return k.to(dtype)
+
+
+def _one_key_tolerance(ref, dtype):
+    """With a scaling of 4 the key that a query names outweighs each other one by e^72: half a step each for its weight
+    and the output, 2^-20 for fp32 products."""
+    fi = torch.finfo(dtype)
+    return ref.abs() * (fi.eps + 2.0 ** -20) + fi.smallest_normal * fi.eps
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [700, 3000, 9000, 12345])
+def test_single_keys_are_found(n, dtype):
+    """Queries that name one key each: the first, the last, both sides of every tile's edge; as one sequence of many
+    queries, and eight heads of one token at a time (items cut over CTAs)."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(n)
+    D = 128
+    k, v = _codes(n, D, dtype)[:, None], torch.randn((n, 1, D), generator=g, device="cuda").to(dtype)
+    names = sorted({x for e in range(0, n + 128, 128) for x in (e - 1, e, e + 1) if 0 <= x < n} | {n - 1})
+    names += names[:-len(names) % 8]
+    query = k[names]
+    out = packed_attention(query, k, v, lens_tensor([len(names)]), lens_tensor([n]), scaling=4.0, is_causal=False)
+    ref = v[names].double()
+    _check(out, ref, _one_key_tolerance(ref, dtype))
+    for at in range(0, len(names), 8):
+        out = packed_attention(query[at:at + 8].transpose(0, 1).contiguous(), k, v, lens_tensor([1]), lens_tensor([n]), scaling=4.0)
+        _check(out[0], ref[at:at + 8, 0], _one_key_tolerance(ref[at:at + 8, 0], dtype))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_prompt_whose_queries_name_themselves(dtype):
+    """The diagonal: query i names key i, the last one it sees."""
+    from helix_online_kv.prefill import packed_attention
+    g = _gen(1)
+    n, D = 3001, 128
+    k, v = _codes(n, D, dtype)[:, None], torch.randn((n, 1, D), generator=g, device="cuda").to(dtype)
+    out = packed_attention(k.expand(-1, 4, -1).contiguous(), k, v, lens_tensor([n]), scaling=4.0)
+    ref = v.double().expand(-1, 4, -1)
+    _check(out, ref, _one_key_tolerance(ref, dtype))
