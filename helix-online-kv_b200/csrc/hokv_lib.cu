@@ -1101,6 +1101,7 @@ static int packed_attention(const hokv_packed_args* a, void* stream) {
   p.zero_tail = a->zero_tail ? 1 : 0;
   p.n_ctas = ctas;
   p.sl2 = a->scale * PA_LOG2E;
+  p.raw_step = (PaRange<__half>::MOST - PaRange<__half>::LIFT - 0x1p-8f) / p.sl2;   // a little less: sums round
   unsigned char* w = reinterpret_cast<unsigned char*>(a->workspace);
   p.ready = reinterpret_cast<unsigned long long*>(w + ws.ready);
   p.token = pa_token();

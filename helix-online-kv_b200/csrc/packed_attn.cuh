@@ -99,6 +99,7 @@ struct PaP : PaSched {
   int64_t ost, osh;              // output element strides (token, head)
   int Hq, G, D, zero_tail, tma_out;   // tma_out: tokens of a warp's 32 rows, 0 when they are not whole tokens
   float sl2;                     // scale * log2(e)
+  float raw_step;                // f16: the step above which m is raised, as a score stands in S
   int k_t, k_h, k_b, v_t, v_h, v_b, pk_t, pk_h, pk_b, pv_t, pv_h, pv_b;   // coordinate slots of the maps
   float2* ml;                    // [n_ctas][2][256] (m, sum)
   float4* o;                     // [n_ctas][2][D / 4][256]
@@ -380,7 +381,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
     const uint32_t p_addr = tmem + lane_sel + (uint32_t)(PG::P0 + sl * 128);
     // rows of out on 32-byte boundaries and in whole 16-element steps: 32-byte stores
     const bool wide = p.D % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) % 32 | (uint64_t)(p.ost % 16) | (uint64_t)(p.osh % 16)) == 0;
-    const float raw_step = (PR::MOST - PR::LIFT - 0x1p-8f) / p.sl2;   // of a score as it stands in S
     unsigned s_ph = 0, o_ph = 0, o1_ph = 0, ml_ph = 0;   // phases of s_full[sl], o_full[sl]; slot 0: o_full[1], ml_full
     int u = 0;   // tasks of the items so far
     bool ok = true;
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
                 m_run = m_new + (mt - mt);            // an infinite maximum gives NaN, as inf - inf does
                 if constexpr (PR::NARROW) {
                   m_raw = raw;
-                  raw_most = __fadd_rd(raw, raw_step);
+                  raw_most = __fadd_rd(raw, p.raw_step);
                 }
               }
               nm = m_run == -INFINITY ? 0.f : -m_run;
