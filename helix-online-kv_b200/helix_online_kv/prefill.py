@@ -87,6 +87,18 @@ def prefill_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     return out
 
 
+def _rows_apart(t: torch.Tensor) -> bool:
+    """No two rows (last dim) of t share memory: in ascending stride order every dim covers the dims inside it."""
+    if t.numel() == 0:
+        return True
+    need = t.shape[-1]
+    for stride, extent in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1):
+        if stride < need:
+            return False
+        need = stride * extent
+    return True
+
+
 def _lengths(t, n: Optional[int], name: str, device) -> None:
     """A contiguous int32 CUDA vector (of n entries, when given) on `device`."""
     if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device or not t.is_cuda:
@@ -154,6 +166,8 @@ def _packed_check(query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling
                             or (out.numel() and (out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8))):
         raise ValueError(f"Expected out [{T}, {Hq}, {D}] {query.dtype} on {dev} with contiguous rows and strides in "
                          f"multiples of 8 elements, got {tuple(out.shape)} {out.dtype} on {out.device}")
+    if out is not None and not _rows_apart(out):
+        raise ValueError(f"Expected out with rows that do not overlap, got {tuple(out.shape)}, strides {out.stride()}")
     a.dtype, a.n_seqs, a.q_heads, a.kv_heads, a.head_dim, a.causal = _DTYPES[query.dtype], B, Hq, Hkv, D, is_causal
     a.scale, a.n_tokens, a.zero_tail = scale, T, out is None
     a.q_stride_t, a.q_stride_h = query.stride(0), query.stride(1)

@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
-from .prefill import _lengths
+from .prefill import _lengths, _rows_apart
 
 _DTYPES = {torch.float16: L.F16, torch.bfloat16: L.BF16, torch.float32: L.F32}
 
@@ -47,6 +47,9 @@ def _check(query, key, value, key_slots, value_slots, cu_seqlens, kv_len, inv_fr
         if t.shape != shape or t.dtype != dt or t.device != dev or (t.numel() and t.stride(-1) != 1):
             raise ValueError(f"Expected {name} {list(shape)} {dt} on {dev} with contiguous head dims, got {tuple(t.shape)} "
                              f"{t.dtype} on {t.device}, strides {t.stride()}")
+    for name, t in (("key_slots", key_slots), ("value_slots", value_slots), ("out", out)):
+        if t is not None and not _rows_apart(t):
+            raise ValueError(f"Expected {name} with rows that do not overlap, got {tuple(t.shape)}, strides {t.stride()}")
     B = slots[0]
     _lengths(kv_len, B, "kv_len", dev)
     if cu_seqlens is not None:

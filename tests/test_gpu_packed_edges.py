@@ -299,3 +299,20 @@ def test_a_prompt_whose_queries_name_themselves(dtype):
     out = packed_attention(k.expand(-1, 4, -1).contiguous(), k, v, lens_tensor([n]), scaling=4.0)
     ref = v.double().expand(-1, 4, -1)
     _check(out, ref, _one_key_tolerance(ref, dtype))
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    """An expanded out, or slots that several sequences share: rows would be written over one another."""
+    from helix_online_kv.prefill import packed_attention
+    from helix_online_kv.rotary import norm_rotate_append
+    z = lambda *s: torch.zeros(s, dtype=F16, device="cuda")   # noqa: E731
+    q, k, cu = z(4, 8, 64), z(4, 2, 64), lens_tensor([4])
+    for out in (z(1, 8, 64).expand(4, 8, 64), z(4, 1, 64).expand(4, 8, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            packed_attention(q, k, k, cu, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            norm_rotate_append(q, k, k, z(1, 2, 16, 64), z(1, 2, 16, 64), cu, lens_tensor([]), torch.ones(32, device="cuda"), out=out)
+    shared, own = z(1, 2, 16, 64).expand(2, 2, 16, 64), z(2, 2, 16, 64)
+    for ks, vs in ((shared, own), (own, shared)):
+        with pytest.raises(ValueError, match="overlap"):
+            norm_rotate_append(q, k, k, ks, vs, lens_tensor([2, 2]), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda"))

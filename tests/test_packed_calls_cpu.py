@@ -90,3 +90,15 @@ def test_half_a_prefix_is_refused():
     for pk, pv in ((q, None), (None, q)):
         with pytest.raises(ValueError, match="prefix_key and prefix_value"):
             shared_prefix_attention(q, pk, pv, q, q, cu_seqlens_q=cu)
+
+
+@pytest.mark.parametrize("shape,stride,ok", [
+    ((4, 8, 64), (512, 64, 1), True), ((4, 8, 64), (64, 256, 1), True),         # heads inside tokens, and outside
+    ((4, 8, 64), (640, 72, 1), True), ((1, 8, 64), (0, 64, 1), True),           # padded; one token
+    ((4, 8, 64), (0, 64, 1), False), ((4, 8, 64), (512, 0, 1), False),          # expanded
+    ((4, 8, 64), (64, 64, 1), False), ((4, 8, 64), (512, 32, 1), False),
+    ((2, 2, 16, 64), (2048, 1024, 64, 1), True), ((2, 2, 16, 64), (0, 1024, 64, 1), False),
+    ((0, 8, 64), (0, 0, 1), True),
+])
+def test_rows_that_overlap(shape, stride, ok):
+    assert F._rows_apart(torch.zeros(1 << 13).as_strided(shape, stride)) is ok
