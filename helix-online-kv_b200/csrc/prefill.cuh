@@ -15,7 +15,12 @@
 // warps of one tile work, the other tile's products run.  The running
 // maximum m is raised lazily: O and the running sum are rescaled only when a
 // row's maximum grows by more than 8 (log2 units), so P stays below 2^8 and
-// the final normalisation by the same m gives the exact softmax.
+// the final normalisation by the same m gives the exact softmax.  f16 weights
+// are subnormal below 2^-14, where a row with one dominant key may have most of
+// its mass: they are stored times 2^7 (up to 2^15), O with them and the sum
+// without, so that a weight keeps its half step down to 2^-21 of the largest and
+// one below that is off by 2^-32 of it at most.  Multiplying by a power of two
+// changes no other bit.
 //
 // Roles (320 threads): warps 0-3 the softmax of query tile 0 (thread = row =
 // TMEM lane), warps 4-7 that of tile 1, warp 8 lane 0 loads the tiles with
@@ -161,6 +166,14 @@ __device__ __forceinline__ float pf_ex2(float x) {
   return y;
 }
 
+// What f16 weights are stored times.  A row whose scores fp32 holds coarsely keeps the room above 2^8 for their rounding.
+constexpr float PF_UP = 128.f, PF_UP_MAX = 0x1p20f;
+template <typename T>
+__device__ __forceinline__ uint32_t pf_pack(float a, float b, float up) {
+  if constexpr (std::is_same<T, __half>::value) return pack2<T>(a * up, b * up);
+  return pack2<T>(a, b);
+}
+
 // Largest raw score of this thread's row of S (BN TMEM columns from
 // s_addr); with MASK, columns j >= lim do not count.
 template <bool MASK, int BN>
@@ -180,10 +193,11 @@ __device__ __forceinline__ float pf_row_max(uint32_t s_addr, int lim) {
 }
 
 // P = 2^(S * sl2 + nm) of this thread's row into the chunk-major P tile
-// (row `row` of PF_ROWS, BN columns), masked columns 0; returns the row's sum
-// of P (fp32, before rounding to T).
+// (row `row` of PF_ROWS, BN columns; f16 times `up`), masked columns 0; returns
+// the row's sum of P (fp32, before rounding to T).
 template <bool MASK, int BN, typename T>
-__device__ __forceinline__ float pf_emit(uint32_t s_addr, unsigned char* sP, int row, float sl2, float nm, int lim) {
+__device__ __forceinline__ float pf_emit(uint32_t s_addr, unsigned char* sP, int row, float sl2, float nm, int lim,
+                                         float up) {
   float s0 = 0.f, s1 = 0.f;
 #pragma unroll
   for (int c = 0; c < BN / 32; ++c) {
@@ -202,7 +216,7 @@ __device__ __forceinline__ float pf_emit(uint32_t s_addr, unsigned char* sP, int
         }
         s0 += e0;
         s1 += e1;
-        w[h] = pack2<T>(e0, e1);
+        w[h] = pf_pack<T>(e0, e1, up);
       }
       *reinterpret_cast<uint4*>(sP + sw128_off(row, c * 32 + j8 * 8, PF_ROWS)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -228,7 +242,7 @@ __device__ __forceinline__ float pf_max_regs(const float (&va)[32], const float 
 // P column block and x7 its swizzle key (row % 8).
 template <bool MASK, typename T>
 __device__ __forceinline__ float pf_emit_regs(const float (&v)[32], int c, unsigned char* sP, uint32_t rowp, int x7,
-                                              float sl2, float nm, int lim) {
+                                              float sl2, float nm, int lim, float up) {
   float2 acc = make_float2(0.f, 0.f);
   const float2 sl = make_float2(sl2, sl2), nn = make_float2(nm, nm);
 #pragma unroll
@@ -244,7 +258,7 @@ __device__ __forceinline__ float pf_emit_regs(const float (&v)[32], int c, unsig
         e.y = c * 32 + j + 1 < lim ? e.y : 0.f;
       }
       acc = __fadd2_rn(acc, e);
-      w[h] = pack2<T>(e.x, e.y);
+      w[h] = pf_pack<T>(e.x, e.y, up);
     }
     const int col = c * 32 + j8 * 8;   // chunk (col % 64) / 8 of column block col / 64
     *reinterpret_cast<uint4*>(sP + (col >> 6) * PF_ROWS * 128 + rowp + ((((col & 63) >> 3) ^ x7) << 4)) =
@@ -357,7 +371,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_prefill_attn(const __grid_con
     const uint32_t s_addr = tmem + lane_sel + (uint32_t)(q * 128);
     const uint32_t o_addr = tmem + lane_sel + (uint32_t)(256 + q * 128);
     unsigned char* sPq = sP + q * PG::P_BYTES;
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = -INFINITY, l_run = 0.f, up = 1.f;
     bool ok = true;
     for (int kt = 0; kt < n_kt_q[q]; ++kt) {
       if (!pf_wait_warp(&s_full[q], (unsigned)(kt & 1), abort_flag)) { ok = false; break; }
@@ -380,6 +394,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_prefill_attn(const __grid_con
       const bool grow = mt > m_run + 8.f;
       const float m_new = grow ? mt : m_run;
       const float f = grow ? pf_ex2(m_run - m_new) : 1.f;   // 0 on the first tile
+      float fo = f;                                         // of O, which follows its weights' factor
+      if constexpr (std::is_same<T, __half>::value) {
+        const float was = up;
+        if (grow) up = fabsf(m_new) < PF_UP_MAX ? PF_UP : 1.f;
+        fo = f * (up * (was == 1.f ? 1.f : 1.f / PF_UP));
+      }
       // O_q was last written by P V of the previous tile, which completed
       // before S of this one (one issuing thread, in order)
       if (kt > 0 && __any_sync(0xffffffffu, grow)) {
@@ -388,7 +408,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_prefill_attn(const __grid_con
           float o[32];
           tmem_ld32(o_addr + c * 32, o);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] *= f;
+          for (int j = 0; j < 32; ++j) o[j] *= fo;
           tmem_st32(o_addr + c * 32, o);
         }
       }
@@ -396,13 +416,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_prefill_attn(const __grid_con
       float ls;
       if constexpr (BN == 64) {
         const uint32_t rowp = (uint32_t)((row >> 3) * 1024 + (row & 7) * 128);
-        ls = masked ? pf_emit_regs<true, T>(va, 0, sPq, rowp, row & 7, p.scale_log2, -m_run, lim) +
-                          pf_emit_regs<true, T>(vb, 1, sPq, rowp, row & 7, p.scale_log2, -m_run, lim)
-                    : pf_emit_regs<false, T>(va, 0, sPq, rowp, row & 7, p.scale_log2, -m_run, lim) +
-                          pf_emit_regs<false, T>(vb, 1, sPq, rowp, row & 7, p.scale_log2, -m_run, lim);
+        ls = masked ? pf_emit_regs<true, T>(va, 0, sPq, rowp, row & 7, p.scale_log2, -m_run, lim, up) +
+                          pf_emit_regs<true, T>(vb, 1, sPq, rowp, row & 7, p.scale_log2, -m_run, lim, up)
+                    : pf_emit_regs<false, T>(va, 0, sPq, rowp, row & 7, p.scale_log2, -m_run, lim, up) +
+                          pf_emit_regs<false, T>(vb, 1, sPq, rowp, row & 7, p.scale_log2, -m_run, lim, up);
       } else {
-        ls = masked ? pf_emit<true, BN, T>(s_addr, sPq, row, p.scale_log2, -m_run, lim)
-                    : pf_emit<false, BN, T>(s_addr, sPq, row, p.scale_log2, -m_run, lim);
+        ls = masked ? pf_emit<true, BN, T>(s_addr, sPq, row, p.scale_log2, -m_run, lim, up)
+                    : pf_emit<false, BN, T>(s_addr, sPq, row, p.scale_log2, -m_run, lim, up);
       }
       l_run = l_run * f + ls;
       fence_async_smem();
@@ -415,7 +435,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) k_prefill_attn(const __grid_con
         give_up();
       } else {
         tc_fence_after();
-        const float inv = 1.f / l_run;
+        const float inv = 1.f / l_run * (up == 1.f ? 1.f : 1.f / PF_UP);
         const bool row_ok = base + row < p.Sq;
         T* og = reinterpret_cast<T*>(p.out) + b * p.osb + hq * p.osh + (int64_t)(base + row) * p.oss;
 #pragma unroll
