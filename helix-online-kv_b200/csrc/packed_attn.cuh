@@ -54,13 +54,14 @@
 // only a value that is not finite shows, at queries up to 2 TT + 126 tokens ahead.
 //
 // What bounds it (B200, 32 query / 8 KV heads of 128 dims, bf16): prompts by a
-// slot's chain of scores, softmax and products, 3,300 cycles a two-tile step
-// against 2,048 of products, and at 16K tokens by the board's power (1.71 ms =
-// 1,285 TFLOP/s cool, 1,107 at the 1,000 W cap); single tokens by memory (8 at
-// 16K keys: 92 us, 5.8 TB/s of K and V); short calls by latency, 4.5 us to the
-// first scores.  Rolled loops and one copy of each role's code are deliberate:
-// with unrolled roles (20 KB more) the instruction cache missed 20 % of its
-// requests and ragged prompts took 240 us instead of 160.
+// slot's chain of scores, softmax and products, 3,500 cycles a two-tile step
+// (fitted over 1 to 4 items of 8 to 64 key tiles a CTA) against 2,048 of
+// products, and at 16K tokens by the board's power (1.83 ms = 1,200 TFLOP/s in a
+// graph, 2.02 = 1,091 called in turn); single tokens by memory (8 at 16K keys: 94
+// us, 5.7 TB/s of K and V); short calls by latency, 12 us besides the steps.
+// Rolled loops and one copy of each role's code are deliberate: with unrolled
+// roles (20 KB more) the instruction cache missed 20 % of its requests and ragged
+// prompts took 240 us, against 184 when the roles were made compact (160 now).
 #pragma once
 #include "packed_schedule.cuh"
 #include "prefill.cuh"

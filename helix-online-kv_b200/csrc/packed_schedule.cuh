@@ -26,7 +26,8 @@ namespace hokv {
 
 constexpr int PA_BN = 128;          // keys of a tile
 constexpr int PA_ITEM = 512;        // units of an item besides its keys (start, epilogue, half an unseen
-                                    // key tile; 448: 16K prompt 1,727 us, 512: 1,711, 576: the same, single tokens 1 % slower)
+                                    // key tile; in turns on one box, 448: 16K prompt 1 % slower, 576: the same and single
+                                    // tokens 1 % slower)
 // An item up to this (8 one-tile key tiles) is not cut: one token at 300 keys takes 11 us whole, 18 in pieces, 8 at
 // 700 keys 17 and 20; at 1,000 keys both take 18.
 constexpr int PA_WHOLE = 1536;

@@ -227,7 +227,8 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
  * f16/bf16, head_dim a multiple of 8 up to 128, up to 128 query heads per KV
  * head, scale > 0, strides multiples of 8 elements, 16-byte aligned pointers.
  * fp32 sums; the softmax weights are rounded to the input type before the
- * second product.  Keys that a causal mask hides from a query never reach it;
+ * second product: half a step of each, and f16 weights below 2^-25 of a row's
+ * largest to 2^-36 of it.  Keys that a causal mask hides from a query never reach it;
  * a non-finite value that the mask hides may (as 0 x NaN), from up to W + 126
  * tokens ahead of it, W = 2 floor(128 / (q_heads / kv_heads)).  Results are the
  * same on every run (no atomics on them).  The workspace needs no
