@@ -242,5 +242,5 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     with n keys and m queries sits at position n - m + i; a query that sees no key gives zeros.  f16/bf16, head
     dims in multiples of 8 up to 128, contiguous head dims, strides in multiples of 8 elements, H_q a multiple of
     H_kv.  -> [T, H_q, D] in the query's dtype; rows behind the last sequence are zeros, or left as they were in a
-    given ``out`` (which must not overlap the inputs)."""
+    given ``out`` (whose rows overlap neither each other nor the inputs)."""
     return _packed("packed_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)

@@ -210,7 +210,8 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
  * (compressed_cache.py:72-105).
  *
  * q and out [n_tokens, q_heads, head_dim], element strides (token, head), the
- * head dim contiguous; q's token stride covers its heads.  cu_seqlens_q
+ * head dim contiguous; q's token stride covers its heads, out's rows overlap
+ * neither each other nor the inputs.  cu_seqlens_q
  * [n_seqs + 1] or NULL (one token per sequence, n_tokens = n_seqs).  Keys and
  * values either packed (kv_in_slots = 0: [kv_rows, kv_heads, head_dim],
  * cu_seqlens_k [n_seqs + 1]) or in slots (kv_in_slots = 1: [n_seqs, kv_heads,

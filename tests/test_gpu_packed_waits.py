@@ -61,6 +61,26 @@ def run_out():
             L.device_status()
 
 
+def run_out_in_long_items():
+    """Hundreds of key tiles an item: a CTA that gave up does not wait for each of them again."""
+    import time
+
+    import torch
+
+    from helix_online_kv import _lib as L
+    from helix_online_kv.prefill import packed_attention
+    query, k, v, kl = _batch(torch, [6 << 20], 4, 1)
+    call = lambda: packed_attention(query, k, v, kv_len=kl)   # noqa: E731
+    want = call()
+    torch.cuda.synchronize()
+    for what in (WEIGHTS, END):
+        t = time.time()
+        _held(L, what, call)
+        assert time.time() - t < 5
+        assert torch.equal(call(), want)
+    L.device_status()
+
+
 def replay():
     """A captured call whose waits run out, marks of some pieces left behind; its replays on new data, at once and after
     more failures, and a graph captured before in the same pool are right."""
@@ -110,6 +130,11 @@ def test_waits_that_run_out_are_reported_and_the_next_call_is_right():
 
 
 @pytest.mark.gpu
+def test_waits_that_run_out_in_long_items():
+    _child("run_out_in_long_items")
+
+
+@pytest.mark.gpu
 def test_replays_after_a_failed_one_do_not_take_its_marks():
     _child("replay")
 
@@ -123,4 +148,4 @@ def test_the_product_keeps_nothing_back():
 
 if __name__ == "__main__":
     sys.path.insert(0, os.path.join(os.path.dirname(HERE), "helix-online-kv_b200"))
-    {f.__name__: f for f in (run_out, replay)}[sys.argv[1]]()
+    {f.__name__: f for f in (run_out, run_out_in_long_items, replay)}[sys.argv[1]]()
