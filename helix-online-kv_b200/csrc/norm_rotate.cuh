@@ -67,9 +67,15 @@ struct NraTok {
 __device__ __forceinline__ NraTok nra_token(const NraP& p, int t) {
   NraTok r;
   int b, i = 0;
+  bool bad = false;   // a negative start
   if (p.cu) {
     b = nra_sequence(p.cu, p.n_seqs, t);
-    if (b < p.n_seqs) i = t - p.cu[b];
+    if (b < p.n_seqs) {
+      const int start = p.cu[b];
+      i = t - start;
+      bad = start < 0;
+      if (b == 0 && i < 0) b = p.n_seqs;   // ahead of the first sequence
+    }
   } else {
     b = t;
   }
@@ -79,7 +85,7 @@ __device__ __forceinline__ NraTok nra_token(const NraP& p, int t) {
   if (r.b >= 0) {
     const int n = p.kv_len[b];
     r.row = n + i;
-    r.keep = n >= 0 && i >= 0 && (int64_t)n + i < p.cap;
+    r.keep = !bad && n >= 0 && i >= 0 && (int64_t)n + i < p.cap;
     if (!r.keep) dev_flag(HOKV_ERR_DEVICE_INPUT);
     r.pos = p.pos ? p.pos[t] : r.row;
   }

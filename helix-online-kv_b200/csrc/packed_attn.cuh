@@ -678,10 +678,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) k_packed_attn(const __grid_cons
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // the last rows are written
-    if (p.zero_tail) {   // rows behind the last sequence of an output this call allocated
+    if (p.zero_tail) {   // rows ahead of the first sequence and behind the last, of an output this call allocated
       // no 64-bit division: it is a call, for which registers of the whole kernel were spilled (prompts 1 to 2 % slower)
+      const int first = pa_first(p), owned = pa_used(p) - first;
 #pragma unroll 1
-      for (int t = pa_used(p) + (int)blockIdx.x; t < p.T; t += (int)gridDim.x) {
+      for (int i = (int)blockIdx.x; i < p.T - owned; i += (int)gridDim.x) {
+        const int64_t t = i < first ? i : i + owned;
 #pragma unroll 1
         for (int e = tid; e < p.Hq * (p.D / 8); e += 256) {
           const int h = e / (p.D / 8);
@@ -1040,7 +1042,7 @@ __global__ void __launch_bounds__(256) k_packed_combine_rows(const PaP p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int t = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane % PA_JOIN, g = blockIdx.z * PA_JOIN + r, hq = hk * p.G + min(g, p.G - 1);
-  if (t >= pa_used(p)) return;
+  if (t < pa_first(p) || t >= pa_used(p)) return;
   int first[2], n[2], prow[2];   // own keys, prefix
 #pragma unroll
   for (int src = 0; src < 2; ++src) {

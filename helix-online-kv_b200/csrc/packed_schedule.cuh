@@ -64,7 +64,8 @@ HD int64_t pa_min(int64_t a, int64_t b) { return a < b ? a : b; }
 HD int64_t pa_max(int64_t a, int64_t b) { return a > b ? a : b; }
 
 HD int pa_n_seqs(const PaSched& p) { return p.n_seqs + (p.prefix > 0 ? 1 : 0); }
-// Query tokens that belong to a sequence.
+// The query tokens [first, used) belong to the sequences.
+HD int pa_first(const PaSched& p) { return p.cu_q && p.n_seqs > 0 ? (int)pa_min(pa_max(p.cu_q[0], 0), p.T) : 0; }
 HD int pa_used(const PaSched& p) {
   if (!p.cu_q || p.n_seqs == 0) return p.n_seqs;
   return (int)pa_min(pa_max(p.cu_q[p.n_seqs], 0), p.T);
@@ -78,8 +79,9 @@ HD PaSeq pa_seq(const PaSched& p, int s) {
   r.bad = 0;
   if (p.prefix > 0) {
     if (s == 0) {
-      r.q0 = r.row0 = r.slot = 0;
-      r.nq = pa_used(p);
+      r.row0 = r.slot = 0;
+      r.q0 = pa_first(p);
+      r.nq = (int)pa_max(pa_used(p) - r.q0, 0);
       r.kv = p.prefix;
       r.src = 1;
       r.causal = 0;
@@ -88,7 +90,7 @@ HD PaSeq pa_seq(const PaSched& p, int s) {
     s -= 1;
   }
   const int a = p.cu_q ? p.cu_q[s] : s, e = p.cu_q ? p.cu_q[s + 1] : s + 1;
-  bool bad = a < 0 || e < a || e > p.T || (s == 0 && a > 0);   // tokens ahead of the first one would belong to none
+  bool bad = a < 0 || e < a || e > p.T;
   r.src = 0;
   r.causal = p.causal;
   if (p.cu_k) {

@@ -235,12 +235,12 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(query key^T * scaling [causal]) value for every sequence of a packed batch.
 
-    query [T, H_q, D]: sequence b owns tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]), the first start being 0
-    (without cu_seqlens_q, token b).  key/value either packed [S, H_kv, D] with cu_seqlens_k [B + 1] (default: cu_seqlens_q) or in slots [B,
+    query [T, H_q, D]: sequence b owns tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (without cu_seqlens_q, token
+    b).  key/value either packed [S, H_kv, D] with cu_seqlens_k [B + 1] (default: cu_seqlens_q) or in slots [B,
     H_kv, capacity, D] with kv_len [B], the keys each sequence holds, its new tokens included (a slot's rows behind
     kv_len are not used).  Lengths are int32 CUDA vectors and stay on the device.  Causal: query i of a sequence
     with n keys and m queries sits at position n - m + i; a query that sees no key gives zeros.  f16/bf16, head
     dims in multiples of 8 up to 128, contiguous head dims, strides in multiples of 8 elements, H_q a multiple of
-    H_kv.  -> [T, H_q, D] in the query's dtype; rows behind the last sequence are zeros, or left as they were in a
-    given ``out`` (whose rows overlap neither each other nor the inputs)."""
+    H_kv.  -> [T, H_q, D] in the query's dtype; rows of no sequence (ahead of the first, behind the last) are zeros,
+    or left as they were in a given ``out`` (whose rows overlap neither each other nor the inputs)."""
     return _packed("packed_attention", query, key, value, cu_seqlens_q, cu_seqlens_k, kv_len, scaling, is_causal, out)

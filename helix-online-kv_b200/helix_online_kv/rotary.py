@@ -88,14 +88,14 @@ def norm_rotate_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     """Rotated queries [T, H_q, D]; keys and values appended to their slots.
 
     query [T, H_q, D], key/value [T, H_kv, D] (contiguous head dims, any other strides: parts of one projection are
-    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]), the first start being 0 (None: token b).  Token i of b sits at
+    fine); sequence b owns tokens [cu_seqlens[b], cu_seqlens[b + 1]) (cu_seqlens None: token b).  Token i of b sits at
     position kv_len[b] + i, or positions[t] when given (sequences behind a shared prefix), and its key and value go to
     row kv_len[b] + i of key_slots/value_slots [B, H_kv, capacity, D].  kv_len (the rows held before the call) is
     not changed.  With q_weight / k_weight [D] the head is first multiplied by weight / sqrt(mean(x^2) + eps).
     inv_freq [F] float32, 2F <= D, turns dims (f, f + F), or (2f, 2f + 1) when ``interleaved``, by position *
     inv_freq[f]; the dims behind 2F keep their values.  f16, bf16 or f32, the same for all but lengths and inv_freq;
-    even head dims up to 256.  ``out`` may be the query itself; rows behind the last sequence are zeros, or left
-    as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
+    even head dims up to 256.  ``out`` may be the query itself; rows of no sequence (ahead of the first,
+    behind the last) are zeros, or left as they were in a given ``out``.  A row that does not fit its slot is reported by the device status."""
     eps, interleaved = float(eps), bool(interleaved)   # values, not objects: a tensor may change behind its identity
     sig = L.signature
     geometry = (sig(query), sig(key), sig(value), sig(key_slots), sig(value_slots), sig(kv_len), sig(inv_freq), eps,

@@ -219,11 +219,10 @@ int hokv_prefill_attention(const void* q, const void* k, const void* v, void* ou
  * whatever they hold); strides that nest, as hokv_prefill_attention.  The
  * prefix is [kv_heads, prefix_len, head_dim].  Lengths are device int32:
  * nothing is read back, so a call can be captured into a graph and replayed
- * with new lengths.  Lengths that do not fit the tensors, and a first start
- * cu_seqlens_q[0] that is not 0, set HOKV_ERR_DEVICE_INPUT in the device status
- * and leave that sequence's rows of out (and those ahead of the first one)
- * unspecified.  Rows of out behind cu_seqlens_q[n_seqs] are left as
- * they are (zero_tail = 0) or zeroed (1).
+ * with new lengths.  Lengths that do not fit the tensors set
+ * HOKV_ERR_DEVICE_INPUT in the device status and leave that sequence's rows
+ * of out unspecified.  Rows of out ahead of cu_seqlens_q[0] and from
+ * cu_seqlens_q[n_seqs] on are left as they are (zero_tail = 0) or zeroed (1).
  *
  * f16/bf16, head_dim a multiple of 8 up to 128, up to 128 query heads per KV
  * head, scale > 0, strides multiples of 8 elements, 16-byte aligned pointers.
@@ -269,10 +268,9 @@ int hokv_packed_attention(const hokv_packed_args* a, void* stream);
  * (layer_state.py:68-133).  f16, bf16 or f32 throughout (weights too;
  * inv_freq f32), element strides, head dims contiguous, even head_dim up to
  * 256; fp32 arithmetic, rounded once.  `out` may be q itself.  A row that does
- * not fit its slot is not written and sets HOKV_ERR_DEVICE_INPUT; so do tokens
- * ahead of a cu_seqlens[0] that is not 0, whose rows of out are unspecified.  Tokens
- * behind the last sequence append nothing; their rows of `out` are left as
- * they are (zero_tail = 0) or zeroed (1). */
+ * not fit its slot is not written and sets HOKV_ERR_DEVICE_INPUT.  Tokens
+ * of no sequence (ahead of the first, behind the last) append nothing; their
+ * rows of `out` are left as they are (zero_tail = 0) or zeroed (1). */
 typedef struct hokv_norm_rotate_args {
   int dtype, n_seqs, q_heads, kv_heads, head_dim, n_freq, interleaved, zero_tail;
   float eps;

@@ -116,34 +116,43 @@ def test_scores_of_any_finite_size(dtype, rising):
 
 
 @pytest.mark.parametrize("kind", ["packed", "prefix", "append"])
-def test_starts_that_do_not_begin_at_the_first_token_are_reported(kind):
-    """Rows ahead of the first sequence would belong to none; the sequences behind the first one stay right, and so do
-    later calls."""
+def test_tokens_ahead_of_the_first_sequence(kind):
+    """Starts that do not begin at 0: the sequences' rows are those of the batch without the tokens ahead, which get
+    zeros, or keep a given out, and append nothing; a negative start is reported."""
     from helix_online_kv import _lib as L
     from helix_online_kv.prefill import packed_attention
     from helix_online_kv.rotary import norm_rotate_append
     from helix_online_kv.shared_prefix import shared_prefix_attention
     g = _gen(3)
     x = lambda *s: torch.randn(s, generator=g, device="cuda").to(F16)   # noqa: E731
-    query, key, k, v, pk, pv = x(9, 4, 64), x(9, 2, 64), x(2, 2, 20, 64), x(2, 2, 20, 64), x(2, 300, 64), x(2, 300, 64)
-    kl, f = torch.tensor([8, 9], dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+    T, ahead, q, kv = 400, 150, [130, 0, 70], [1000, 20, 300]
+    query, key = x(T, 4, 64), x(T, 2, 64)
+    k, v, pk, pv = x(3, 2, 1100, 64), x(3, 2, 1100, 64), x(2, 3000, 64), x(2, 3000, 64)
+    kl, f = torch.tensor(kv, dtype=torch.int32, device="cuda"), torch.rand(32, generator=g, device="cuda")
 
-    def call(cu):
+    def call(query, key, cu, out=None):
         if kind == "packed":
-            return packed_attention(query, k, v, cu, kv_len=kl)
+            return packed_attention(query, k, v, cu, kv_len=kl, out=out), ()
         if kind == "prefix":
-            return shared_prefix_attention(query, pk, pv, k, v, kl, cu)
-        return norm_rotate_append(query, key, key, k, v, cu, kl, f)
+            return shared_prefix_attention(query, pk, pv, k, v, kl, cu, out=out), ()
+        slots = torch.full_like(k, 3.0), torch.full_like(v, 3.0)
+        return norm_rotate_append(query, key, key, *slots, cu, kl - torch.tensor(q, device="cuda", dtype=torch.int32), f, out=out), slots
 
-    good = call(lens_tensor([4, 5]))
-    cu = torch.tensor([2, 4, 9], dtype=torch.int32, device="cuda")
-    out = call(cu)
+    want, kept = call(query[ahead:], key[ahead:], lens_tensor(q))
+    cu = lens_tensor(q) + ahead
+    out, slots = call(query, key, cu)
+    end = ahead + sum(q)
+    assert torch.equal(out[ahead:end], want[:sum(q)]) and not out[:ahead].any() and not out[end:].any()
+    assert all(torch.equal(a, b) for a, b in zip(slots, kept))
+    out, slots = call(query, key, cu, torch.full_like(query, 5.0))
+    assert torch.equal(out[ahead:end], want[:sum(q)]) and (out[:ahead] == 5).all() and (out[end:] == 5).all()
+    assert all(torch.equal(a, b) for a, b in zip(slots, kept))
+    L.device_status()
+    cu[0] = -1
+    call(query, key, cu)
     with pytest.raises(L.HokvError) as e:
         L.device_status()
     assert e.value.status == L.ERR_DEVICE_INPUT
-    assert torch.equal(out[4:], good[4:])
-    assert torch.equal(call(lens_tensor([4, 5])), good)
-    L.device_status()
 
 
 def test_keys_may_start_behind_the_first_row():

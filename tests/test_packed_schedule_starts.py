@@ -1,5 +1,5 @@
-"""The packed attention's schedule (packed_schedule.cuh) built for the host: where
-the first sequence must start, and the search for the sequence and pair in which
+"""The packed attention's schedule (packed_schedule.cuh) built for the host: tokens
+ahead of the first sequence, and the search for the sequence and pair in which
 a CTA's share begins, the kernel's own code over 32 emulated lanes.  CPU only."""
 
 import bisect
@@ -23,17 +23,17 @@ def _items(lib, starts, kv, T, prefix=0):   # noqa: F811
     return {(int(r[5]), int(r[3])): int(r[4]) for r in out[:n]}   # (source, first token): tokens
 
 
-@pytest.mark.parametrize("first", [1, 3, -1])
-def test_a_batch_that_does_not_start_at_its_first_token(lib, first):   # noqa: F811
-    """Its first sequence gets no work, like any other whose lengths do not fit; the others get theirs."""
-    assert _items(lib, [0, 4, 9], [8, 8], 9) == {(0, 0): 4, (0, 4): 5}
-    assert _items(lib, [first, 4, 9], [8, 8], 9) == {(0, 4): 5}
-
-
-def test_no_sequence_owns_no_token(lib):   # noqa: F811
-    """A single start that is not 0 gives the prefix no rows."""
-    assert _items(lib, [0], [], 9, prefix=300) == {}
-    assert _items(lib, [5], [], 9, prefix=300) == {}
+@pytest.mark.parametrize("prefix", [0, 300])
+def test_tokens_ahead_of_the_first_sequence_have_no_work(lib, prefix):   # noqa: F811
+    """They belong to no sequence, and are no queries of a prefix."""
+    ahead = lambda n, m: {(1, n): m} if prefix else {}   # noqa: E731
+    assert _items(lib, [0, 4, 9], [8, 8], 9, prefix) == {**ahead(0, 9), (0, 0): 4, (0, 4): 5}
+    assert _items(lib, [3, 4, 9], [8, 8], 9, prefix) == {**ahead(3, 6), (0, 3): 1, (0, 4): 5}
+    assert _items(lib, [9, 9, 9], [8, 8], 9, prefix) == {}
+    assert _items(lib, [5], [], 9, prefix) == {}
+    # a start that no tensor has, or behind the end of the batch: no work for that sequence, none outside the tokens
+    assert _items(lib, [-1, 4, 9], [8, 8], 9, prefix) == {**ahead(0, 9), (0, 4): 5}
+    assert _items(lib, [20, 4, 9], [8, 8], 9, prefix) == {(0, 4): 5}
 
 
 # ---- the warp's search for where a share begins ------------------------------------
